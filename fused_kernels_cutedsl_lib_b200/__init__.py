@@ -20,6 +20,13 @@ from .gemm import (
     swiglu_gemm2,
     workspace_bytes,
 )
+from .w4 import W4Weight, pack_w4, quantize_w4, w4_linear
+from .cache_ops import (
+    alloc_cache_attention_workspace,
+    cache_attention,
+    cache_attention_workspace_bytes,
+    cache_evict,
+)
 from .prefill_attention import FlashSM90, flash_attention
 from .decoding_attention import (
     DAttn1,
@@ -52,6 +59,14 @@ __all__ = [
     "swiglu_gemm",
     "swiglu_gemm2",
     "workspace_bytes",
+    "W4Weight",
+    "pack_w4",
+    "quantize_w4",
+    "w4_linear",
+    "alloc_cache_attention_workspace",
+    "cache_attention",
+    "cache_attention_workspace_bytes",
+    "cache_evict",
     "FlashSM90",
     "flash_attention",
     "DAttn1",

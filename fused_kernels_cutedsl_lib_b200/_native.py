@@ -125,6 +125,24 @@ SIGNATURES: dict[str, tuple] = {
     ),
     "fk_rmsnorm_swiglu": (
         _c_int, [_p, _p, _p, _p, _c_int, _c_int, _c_int, _c_float, _p, ctypes.c_size_t, _p]),
+    "fk_w4_linear": (
+        _c_int,
+        [_p, ctypes.c_longlong, _p, _p, _p, _p, _c_int, _c_int, _c_int, _c_int, _c_int, _p],
+    ),
+    "fk_cache_attn_workspace_bytes": (
+        _c_int,
+        [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, ctypes.POINTER(ctypes.c_size_t)],
+    ),
+    "fk_cache_attn_fwd": (
+        _c_int,
+        [_p, ctypes.c_longlong, _p, _p, _p, _p, _p, _p, ctypes.c_longlong, _p, _p, _c_int, _c_int, _c_int, _c_int,
+         _c_int, _c_int, _c_int, _c_int, _c_float, _p, ctypes.c_size_t, _p],
+    ),
+    "fk_cache_evict": (
+        _c_int,
+        [_p, _p, _p, _p, _p, ctypes.c_longlong, _p, _p, _p, _p, _p, ctypes.c_longlong, _p, _c_int, _c_int, _c_int,
+         _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _p],
+    ),
 }
 
 _lock = threading.Lock()

@@ -1,0 +1,653 @@
+// Attention of one new token per sequence over a contiguous or paged KV cache,
+// optionally adding every cached token's attention weight to its running mass
+// (what cache_evict.cu selects by).
+//
+//   s_j = scale * q . k_j,  w_j = exp(s_j - lse),  lse = log sum_{j < len} exp(s_j)
+//   out = sum_j w_j v_j,    mass_out[j] = mass[j] + sum over the group's q heads of w_j
+//
+// Bound: HBM, 4 * D bytes per (token, kv head), plus 8 bytes of mass and the
+// scores' round trip described below.
+//
+// Pass 1 (`attend_kernel`): a persistent grid walks units (row b, kv head h,
+// split of `chunk` tokens). Four warps each take 16 tokens of every 64-token
+// tile and own a private ring of K/V stages filled by their own 16-byte
+// cp.async copies, so no barrier is needed inside a unit, and each token's
+// address comes from its own page: pages may have any size. The load side runs
+// STAGES - 1 tiles ahead of the arithmetic, across units. Tokens are the M side
+// of mma.sync m16n8k16 and the group's query heads the N side (NT tiles of 8),
+// so a K/V byte is read once for all heads that share it. Each warp keeps its
+// own running maximum and sum (fp32, log2 domain); the four are merged at the
+// end of a unit. P is multiplied as a sum of two 16-bit numbers (its rounding and
+// the rounding of the rest): the products cost nothing next to the loads, and the
+// output's error is then that of its own rounding instead of sqrt(2) times it.
+// With a mass, the raw log2-domain scores go to scratch as fp32 (4 bytes per
+// token and q head), because a token's weight is known only with the lse of the
+// whole row.
+//
+// Pass 2 (`finish_kernel`, a programmatic dependent): blocks that merge the
+// splits of each (row, q head) into out and lse, and blocks that turn a stretch
+// of scores into weights and add them to the mass.
+//
+// A row of length 0 gives out = 0, lse = -inf and leaves its mass. A page id
+// outside the pool reads as zero rows, as a TMA load outside its tensor does.
+#include <cuda_fp16.h>
+#include <math.h>
+
+#include "common.cuh"
+#include "fk_b200.h"
+
+namespace fk {
+namespace cattn {
+
+constexpr int T = 64;   // tokens per tile
+constexpr int NW = 4;   // warps, 16 tokens of a tile each
+constexpr int kThreads = NW * 32;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.69314718055994531f;
+
+struct Params {
+  const void* q;            // row b at q + b * q_stride: [Hq, D]
+  long long q_stride;
+  const void* k;            // [B, Lmax, Hkv, D] or [num_blocks, block_size, Hkv, D]
+  const void* v;
+  const int* block_table;   // [B, max_blocks] or null
+  int max_blocks, block_size, num_blocks;
+  const int* seqlens;
+  float* o_part;            // [S, B, Hq, D], normalised per split
+  float* lse_part;          // [S, B, Hq], log2 domain
+  float* scores;            // [B * Hkv, Lmax, gs] log2-domain scores, or null
+  int gs;                   // floats per token in scores
+  const float* mass_in;     // [B, Hkv, mass_cap]
+  float* mass_out;
+  long long mass_cap;
+  void* out;                // [B, Hq, D]
+  float* lse;               // [B, Hq]
+  int B, Lmax, Hq, Hkv, G, chunk;
+  float scale_log2;
+};
+
+template <typename E>
+struct Elem;
+template <>
+struct Elem<__nv_bfloat16> {
+  static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
+  static __device__ __forceinline__ float lo(uint32_t v) { return __uint_as_float(v << 16); }
+  static __device__ __forceinline__ float hi(uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); }
+  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    mma_bf16_16816(d, a, b0, b1);
+  }
+};
+template <>
+struct Elem<__half> {
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ float lo(uint32_t v) {
+    return __half2float(__ushort_as_half((unsigned short)(v & 0xFFFFu)));
+  }
+  static __device__ __forceinline__ float hi(uint32_t v) {
+    return __half2float(__ushort_as_half((unsigned short)(v >> 16)));
+  }
+  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    mma_f16_16816(d, a, b0, b1);
+  }
+};
+
+__device__ __forceinline__ int seq_len(const Params& p, int b) {
+  const int L = __ldg(p.seqlens + b);
+  return min(max(L, 0), p.Lmax);
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+  const int n = valid ? 16 : 0;  // 0: the 16 bytes are zero-filled and src is not read
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Transposes an 8x8 matrix of 16-bit values held one 2-value row piece per lane.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+// The tiles a CTA works on, in order: units (b, h, split) dealt round-robin over
+// the grid, and the 64-token tiles of each.
+struct TileIter {
+  long long u, base;  // current unit, first unit of row b
+  int b, nb, len;     // row, its splits and length
+  int h, s;           // kv head and split of the unit
+  int t, t1;          // current tile's first token, end of the unit
+  bool valid;
+  __device__ __forceinline__ void row(const Params& p) {
+    len = seq_len(p, b);
+    nb = (len + p.chunk - 1) / p.chunk;
+  }
+  __device__ __forceinline__ void locate(const Params& p) {
+    while (true) {
+      const long long cnt = (long long)nb * p.Hkv;
+      if (u < base + cnt) break;
+      base += cnt;
+      if (++b >= p.B) {
+        valid = false;
+        return;
+      }
+      row(p);
+    }
+    const int r = (int)(u - base);
+    h = r / nb;
+    s = r - h * nb;
+    t = s * p.chunk;
+    t1 = min(t + p.chunk, len);
+  }
+  __device__ __forceinline__ void init(const Params& p) {
+    u = blockIdx.x;
+    base = 0;
+    b = 0;
+    valid = true;
+    row(p);
+    locate(p);
+  }
+  __device__ __forceinline__ void next(const Params& p) {
+    t += T;
+    if (t >= t1) {
+      u += gridDim.x;
+      locate(p);
+    }
+  }
+};
+
+template <int D>
+__host__ __device__ constexpr int stage_bytes() { return 2 * 16 * D * 2; }  // one warp's K and V of 16 tokens
+template <int D>
+__host__ __device__ constexpr int stages() { return D == 128 ? 3 : 5; }
+
+template <typename E, int D, int NT, bool MASS>
+__global__ void __launch_bounds__(kThreads, 2) attend_kernel(const Params p) {
+  using El = Elem<E>;
+  constexpr int S = stages<D>();
+  constexpr int HALVES = D / 64;  // 128-byte row halves of a tile row
+  constexpr int KS = D / 16;
+  constexpr int LPR = D / 8;      // lanes (16-byte pieces) per token row
+  constexpr int RPI = 32 / LPR;   // rows per copy instruction
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, c = lane & 3;
+  const int j = lane >> 3, r = lane & 7;
+  const int tw = warp * 16;
+  const float NEG_INF = -INFINITY;
+  const int G = p.G;
+  const uint32_t ring = smem_u32(smem) + warp * S * stage_bytes<D>();
+  float* cm = reinterpret_cast<float*>(smem + NW * S * stage_bytes<D>());  // [NW][NT * 8] row max
+  float* cl = cm + NW * NT * 8;                                            // [NW][NT * 8] row sum
+  float* co = cl + NW * NT * 8;                                            // [NW][G][D]
+
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  TileIter ld, it;
+  ld.init(p);
+  it = ld;
+
+  // Lanes 0..15 resolve the cache row of "their" token of the next tile to load
+  // one tile ahead, so the page lookup's latency is off the copies' path.
+  auto resolve = [&]() -> int {
+    if (!ld.valid) return -1;
+    const int t = ld.t + tw + (lane & 15);
+    if (t >= ld.t1) return -1;
+    if (p.block_table == nullptr) return ld.b * p.Lmax + t;
+    const int page = __ldg(p.block_table + (size_t)ld.b * p.max_blocks + t / p.block_size);
+    if (page < 0 || page >= p.num_blocks) return -1;
+    return page * p.block_size + t % p.block_size;
+  };
+  int next_row = resolve();
+  int ld_stage = 0;
+  auto issue = [&]() {
+    if (ld.valid) {
+      const int row = next_row, h = ld.h;
+      ld.next(p);
+      next_row = resolve();
+      const uint32_t kd = ring + ld_stage * stage_bytes<D>();
+      const uint32_t vd = kd + 16 * D * 2;
+      const int piece = lane % LPR;
+      const uint32_t half_off = (piece >> 3) * (16 * 128);
+#pragma unroll
+      for (int i = 0; i < 16 / RPI; ++i) {
+        const int tok = i * RPI + lane / LPR;
+        const int rr = __shfl_sync(0xffffffffu, row, tok);
+        const size_t off = ((size_t)max(rr, 0) * p.Hkv + h) * D + piece * 8;
+        const uint32_t so = half_off + tok * 128 + (((piece ^ tok) & 7) << 4);
+        cp_async16(kd + so, static_cast<const E*>(p.k) + off, rr >= 0);
+        cp_async16(vd + so, static_cast<const E*>(p.v) + off, rr >= 0);
+      }
+      if (++ld_stage == S) ld_stage = 0;
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < S - 1; ++i) issue();
+
+  int stage = 0;
+  while (it.valid) {
+    const int b = it.b, h = it.h, t1 = it.t1, split = it.s;
+    // Q^T as the B operand: column n = query head of the group (zero past the group).
+    uint32_t qf[NT][KS][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int hh = nt * 8 + g;
+      const E* qrow = static_cast<const E*>(p.q) + (size_t)b * p.q_stride + ((size_t)h * G + hh) * D;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        qf[nt][ks][0] = hh < G ? __ldg(reinterpret_cast<const uint32_t*>(qrow + 16 * ks + 2 * c)) : 0u;
+        qf[nt][ks][1] = hh < G ? __ldg(reinterpret_cast<const uint32_t*>(qrow + 16 * ks + 8 + 2 * c)) : 0u;
+      }
+    }
+    float o[NT][KS][4];
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt][0] = m[nt][1] = NEG_INF;
+      l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < KS; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+    }
+
+    bool last;
+    do {
+      const int t = it.t;
+      cp_async_wait<S - 2>();
+      __syncwarp();  // every lane's copies of this stage are in, and the stage refilled below is free
+      issue();
+      const uint32_t kb = ring + stage * stage_bytes<D>();
+      const uint32_t vb = kb + 16 * D * 2;
+      if (++stage == S) stage = 0;
+
+      // S^T[16 tokens x 8 heads] = K[16 x D] . Q^T[D x 8]
+      float sc[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const int tok = (j & 1) * 8 + r;
+        const int cc = 2 * (ks & 3) + (j >> 1);
+        uint32_t a[4];
+        ldsm_x4(kb + (ks >> 2) * (16 * 128) + tok * 128 + (((cc ^ tok) & 7) << 4), a[0], a[1], a[2], a[3]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) El::mma(sc[nt], a, qf[nt][ks][0], qf[nt][ks][1]);
+      }
+
+      const int nv = t1 - (t + tw);  // valid tokens among this warp's 16
+      uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float x0 = sc[nt][0] * p.scale_log2, x1 = sc[nt][1] * p.scale_log2;
+        const float x2 = sc[nt][2] * p.scale_log2, x3 = sc[nt][3] * p.scale_log2;
+        if (MASS) {
+          const int h0 = nt * 8 + 2 * c;
+          float* dst = p.scores + (((size_t)b * p.Hkv + h) * p.Lmax + (t + tw + g)) * p.gs + h0;
+          if (p.gs > 1) {  // gs is even: a pair of heads per store
+            if (h0 < p.gs) {
+              if (g < nv) *reinterpret_cast<float2*>(dst) = make_float2(x0, x1);
+              if (g + 8 < nv) *reinterpret_cast<float2*>(dst + 8 * (size_t)p.gs) = make_float2(x2, x3);
+            }
+          } else if (h0 == 0) {
+            if (g < nv) dst[0] = x0;
+            if (g + 8 < nv) dst[8] = x2;
+          }
+        }
+        const float y0 = g < nv ? x0 : NEG_INF, y1 = g < nv ? x1 : NEG_INF;
+        const float y2 = g + 8 < nv ? x2 : NEG_INF, y3 = g + 8 < nv ? x3 : NEG_INF;
+        float mx0 = fmaxf(y0, y2), mx1 = fmaxf(y1, y3);
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) {
+          mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, off));
+          mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, off));
+        }
+        const float mn0 = fmaxf(m[nt][0], mx0), mn1 = fmaxf(m[nt][1], mx1);
+        const float sf0 = mn0 == NEG_INF ? 0.f : mn0;  // nothing but -inf so far
+        const float sf1 = mn1 == NEG_INF ? 0.f : mn1;
+        const float al0 = exp2f(m[nt][0] - sf0), al1 = exp2f(m[nt][1] - sf1);
+        const float p0 = exp2f(y0 - sf0), p1 = exp2f(y1 - sf1);
+        const float p2 = exp2f(y2 - sf0), p3 = exp2f(y3 - sf1);
+        l[nt][0] = l[nt][0] * al0 + (p0 + p2);
+        l[nt][1] = l[nt][1] * al1 + (p1 + p3);
+        m[nt][0] = mn0;
+        m[nt][1] = mn1;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          o[nt][i][0] *= al0;
+          o[nt][i][1] *= al1;
+          o[nt][i][2] *= al0;
+          o[nt][i][3] *= al1;
+        }
+        // P^T (rows = tokens) as the B operand (rows = tokens as k): two 8x8 transposes
+        // each for the rounded P and for what the rounding left.
+        const uint32_t h01 = El::pack(p0, p1), h23 = El::pack(p2, p3);
+        ph[nt][0] = transpose8x8(h01);
+        ph[nt][1] = transpose8x8(h23);
+        pl[nt][0] = transpose8x8(El::pack(p0 - El::lo(h01), p1 - El::hi(h01)));
+        pl[nt][1] = transpose8x8(El::pack(p2 - El::lo(h23), p3 - El::hi(h23)));
+      }
+
+      // O^T[D x 8 heads] += V^T[D x 16 tokens] . P^T[16 x 8]; rows past the end are zero-filled.
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        const int tok = (j >> 1) * 8 + r;
+        const int cc = 2 * (i & 3) + (j & 1);
+        uint32_t a[4];
+        ldsm_x4_t(vb + (i >> 2) * (16 * 128) + tok * 128 + (((cc ^ tok) & 7) << 4), a[0], a[1], a[2], a[3]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          El::mma(o[nt][i], a, ph[nt][0], ph[nt][1]);
+          El::mma(o[nt][i], a, pl[nt][0], pl[nt][1]);
+        }
+      }
+      last = t + T >= t1;
+      it.next(p);
+    } while (!last);
+
+    // ---- merge the four warps' softmax states and write the split's partial ----
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) {
+        l[nt][0] += __shfl_xor_sync(0xffffffffu, l[nt][0], off);
+        l[nt][1] += __shfl_xor_sync(0xffffffffu, l[nt][1], off);
+      }
+      const int h0 = nt * 8 + 2 * c;
+      if (g == 0) {
+        cm[warp * NT * 8 + h0] = m[nt][0];
+        cm[warp * NT * 8 + h0 + 1] = m[nt][1];
+        cl[warp * NT * 8 + h0] = l[nt][0];
+        cl[warp * NT * 8 + h0 + 1] = l[nt][1];
+      }
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        if (h0 < G) {
+          float* dst = co + ((size_t)warp * G + h0) * D + 16 * i + g;
+          dst[0] = o[nt][i][0];
+          dst[8] = o[nt][i][2];
+        }
+        if (h0 + 1 < G) {
+          float* dst = co + ((size_t)warp * G + h0 + 1) * D + 16 * i + g;
+          dst[0] = o[nt][i][1];
+          dst[8] = o[nt][i][3];
+        }
+      }
+    }
+    __syncthreads();
+    const size_t row0 = ((size_t)split * p.B + b) * p.Hq + (size_t)h * G;
+    for (int e = threadIdx.x; e < G * D; e += kThreads) {
+      const int hh = e / D, d = e % D;
+      float M = NEG_INF;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) M = fmaxf(M, cm[w * NT * 8 + hh]);
+      // fmaxf passes over NaN, the sums do not: NaN scores reach the output, and a
+      // sum of exactly 0 means that every score was -inf.
+      const float ms = M == NEG_INF ? 0.f : M;
+      float L = 0.f, acc = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float sw = exp2f(cm[w * NT * 8 + hh] - ms);
+        L += sw * cl[w * NT * 8 + hh];
+        acc += sw * co[((size_t)w * G + hh) * D + d];
+      }
+      p.o_part[(row0 + hh) * D + d] = L == 0.f ? 0.f : acc / L;
+      if (d == 0) p.lse_part[row0 + hh] = L == 0.f ? NEG_INF : M + log2f(L);
+    }
+    __syncthreads();
+  }
+  cp_async_wait<0>();
+}
+
+constexpr int kMassTokens = 2048;  // tokens per mass block
+
+// Blocks [0, merge_blocks): four (row, q head) pairs each, one per warp, merge the
+// splits. The others: one stretch of kMassTokens tokens of one (row, kv head).
+template <typename E, int D>
+__global__ void __launch_bounds__(128) finish_kernel(const Params p, int merge_blocks, int stretches) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const size_t plane = (size_t)p.B * p.Hq;
+  if ((int)blockIdx.x < merge_blocks) {
+    const int row = blockIdx.x * 4 + warp;
+    if (row >= p.B * p.Hq) return;
+    const int b = row / p.Hq;
+    const int n = (seq_len(p, b) + p.chunk - 1) / p.chunk;
+    constexpr int PER = D / 32;  // dims per lane
+    float M = -INFINITY;
+    for (int s = lane; s < n; s += 32) M = fmaxf(M, __ldg(p.lse_part + s * plane + row));
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+    const float ms = M == -INFINITY ? 0.f : M;
+    float W = 0.f, acc[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+    constexpr int CH = 8;  // splits whose loads are in flight together; summed in split order
+    for (int s0 = 0; s0 < n; s0 += CH) {
+      float ls[CH], v[CH][PER];
+#pragma unroll
+      for (int u = 0; u < CH; ++u) {
+        const bool in = s0 + u < n;
+        ls[u] = in ? __ldg(p.lse_part + (s0 + u) * plane + row) : -INFINITY;
+        const float* src = p.o_part + ((s0 + u) * plane + row) * D + PER * lane;
+        if constexpr (PER == 4) {
+          const float4 f = in ? __ldg(reinterpret_cast<const float4*>(src)) : make_float4(0.f, 0.f, 0.f, 0.f);
+          v[u][0] = f.x, v[u][1] = f.y, v[u][2] = f.z, v[u][3] = f.w;
+        } else {
+          const float2 f = in ? __ldg(reinterpret_cast<const float2*>(src)) : make_float2(0.f, 0.f);
+          v[u][0] = f.x, v[u][1] = f.y;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < CH; ++u) {
+        if (s0 + u < n) {
+          const float w = exp2f(ls[u] - ms);
+          W += w;
+#pragma unroll
+          for (int i = 0; i < PER; ++i) acc[i] += w * v[u][i];
+        }
+      }
+    }
+    const bool none = W == 0.f;
+    const float inv = none ? 0.f : 1.f / W;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<E*>(p.out) + (size_t)row * D + PER * lane);
+#pragma unroll
+    for (int i = 0; i < PER / 2; ++i) dst[i] = Elem<E>::pack(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+    if (lane == 0) p.lse[row] = none ? -INFINITY : (M + log2f(W)) * kLn2;
+    return;
+  }
+
+  __shared__ float s_lse[16];
+  const int i = blockIdx.x - merge_blocks;
+  const int pair = i / stretches;
+  const int t0 = (i - pair * stretches) * kMassTokens;
+  const int b = pair / p.Hkv, h = pair - b * p.Hkv;
+  const int len = seq_len(p, b);
+  if (t0 >= len) return;
+  const int n = (len + p.chunk - 1) / p.chunk;
+  for (int hh = warp; hh < p.G; hh += 4) {
+    const float* src = p.lse_part + (size_t)b * p.Hq + (size_t)h * p.G + hh;
+    float M = -INFINITY, W = 0.f;
+    for (int s = lane; s < n; s += 32) M = fmaxf(M, __ldg(src + s * plane));
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+    const float ms = M == -INFINITY ? 0.f : M;
+    for (int s = lane; s < n; s += 32) W += exp2f(__ldg(src + s * plane) - ms);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) W += __shfl_xor_sync(0xffffffffu, W, off);
+    // A head whose scores are all -inf gives no weight: +inf makes exp2(-inf - inf) = 0.
+    if (lane == 0) s_lse[hh] = W == 0.f ? INFINITY : M + log2f(W);
+  }
+  __syncthreads();
+  const float* sc = p.scores + (size_t)pair * p.Lmax * p.gs;
+  const size_t mrow = (size_t)pair * p.mass_cap;
+  const int t1 = min(t0 + kMassTokens, len);
+  for (int t = t0 + (int)threadIdx.x; t < t1; t += 128) {
+    float w = 0.f;
+    for (int hh = 0; hh < p.G; ++hh) w += exp2f(__ldg(sc + (size_t)t * p.gs + hh) - s_lse[hh]);
+    p.mass_out[mrow + t] = p.mass_in[mrow + t] + w;
+  }
+}
+
+static int chunk_tokens(int B, int Hkv, int Lmax) {
+  // The largest of 1024..64 tokens that still gives units for three quarters of the SMs.
+  int chunk = T;
+  const long long total = (long long)B * Lmax;
+  for (int cand = 1024; cand >= T; cand >>= 1) {
+    const long long units = (long long)Hkv * ((total + cand - 1) / cand);
+    if (4 * units >= 3LL * num_sms()) {
+      chunk = cand;
+      break;
+    }
+  }
+  return chunk;
+}
+
+static int score_stride(int G) { return G == 1 ? 1 : (G + 1) & ~1; }
+
+struct Layout {
+  int chunk, splits;
+  size_t o_bytes, lse_bytes, score_bytes;
+  size_t total() const { return o_bytes + lse_bytes + score_bytes; }
+};
+
+static size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
+
+static Layout layout(int B, int Lmax, int Hq, int Hkv, int D, bool mass) {
+  Layout w;
+  w.chunk = chunk_tokens(B, Hkv, Lmax);
+  w.splits = (Lmax + w.chunk - 1) / w.chunk;
+  const size_t rows = (size_t)w.splits * B * Hq;
+  w.o_bytes = round256(rows * D * 4);
+  w.lse_bytes = round256(rows * 4);
+  w.score_bytes = mass ? round256((size_t)B * Hkv * Lmax * score_stride(Hq / Hkv) * 4) : 0;
+  return w;
+}
+
+template <typename E, int D, int NT, bool MASS>
+static int launch_attend(const Params& p, cudaStream_t st) {
+  auto kern = attend_kernel<E, D, NT, MASS>;
+  const size_t smem = (size_t)NW * stages<D>() * stage_bytes<D>() + (size_t)(2 * NW * NT * 8 + NW * p.G * D) * 4;
+  FK_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  int occ = 0;
+  FK_CHECK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kern, kThreads, smem));
+  if (occ < 1) occ = 1;
+  long long grid = (long long)num_sms() * occ;
+  const long long units = (long long)p.B * p.Hkv * ((p.Lmax + p.chunk - 1) / p.chunk);
+  if (grid > units) grid = units;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid, 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  FK_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, p));
+  const int merge_blocks = (p.B * p.Hq + 3) / 4;
+  const int stretches = (p.Lmax + kMassTokens - 1) / kMassTokens;
+  const long long blocks = merge_blocks + (MASS ? (long long)p.B * p.Hkv * stretches : 0);
+  cfg.gridDim = dim3((unsigned)blocks, 1, 1);
+  cfg.dynamicSmemBytes = 0;
+  FK_CHECK_CUDA(cudaLaunchKernelEx(&cfg, finish_kernel<E, D>, p, merge_blocks, stretches));
+  return kOk;
+}
+
+template <typename E, int D>
+static int by_group(const Params& p, cudaStream_t st) {
+  const bool mass = p.mass_out != nullptr;
+  if (p.G <= 8) return mass ? launch_attend<E, D, 1, true>(p, st) : launch_attend<E, D, 1, false>(p, st);
+  return mass ? launch_attend<E, D, 2, true>(p, st) : launch_attend<E, D, 2, false>(p, st);
+}
+
+static int check_sizes(int B, int Lmax, int Hq, int Hkv, int D) {
+  FK_CHECK_ARG(B >= 1 && Lmax >= 1, "batch and max_seqlen must be >= 1");
+  FK_CHECK_ARG(D == 64 || D == 128, "head_dim must be 64 or 128");
+  FK_CHECK_ARG(Hkv >= 1 && Hq >= Hkv && Hq % Hkv == 0, "num_heads_q must be a positive multiple of num_heads_kv");
+  FK_CHECK_ARG(Hq / Hkv <= 16, "GQA group size (num_heads_q / num_heads_kv) must be <= 16");
+  FK_CHECK_ARG((long long)B * Hq <= (1 << 24) && (long long)B * Lmax < (1LL << 31), "batch too large");
+  const long long stretches = (Lmax + kMassTokens - 1) / kMassTokens;
+  FK_CHECK_ARG((long long)B * Hkv * stretches < (1LL << 30), "batch * num_heads_kv * max_seqlen too large");
+  return kOk;
+}
+
+}  // namespace cattn
+}  // namespace fk
+
+using namespace fk;
+
+extern "C" int fk_cache_attn_workspace_bytes(int batch, int max_seqlen, int num_heads_q, int num_heads_kv,
+                                             int head_dim, int with_mass, size_t* bytes_out) {
+  FK_CHECK_ARG(bytes_out != nullptr, "bytes_out is null");
+  int rc = cattn::check_sizes(batch, max_seqlen, num_heads_q, num_heads_kv, head_dim);
+  if (rc) return rc;
+  *bytes_out = cattn::layout(batch, max_seqlen, num_heads_q, num_heads_kv, head_dim, with_mass != 0).total();
+  return kOk;
+}
+
+extern "C" int fk_cache_attn_fwd(const void* q, long long q_batch_stride, const void* k_cache, const void* v_cache,
+                                 const int32_t* block_table, const int32_t* cache_seqlens, const float* mass_in,
+                                 float* mass_out, long long mass_capacity, void* out, float* lse, int dtype,
+                                 int batch, int max_seqlen, int block_size, int num_blocks, int num_heads_q,
+                                 int num_heads_kv, int head_dim, float softmax_scale, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
+  FK_CHECK_ARG(q && k_cache && v_cache && cache_seqlens && out && lse && workspace, "null tensor pointer");
+  FK_CHECK_ARG(dtype == FK_BF16 || dtype == FK_FP16, "dtype must be FK_BF16 or FK_FP16");
+  int rc = cattn::check_sizes(batch, max_seqlen, num_heads_q, num_heads_kv, head_dim);
+  if (rc) return rc;
+  FK_CHECK_ARG(isfinite(softmax_scale), "softmax_scale must be finite");
+  FK_CHECK_ARG(q_batch_stride >= (long long)num_heads_q * head_dim && q_batch_stride % 2 == 0,
+               "q row stride must be even and >= num_heads_q * head_dim");
+  FK_CHECK_ARG(((uintptr_t)q & 3) == 0 && ((uintptr_t)out & 3) == 0, "q and out must be 4-byte aligned");
+  FK_CHECK_ARG(((uintptr_t)k_cache & 15) == 0 && ((uintptr_t)v_cache & 15) == 0 && ((uintptr_t)workspace & 15) == 0,
+               "caches and workspace must be 16-byte aligned");
+  FK_CHECK_ARG((mass_in == nullptr) == (mass_out == nullptr), "give both mass_in and mass_out, or neither");
+  FK_CHECK_ARG(!mass_in || mass_capacity >= max_seqlen, "mass_capacity must be >= max_seqlen");
+  if (block_table) {
+    FK_CHECK_ARG(block_size >= 1 && num_blocks >= 1 && max_seqlen % block_size == 0,
+                 "paged cache: max_seqlen must be max_blocks_per_seq * block_size, num_blocks >= 1");
+    FK_CHECK_ARG((long long)num_blocks * block_size < (1LL << 31), "pool too large");
+  }
+  const cattn::Layout w = cattn::layout(batch, max_seqlen, num_heads_q, num_heads_kv, head_dim, mass_out != nullptr);
+  FK_CHECK_ARG(workspace_bytes >= w.total(), "workspace too small");
+  cattn::Params p = {};
+  p.q = q;
+  p.q_stride = q_batch_stride;
+  p.k = k_cache;
+  p.v = v_cache;
+  p.block_table = block_table;
+  p.block_size = block_table ? block_size : 1;
+  p.max_blocks = block_table ? max_seqlen / block_size : 0;
+  p.num_blocks = num_blocks;
+  p.seqlens = cache_seqlens;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.o_part = reinterpret_cast<float*>(ws);
+  p.lse_part = reinterpret_cast<float*>(ws + w.o_bytes);
+  p.scores = mass_out ? reinterpret_cast<float*>(ws + w.o_bytes + w.lse_bytes) : nullptr;
+  p.gs = cattn::score_stride(num_heads_q / num_heads_kv);
+  p.mass_in = mass_in;
+  p.mass_out = mass_out;
+  p.mass_cap = mass_capacity;
+  p.out = out;
+  p.lse = lse;
+  p.B = batch;
+  p.Lmax = max_seqlen;
+  p.Hq = num_heads_q;
+  p.Hkv = num_heads_kv;
+  p.G = num_heads_q / num_heads_kv;
+  p.chunk = w.chunk;
+  p.scale_log2 = softmax_scale * cattn::kLog2e;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == FK_BF16)
+    return head_dim == 128 ? cattn::by_group<__nv_bfloat16, 128>(p, st) : cattn::by_group<__nv_bfloat16, 64>(p, st);
+  return head_dim == 128 ? cattn::by_group<__half, 128>(p, st) : cattn::by_group<__half, 64>(p, st);
+}

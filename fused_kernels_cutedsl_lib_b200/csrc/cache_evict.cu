@@ -1,0 +1,367 @@
+// Eviction from a KV cache by accumulated attention weight.
+//
+// Per row b with len > budget and per kv head: of the tokens [0, len) the first
+// `sinks`, the last `recent` and the budget - sinks - recent others of greatest
+// mass stay (equal masses: the earlier token), in their order. Their K and V
+// rows and masses are written to [0, budget) of the output cache, zeros to the
+// masses behind, and the new length and old positions beside them. Rows of at
+// most `budget` tokens are copied whole. The output cache is another one than
+// the input cache, contiguous or paged, with pages of any size on either side.
+//
+// Bound: HBM. Every mass is read once (4 bytes), every kept token's K and V row
+// is read and written once.
+//
+// `select_kernel`: a cluster of CL CTAs per (row, kv head) finds the threshold
+// mass by radix selection: floats map to order-preserving unsigned keys, and
+// four passes narrow the key of the r-th greatest 8 bits at a time. Each CTA
+// counts the digits of its stretch in shared memory, all CTAs read all counts
+// through distributed shared memory and draw the same conclusion, so a pass is
+// one cluster barrier. Then each warp counts what it keeps, one scan over the
+// cluster's warps gives every warp its place, and kept positions and masses are
+// written in order. No atomics decide an order: results do not depend on timing.
+//
+// `gather_kernel` (a programmatic dependent): copies the kept rows, 16 bytes per
+// thread and cache, neighbouring threads along the heads of one output token.
+#include <cooperative_groups.h>
+
+#include "common.cuh"
+#include "fk_b200.h"
+
+namespace fk {
+namespace evict {
+
+namespace cg = cooperative_groups;
+
+constexpr int kThreads = 1024;
+constexpr int kWarps = kThreads / 32;
+constexpr int kBins = 256;
+constexpr int kMaxCluster = 8;
+
+struct Params {
+  const uint8_t* k;          // [B, Lmax, Hkv, row_bytes] or [num_blocks, block_size, Hkv, row_bytes]
+  const uint8_t* v;
+  const int* table;          // [B, max_blocks] or null
+  int max_blocks, block_size, num_blocks;
+  const int* seqlens;
+  const float* mass;         // [B, Hkv, mass_cap]
+  long long mass_cap;
+  uint8_t* k_out;
+  uint8_t* v_out;
+  const int* out_table;
+  int out_max_blocks, out_block_size, out_num_blocks, out_max_seqlen;
+  int* seqlens_out;
+  float* mass_out;           // [B, Hkv, out_mass_cap]
+  long long out_mass_cap;
+  int* kept;                 // [B, Hkv, budget], -1 behind the new length
+  int B, Lmax, Hkv, row_bytes, budget, sinks, recent;
+};
+
+__device__ __forceinline__ int seq_len(const Params& p, int b) {
+  const int L = __ldg(p.seqlens + b);
+  return min(max(L, 0), p.Lmax);
+}
+
+// Order-preserving key: -inf < ... < -0 = +0 < ... < +inf < NaN.
+__device__ __forceinline__ uint32_t mass_key(float f) {
+  if (f != f) return 0xFFFFFFFFu;
+  const uint32_t u = __float_as_uint(f + 0.f);  // -0 + 0 = +0
+  return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+
+__global__ void __launch_bounds__(kThreads) select_kernel(const Params p) {
+  __shared__ int s_hist[2][kBins];   // this CTA's digit counts, double-buffered over the passes
+  __shared__ int s_tot[kBins];       // the cluster's
+  __shared__ int s_digit, s_above;
+  __shared__ int s_gt[kWarps], s_tie[kWarps];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  cg::cluster_group cluster = cg::this_cluster();
+  const int cl = cluster.num_blocks(), rank = cluster.block_rank();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int pair = blockIdx.x / cl;
+  const int b = pair / p.Hkv, h = pair - b * p.Hkv;
+  const int len = seq_len(p, b);
+  const int kept = min(len, p.budget);
+  const float* mass = p.mass + (size_t)pair * p.mass_cap;
+  float* mass_out = p.mass_out + (size_t)pair * p.out_mass_cap;
+  int* out = p.kept + (size_t)pair * p.budget;
+  const int t0 = rank * kThreads + threadIdx.x, step = cl * kThreads;
+
+  // Behind the new length: no positions, and masses that start at zero.
+  for (int i = kept + t0; i < p.budget; i += step) out[i] = -1;
+  for (long long i = kept + t0; i < p.out_mass_cap; i += step) mass_out[i] = 0.f;
+  if (h == 0 && rank == 0 && threadIdx.x == 0) p.seqlens_out[b] = kept;
+  if (len <= p.budget) {  // the same for the whole cluster
+    for (int i = t0; i < len; i += step) {
+      out[i] = i;
+      mass_out[i] = mass[i];
+    }
+    return;
+  }
+  const int first = p.sinks, m = len - p.recent - p.sinks;  // the candidates [first, first + m)
+  const int want = p.budget - p.sinks - p.recent;           // 0 <= want < m
+  for (int i = t0; i < p.sinks; i += step) {
+    out[i] = i;
+    mass_out[i] = mass[i];
+  }
+  for (int i = t0; i < p.recent; i += step) {
+    out[p.budget - p.recent + i] = len - p.recent + i;
+    mass_out[p.budget - p.recent + i] = mass[len - p.recent + i];
+  }
+  if (want == 0) return;
+
+  // Each warp of the cluster owns a contiguous stretch of the candidates.
+  const int warps = cl * kWarps, gw = rank * kWarps + warp;
+  const int seg = ((m + warps - 1) / warps + 31) & ~31;
+  const int w0 = min(gw * seg, m), w1 = min(w0 + seg, m);
+  mass += first;
+
+  uint32_t prefix = 0, mask = 0;  // the digits of the threshold key found so far
+  int above = 0;                  // candidates with a greater key than every key with this prefix
+  for (int pass = 0; pass < 4; ++pass) {
+    const int shift = 24 - 8 * pass;
+    int* hist = s_hist[pass & 1];
+    for (int i = threadIdx.x; i < kBins; i += kThreads) hist[i] = 0;
+    __syncthreads();
+    for (int i = w0 + lane; i < w1; i += 32) {
+      const uint32_t key = mass_key(__ldg(mass + i));
+      if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1);
+    }
+    cluster.sync();
+    // The other buffer is free to be cleared in the next pass: whoever read it has
+    // passed this barrier.
+    if (threadIdx.x < kBins) {
+      int n = 0;
+      for (int q = 0; q < cl; ++q) n += cluster.map_shared_rank(hist, q)[threadIdx.x];
+      s_tot[threadIdx.x] = n;
+    }
+    __syncthreads();
+    if (warp == 0) {
+      // The digit in which the want-th greatest lies: lane l holds digits [8l, 8l + 8), suffix sums over lanes.
+      int own[8], sum = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        own[i] = s_tot[lane * 8 + i];
+        sum += own[i];
+      }
+      int suffix = sum;  // sum over lanes >= this one
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int o = __shfl_down_sync(0xffffffffu, suffix, off);
+        if (lane + off < 32) suffix += o;
+      }
+      int over = above + suffix - sum;  // candidates of greater digits than this lane's
+      const int need = want;
+      if (over < need && need <= over + sum) {
+#pragma unroll
+        for (int i = 7; i >= 0; --i) {
+          if (over < need && need <= over + own[i]) {
+            s_digit = lane * 8 + i;
+            s_above = over;
+          }
+          over += own[i];
+        }
+      }
+    }
+    __syncthreads();
+    prefix |= (uint32_t)s_digit << shift;
+    mask |= 0xFFu << shift;
+    above = s_above;
+  }
+  // Keys above `prefix` all stay (`above` of them); of the equal ones the first want - above.
+  const int ties = want - above;
+
+  int n_gt = 0, n_tie = 0;
+  for (int i = w0 + lane; i < w1; i += 32) {
+    const uint32_t key = mass_key(__ldg(mass + i));
+    n_gt += key > prefix;
+    n_tie += key == prefix;
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    n_gt += __shfl_xor_sync(0xffffffffu, n_gt, off);
+    n_tie += __shfl_xor_sync(0xffffffffu, n_tie, off);
+  }
+  if (lane == 0) {
+    s_gt[warp] = n_gt;
+    s_tie[warp] = n_tie;
+  }
+  cluster.sync();
+  // What the warps before this one hold.
+  int b_gt = 0, b_tie = 0;
+  for (int q = 0; q <= rank; ++q) {
+    const int* gq = cluster.map_shared_rank(s_gt, q);
+    const int* tq = cluster.map_shared_rank(s_tie, q);
+    if (q < rank || lane < warp) {
+      b_gt += gq[lane];
+      b_tie += tq[lane];
+    }
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    b_gt += __shfl_xor_sync(0xffffffffu, b_gt, off);
+    b_tie += __shfl_xor_sync(0xffffffffu, b_tie, off);
+  }
+  const uint32_t below = (1u << lane) - 1u;
+  for (int i0 = w0; i0 < w1; i0 += 32) {
+    const int i = i0 + lane;
+    const float f = i < w1 ? __ldg(mass + i) : 0.f;
+    const uint32_t key = mass_key(f);
+    const bool gt = i < w1 && key > prefix, tie = i < w1 && key == prefix;
+    const uint32_t bg = __ballot_sync(0xffffffffu, gt), bt = __ballot_sync(0xffffffffu, tie);
+    const int tie_rank = b_tie + __popc(bt & below);
+    if (gt || (tie && tie_rank < ties)) {
+      const int pos = p.sinks + b_gt + __popc(bg & below) + min(tie_rank, ties);
+      out[pos] = first + i;
+      mass_out[pos] = f;
+    }
+    b_gt += __popc(bg);
+    b_tie += __popc(bt);
+  }
+  cluster.sync();  // no CTA leaves while another reads its counts
+}
+
+__global__ void __launch_bounds__(256) gather_kernel(const Params p, long long pieces, int slots) {
+  constexpr int U = 4;  // copies in flight per thread
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int per_row = p.row_bytes / 16;
+  uint4 kv[U], vv[U];
+  long long dst[U];
+  const long long base = (long long)blockIdx.x * (blockDim.x * U) + threadIdx.x;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    dst[u] = -1;
+    const long long i = base + (long long)u * blockDim.x;
+    if (i >= pieces) continue;
+    // piece i: 16 bytes of (row b, output token s, head h), heads and pieces fastest.
+    const long long tok = i / (p.Hkv * per_row);
+    const int in_tok = (int)(i - tok * (p.Hkv * per_row));
+    const int h = in_tok / per_row;
+    const int b = (int)(tok / slots), s = (int)(tok - (long long)b * slots);
+    const int src = __ldcg(p.kept + ((size_t)b * p.Hkv + h) * p.budget + s);
+    if (src < 0) continue;
+    long long from = (long long)b * p.Lmax + src, to = (long long)b * p.out_max_seqlen + s;
+    if (p.table) {
+      const int page = __ldg(p.table + (size_t)b * p.max_blocks + src / p.block_size);
+      from = page < 0 || page >= p.num_blocks ? -1 : (long long)page * p.block_size + src % p.block_size;
+    }
+    if (p.out_table) {
+      const int page = __ldg(p.out_table + (size_t)b * p.out_max_blocks + s / p.out_block_size);
+      if (page < 0 || page >= p.out_num_blocks) continue;
+      to = (long long)page * p.out_block_size + s % p.out_block_size;
+    }
+    const size_t row = (size_t)p.Hkv * p.row_bytes;
+    kv[u] = vv[u] = make_uint4(0u, 0u, 0u, 0u);
+    if (from >= 0) {
+      const size_t off = (size_t)from * row + (size_t)in_tok * 16;
+      kv[u] = *reinterpret_cast<const uint4*>(p.k + off);  // not through the read-only path: one pool may serve both sides
+      vv[u] = *reinterpret_cast<const uint4*>(p.v + off);
+    }
+    dst[u] = to * (long long)row + (long long)in_tok * 16;
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (dst[u] < 0) continue;
+    *reinterpret_cast<uint4*>(p.k_out + dst[u]) = kv[u];
+    *reinterpret_cast<uint4*>(p.v_out + dst[u]) = vv[u];
+  }
+}
+
+static int launch(const Params& p, cudaStream_t st) {
+  // CTAs per (row, head): enough that the pairs fill the SMs, as long as each warp
+  // still has 32 candidates of the longest row.
+  int cl = 1;
+  while (cl < kMaxCluster && (long long)p.B * p.Hkv * cl < num_sms() && p.Lmax > cl * kThreads) cl *= 2;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cl;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.B * p.Hkv * cl), 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  FK_CHECK_CUDA(cudaLaunchKernelEx(&cfg, select_kernel, p));
+  const int slots = p.budget < p.Lmax ? p.budget : p.Lmax;
+  const long long pieces = (long long)p.B * slots * p.Hkv * (p.row_bytes / 16);
+  cfg.gridDim = dim3((unsigned)((pieces + 1023) / 1024), 1, 1);
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.numAttrs = 1;
+  FK_CHECK_CUDA(cudaLaunchKernelEx(&cfg, gather_kernel, p, pieces, slots));
+  return kOk;
+}
+
+}  // namespace evict
+}  // namespace fk
+
+using namespace fk;
+
+extern "C" int fk_cache_evict(const void* k_cache, const void* v_cache, const int32_t* block_table,
+                              const int32_t* cache_seqlens, const float* mass, long long mass_capacity, void* k_out,
+                              void* v_out, const int32_t* out_block_table, int32_t* seqlens_out, float* mass_out,
+                              long long out_mass_capacity, int32_t* kept, int batch, int max_seqlen, int block_size,
+                              int num_blocks, int out_max_seqlen, int out_block_size, int out_num_blocks,
+                              int num_heads_kv, int row_bytes, int budget, int sinks, int recent, void* stream) {
+  FK_CHECK_ARG(k_cache && v_cache && cache_seqlens && mass && k_out && v_out && seqlens_out && mass_out && kept,
+               "null tensor pointer");
+  FK_CHECK_ARG(batch >= 1 && max_seqlen >= 1 && num_heads_kv >= 1, "sizes must be positive");
+  FK_CHECK_ARG(row_bytes >= 16 && row_bytes % 16 == 0, "row_bytes must be a positive multiple of 16");
+  FK_CHECK_ARG(budget >= 1 && sinks >= 0 && recent >= 0 && (long long)sinks + recent <= budget,
+               "budget must be >= 1 and sinks + recent must lie in [0, budget]");
+  FK_CHECK_ARG(out_max_seqlen >= (budget < max_seqlen ? budget : max_seqlen),
+               "the output cache must hold min(budget, max_seqlen) tokens per row");
+  FK_CHECK_ARG(mass_capacity >= max_seqlen && out_mass_capacity >= (budget < max_seqlen ? budget : max_seqlen),
+               "mass arrays too short");
+  FK_CHECK_ARG((long long)batch * num_heads_kv <= (1 << 24) && (long long)num_heads_kv * row_bytes < (1LL << 31),
+               "batch or row too large");
+  FK_CHECK_ARG((((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0,
+               "caches must be 16-byte aligned");
+  FK_CHECK_ARG(mass_out != mass && seqlens_out != cache_seqlens && k_out != v_out, "outputs must not alias");
+  // One pool on both sides is fine with two tables over different pages.
+  FK_CHECK_ARG((k_out != k_cache && v_out != v_cache && k_out != v_cache && v_out != k_cache) ||
+                   (block_table && out_block_table && block_table != out_block_table && k_out == k_cache &&
+                    v_out == v_cache),
+               "the output cache must not alias the input cache");
+  if (block_table)
+    FK_CHECK_ARG(block_size >= 1 && num_blocks >= 1 && max_seqlen % block_size == 0,
+                 "paged cache: max_seqlen must be max_blocks_per_seq * block_size, num_blocks >= 1");
+  if (out_block_table)
+    FK_CHECK_ARG(out_block_size >= 1 && out_num_blocks >= 1 && out_max_seqlen % out_block_size == 0,
+                 "paged output: out_max_seqlen must be max_blocks_per_seq * out_block_size, out_num_blocks >= 1");
+  const long long slots = budget < max_seqlen ? budget : max_seqlen;
+  FK_CHECK_ARG((long long)batch * slots * num_heads_kv * (row_bytes / 16) < (1LL << 40), "cache too large");
+  evict::Params p = {};
+  p.k = static_cast<const uint8_t*>(k_cache);
+  p.v = static_cast<const uint8_t*>(v_cache);
+  p.table = block_table;
+  p.block_size = block_table ? block_size : 1;
+  p.max_blocks = block_table ? max_seqlen / block_size : 0;
+  p.num_blocks = num_blocks;
+  p.seqlens = cache_seqlens;
+  p.mass = mass;
+  p.mass_cap = mass_capacity;
+  p.k_out = static_cast<uint8_t*>(k_out);
+  p.v_out = static_cast<uint8_t*>(v_out);
+  p.out_table = out_block_table;
+  p.out_block_size = out_block_table ? out_block_size : 1;
+  p.out_max_blocks = out_block_table ? out_max_seqlen / out_block_size : 0;
+  p.out_num_blocks = out_num_blocks;
+  p.out_max_seqlen = out_max_seqlen;
+  p.seqlens_out = seqlens_out;
+  p.mass_out = mass_out;
+  p.out_mass_cap = out_mass_capacity;
+  p.kept = kept;
+  p.B = batch;
+  p.Lmax = max_seqlen;
+  p.Hkv = num_heads_kv;
+  p.row_bytes = row_bytes;
+  p.budget = budget;
+  p.sinks = sinks;
+  p.recent = recent;
+  return evict::launch(p, static_cast<cudaStream_t>(stream));
+}

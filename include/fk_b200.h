@@ -362,6 +362,72 @@ FK_API int fk_kv_append_wait(const void* src, long long src_row_stride, int k_co
 FK_API int fk_skinny_gemm_noalloc(const void* x, const void* w, void* y, int M, int N, int K,
                                   void* stream);
 
+/* ---- memory-bound decode: 4-bit weights, cache attention with mass, eviction -- */
+
+/* Element types of the entry points below. */
+#define FK_BF16 0
+#define FK_FP16 1
+
+/* Linear layer with 4-bit weights: y[M, N] = x[M, K] W^T (+ residual[M, N]) with
+ * W[n, k] = (q[n, k] - z[n, k / group]) * s[n, k / group], q and z in [0, 15],
+ * group_size 32, 64 or 128 dividing K. x, s, residual and y are bf16 or fp16
+ * (dtype); x rows are ldx elements apart (ldx >= K, a multiple of 8), y and
+ * residual dense; residual may be null and may alias y. fp32 accumulation, one
+ * rounding. Weights never become 16-bit products: integers are multiplied and the
+ * scale is applied in fp32, so a non-finite x gives non-finite y.
+ *   packed      [ceil(N/16)][ceil(K/128)][2][32][4] uint32, 16-byte aligned: word j
+ *               of lane 4g + c in half h holds, lowest nibble first, q of row
+ *               16 nb + 8 h + g, inputs 128 kb + 32 j + 8 c + 0..7 (anything past N or K)
+ *   scale_zero  [ceil(N/16)][ceil(K/128) * 128 / group_size][16] uint32: s in the
+ *               low half, 16 + z (as dtype) in the high half; 0 past N or K
+ * No workspace. As for every GEMM here, the weights must not be written by the
+ * kernel of this library that precedes the call on its stream. */
+FK_API int fk_w4_linear(const void* x, long long ldx, const void* packed, const void* scale_zero,
+                        const void* residual, void* y, int dtype, int M, int N, int K, int group_size,
+                        void* stream);
+
+/* Attention of one new token per row over a KV cache, with the attention mass:
+ *   out = softmax(scale q K^T) V over the first cache_seqlens[b] tokens,
+ *   mass_out[b, h, j] = mass_in[b, h, j] + sum over the q heads of kv head h of the
+ *   softmax weight of token j, for j < cache_seqlens[b]; the rest is left as it is.
+ * q and out [batch, num_heads_q, head_dim], q rows q_batch_stride elements apart;
+ * caches [batch, max_seqlen, num_heads_kv, head_dim], or with block_table
+ * [batch, max_seqlen / block_size] pools [num_blocks, block_size, num_heads_kv,
+ * head_dim] with pages of any size; all bf16 or fp16 (dtype). lse [batch,
+ * num_heads_q] fp32, natural log. head_dim 64 or 128, at most 16 q heads per kv
+ * head. mass_in / mass_out [batch, num_heads_kv, mass_capacity] fp32, may be the
+ * same, null for no mass. Lengths are clamped to [0, max_seqlen]; a row of length 0
+ * gives out = 0, lse = -inf. A page id outside [0, num_blocks) reads as zero rows.
+ * workspace: fk_cache_attn_workspace_bytes bytes, 16-byte aligned, any contents;
+ * calls that may overlap on the GPU need their own. */
+FK_API int fk_cache_attn_workspace_bytes(int batch, int max_seqlen, int num_heads_q, int num_heads_kv,
+                                         int head_dim, int with_mass, size_t* bytes_out);
+FK_API int fk_cache_attn_fwd(const void* q, long long q_batch_stride, const void* k_cache, const void* v_cache,
+                             const int32_t* block_table, const int32_t* cache_seqlens, const float* mass_in,
+                             float* mass_out, long long mass_capacity, void* out, float* lse, int dtype,
+                             int batch, int max_seqlen, int block_size, int num_blocks, int num_heads_q,
+                             int num_heads_kv, int head_dim, float softmax_scale, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/* Eviction by mass: per row with len = cache_seqlens[b] > budget, and per kv head,
+ * the first `sinks` tokens, the last `recent` and the budget - sinks - recent others
+ * of greatest mass (equal: the earlier one; NaN counts as greatest) stay, in order;
+ * rows of at most budget tokens stay whole. Their K and V rows (row_bytes =
+ * head_dim * element size, a multiple of 16) and masses go to slots
+ * [0, min(len, budget)) of the output cache, seqlens_out[b] = min(len, budget),
+ * kept[b, h, i] = old position of slot i (-1 behind), mass_out = 0 behind. Cache
+ * layouts as fk_cache_attn_fwd; the output cache (contiguous [batch,
+ * out_max_seqlen, ...] or paged) is other memory than the input cache, or other
+ * pages of the same pools: no page that the input table names for a live token.
+ * No output page may serve two places. Input page ids outside the pool read as
+ * zero rows, output ones are not written. */
+FK_API int fk_cache_evict(const void* k_cache, const void* v_cache, const int32_t* block_table,
+                          const int32_t* cache_seqlens, const float* mass, long long mass_capacity, void* k_out,
+                          void* v_out, const int32_t* out_block_table, int32_t* seqlens_out, float* mass_out,
+                          long long out_mass_capacity, int32_t* kept, int batch, int max_seqlen, int block_size,
+                          int num_blocks, int out_max_seqlen, int out_block_size, int out_num_blocks,
+                          int num_heads_kv, int row_bytes, int budget, int sinks, int recent, void* stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif

@@ -1,0 +1,170 @@
+"""4-bit linear against its definition in 64 bits (GPU)."""
+import pytest
+import torch
+
+from fused_kernels_cutedsl_lib_b200 import _native, pack_w4, quantize_w4, w4_linear
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+def weight(n, k, group, dtype, zeros=True, seed=0, lo=0, hi=15):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    q = torch.randint(lo, hi + 1, (n, k), generator=g, device="cuda", dtype=torch.uint8)
+    s = (0.004 + 0.008 * torch.rand(n, k // group, generator=g, device="cuda")).to(dtype)
+    z = torch.randint(0, 16, (n, k // group), generator=g, device="cuda", dtype=torch.uint8) if zeros else None
+    return q, s, z
+
+
+def activations(m, k, dtype, seed=1):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(m, k, generator=g, device="cuda")
+    x[:, ::53] *= 10.0
+    return x.to(dtype)
+
+
+def check(y, x, q, s, z, residual=None):
+    """|y - ref| within the output's rounding plus the fp32 sums' worst case.
+
+    Inside a group of g inputs the integers 16 + q are summed by g/16 mma steps, each
+    off by at most 2 units of 2^-23 of the magnitude summed, and the zero point is
+    one more rounding (A below bounds both magnitudes); the scaled groups are then added
+    in at most K/g + 72 roundings (slices of up to 8 warps and 8 CTAs, residual) relative
+    to sum |x w| and the residual (B).
+    """
+    n, k = q.shape
+    g = k // s.shape[1]
+    rep = lambda t: t.repeat_interleave(g, dim=1).double()  # noqa: E731
+    zz = 8.0 if z is None else rep(z)
+    w = (q.double() - zz) * rep(s)
+    xd = x.double()
+    ref = xd @ w.t()
+    a = xd.abs() @ ((32.0 + q.double() + zz) * rep(s)).t()
+    b = xd.abs() @ w.abs().t()
+    if residual is not None:
+        ref = ref + residual.double()
+        b = b + residual.double().abs()
+    half_step = torch.finfo(y.dtype).eps / 2
+    tol = half_step * ref.abs() + 2.0 ** -23 * ((g / 8 + 2) * a + (k / g + 72) * b) + torch.finfo(y.dtype).tiny
+    err = (y.double() - ref).abs()
+    assert torch.isfinite(y).all()
+    assert (err <= tol).all(), f"worst {(err / tol).max().item():.3g} of the tolerance"
+
+
+SHAPES = [(1, 16, 128), (1, 1, 32), (2, 5, 96), (8, 100, 160), (9, 333, 4096), (16, 1000, 256), (17, 64, 512),
+          (33, 48, 1024), (64, 130, 2048), (65, 70, 640), (130, 33, 128), (3, 40, 14336), (1, 6144, 4096),
+          (40, 200, 14336), (7, 4100, 2080)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_matches_definition(m, n, k, dtype):
+    for group in (32, 64, 128):
+        if k % group:
+            continue
+        q, s, z = weight(n, k, group, dtype, zeros=(m + group) % 3 != 0, seed=m + n + group)
+        x = activations(m, k, dtype)
+        y = torch.full((m, n), float("nan"), dtype=dtype, device="cuda")
+        got = w4_linear(x, pack_w4(q, s, z), y)
+        assert got is y
+        check(y, x, q, s, z)
+    assert _native.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("m", [1, 5, 20, 70])
+def test_residual_may_be_the_output(m, dtype):
+    q, s, z = weight(210, 512, 64, dtype)
+    x, r = activations(m, 512, dtype), activations(m, 210, dtype, seed=3)
+    w = pack_w4(q, s, z)
+    check(w4_linear(x, w, residual=r), x, q, s, z, r)
+    y = r.clone()
+    w4_linear(x, w, y, residual=y)
+    check(y, x, q, s, z, r)
+
+
+@pytest.mark.parametrize("codes,zero", [((0, 0), 15), ((15, 15), 0), ((0, 0), 0), ((15, 15), 15)])
+def test_extreme_codes(codes, zero):
+    q, s, _ = weight(64, 256, 32, BF16, lo=codes[0], hi=codes[1])
+    z = torch.full((64, 8), zero, dtype=torch.uint8, device="cuda")
+    x = activations(4, 256, BF16)
+    y = w4_linear(x, pack_w4(q, s, z))
+    check(y, x, q, s, z)
+    if codes[0] == zero:  # every weight is 0: so is the result, up to the sums' rounding checked above
+        assert y.abs().max().item() < 1e-2
+
+
+def test_strided_rows_streams_and_repeats():
+    q, s, z = weight(300, 1024, 128, BF16)
+    w = pack_w4(q, s, z)
+    wide = activations(6, 1024 + 512, BF16)
+    x = wide[:, 256:1280]
+    y = w4_linear(x, w)
+    check(y, x, q, s, z)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    y2 = torch.empty_like(y)
+    w4_linear(x, w, y2, stream=st)
+    st.synchronize()
+    assert torch.equal(y, y2)
+    for _ in range(20):
+        assert torch.equal(w4_linear(x, w), y)
+
+
+def test_zero_tokens_and_graph_replay():
+    q, s, z = weight(96, 640, 128, FP16)
+    w = pack_w4(q, s, z)
+    assert w4_linear(torch.empty(0, 640, dtype=FP16, device="cuda"), w).shape == (0, 96)
+    x, y = activations(3, 640, FP16), torch.empty(3, 96, dtype=FP16, device="cuda")
+    w4_linear(x, w, y)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        w4_linear(x, w, y)
+        w4_linear(x, w, y, residual=y)  # y = 2 x W^T, rounded twice
+    for seed in (5, 6):
+        x.copy_(activations(3, 640, FP16, seed=seed))
+        graph.replay()
+        one = w4_linear(x, w)
+        two = w4_linear(x, w, residual=one)
+        assert torch.equal(y, two)
+
+
+def test_quantized_weight_times_tokens():
+    torch.manual_seed(0)
+    for symmetric in (False, True):
+        w = torch.randn(200, 384, device="cuda") * 0.02
+        p = quantize_w4(w, 64, symmetric=symmetric)
+        x = activations(4, 384, BF16)
+        # The codes' half step (asymmetric: range / 15, symmetric: max / 7), with the scale's own rounding to
+        # bf16 moving a code's value by up to 15 (8) of its half steps of 2^-8.
+        v = w.view(200, -1, 64)
+        step = (v.amax(-1).clamp_min(0) - v.amin(-1).clamp_max(0)) / 15 if not symmetric else v.abs().amax(-1) / 7
+        off = (p.dequantize().view(200, -1, 64) - v).abs()
+        assert (off <= step[..., None] * (1.0 + 16 * 2.0 ** -8)).all()
+        y = w4_linear(x, p).double()
+        ref = x.double() @ p.dequantize().double().t()
+        assert ((y - ref).norm() / ref.norm()).item() <= 2.0 ** -8
+
+
+def test_refusals():
+    q, s, z = weight(32, 256, 64, BF16)
+    w = pack_w4(q, s, z)
+    x = activations(2, 256, BF16)
+    with pytest.raises(TypeError):
+        w4_linear(x.half(), w)
+    with pytest.raises(TypeError):
+        w4_linear(x, q)
+    with pytest.raises(ValueError):
+        w4_linear(x[:, :192], w)
+    with pytest.raises(ValueError):
+        w4_linear(x.t().contiguous().t(), w)  # columns are not dense
+    with pytest.raises(ValueError):
+        w4_linear(activations(2, 260, BF16)[:, :256], w)  # row stride 260
+    with pytest.raises(ValueError):
+        w4_linear(x, w, torch.empty(2, 33, dtype=BF16, device="cuda"))
+    with pytest.raises(ValueError):
+        w4_linear(x, w, residual=torch.empty(1, 32, dtype=BF16, device="cuda"))
+    with pytest.raises(ValueError):  # 2-byte aligned rows
+        w4_linear(torch.empty(2 * 256 + 1, dtype=BF16, device="cuda")[1:].view(2, 256), w)
