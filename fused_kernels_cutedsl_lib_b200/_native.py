@@ -127,7 +127,7 @@ SIGNATURES: dict[str, tuple] = {
         _c_int, [_p, _p, _p, _p, _c_int, _c_int, _c_int, _c_float, _p, ctypes.c_size_t, _p]),
     "fk_w4_linear": (
         _c_int,
-        [_p, ctypes.c_longlong, _p, _p, _p, _p, _c_int, _c_int, _c_int, _c_int, _c_int, _p],
+        [_p, ctypes.c_longlong, _p, _p, _p, _c_int, _c_int, _c_int, _c_int, _c_int, _p],
     ),
     "fk_cache_attn_workspace_bytes": (
         _c_int,

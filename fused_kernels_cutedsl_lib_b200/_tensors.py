@@ -40,11 +40,23 @@ def same_device(*ts: torch.Tensor) -> torch.device:
     return dev
 
 
+def raw_current_stream(idx: int) -> int:
+    """Torch's current stream on device ``idx`` as an int, without building a Stream object
+    (0.1 instead of 2.2 us of host time per call)."""
+    return torch._C._cuda_getCurrentRawStream(idx)
+
+
+if not hasattr(torch._C, "_cuda_getCurrentRawStream"):  # a torch without that accessor
+    def raw_current_stream(idx: int) -> int:  # noqa: F811
+        return torch.cuda.current_stream(idx).cuda_stream
+
+
 def stream_for(dev: torch.device, stream=None) -> int:
     """cudaStream_t (as int) to launch on: explicit, else torch's current stream."""
-    _native.use_device(dev.index if dev.index is not None else torch.cuda.current_device())
+    idx = dev.index if dev.index is not None else torch.cuda.current_device()
+    _native.use_device(idx)
     if stream is None:
-        return torch.cuda.current_stream(dev).cuda_stream
+        return raw_current_stream(idx)
     if isinstance(stream, torch.cuda.Stream):
         return stream.cuda_stream
     return int(stream)
@@ -61,9 +73,13 @@ def dtype_code(dtype: torch.dtype) -> int:
     return _DTYPE_CODES[dtype]
 
 
-def require_float16ish(name: str, t, ndim: int | None = None, *, dtype=None, strided_rows: bool = False):
+def require_half(name: str, t, ndim: int | None = None, *, dtype=None, strided_rows: bool = False) -> None:
     """:func:`require_tensor` for bf16 or fp16 (or the given one of the two). ``strided_rows``
     allows any stride of the first dimension, the others dense."""
+    if (isinstance(t, torch.Tensor) and (t.dtype in _DTYPE_CODES if dtype is None else t.dtype == dtype)
+            and (ndim is None or t.dim() == ndim) and t.is_cuda
+            and (t.is_contiguous() or (strided_rows and t.shape[0] > 0 and t[0].is_contiguous()))):
+        return
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
     if (t.dtype not in _DTYPE_CODES) if dtype is None else (t.dtype != dtype):
@@ -72,40 +88,59 @@ def require_float16ish(name: str, t, ndim: int | None = None, *, dtype=None, str
         raise ValueError(f"{name} must have {ndim} dims, got shape {tuple(t.shape)}")
     if t.device.type != "cuda":
         raise ValueError(f"{name} must be a CUDA tensor, got device {t.device}")
-    if not t.is_contiguous() and not (strided_rows and t.shape[0] > 0 and t[0].is_contiguous()):
-        raise ValueError(f"{name} must be {'dense behind its first dimension' if strided_rows else 'contiguous (row-major)'}")
-    return t
+    raise ValueError(f"{name} must be {'dense behind its first dimension' if strided_rows else 'contiguous (row-major)'}")
 
 
-class launching_on:
-    """``with launching_on(dev, stream) as handle``: the library's current device is ``dev``
-    inside, and what was current before is current again after, in torch and in the library."""
+def require_dense(name: str, t, dtype: torch.dtype, shape: tuple) -> None:
+    """A contiguous CUDA tensor of the given type and shape: :func:`require_tensor` and
+    :func:`require_shape` with one pass of checks where nothing is wrong."""
+    if (isinstance(t, torch.Tensor) and t.dtype == dtype and t.shape == shape and t.is_cuda and t.is_contiguous()):
+        return
+    require_tensor(name, t, dtype, len(shape))
+    require_shape(name, t, shape)
 
-    __slots__ = ("dev", "stream", "guard", "before")
 
-    def __init__(self, dev: torch.device, stream=None):
-        self.dev, self.stream = dev, stream
+def one_device(*ts) -> int:
+    """Index of the CUDA device that holds every tensor (None entries are passed over)."""
+    idx = ts[0].get_device()
+    for t in ts:
+        if t is not None and t.get_device() != idx:
+            same_device(*[u for u in ts if u is not None])
+    return idx
 
-    def __enter__(self) -> int:
-        self.before = torch.cuda.current_device()
-        self.guard = None
-        if self.dev.index is not None and self.dev.index != self.before:
-            self.guard = torch.cuda.device(self.dev)
-            self.guard.__enter__()
-        return stream_for(self.dev, self.stream)
+
+current_device = torch.cuda.current_device
+
+
+class on_device:
+    """``with on_device(idx)``: device ``idx`` is current in torch; behind it the one that was
+    current before is so again, in torch and in the library."""
+
+    def __init__(self, idx: int):
+        self.guard, self.before = torch.cuda.device(idx), torch.cuda.current_device()
+
+    def __enter__(self):
+        self.guard.__enter__()
 
     def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-            _native.use_device(self.before)
-        return False
+        self.guard.__exit__(*exc)
+        _native.use_device(self.before)
 
 
-def scratch(nbytes: int, dev: torch.device, stream_handle: int) -> torch.Tensor:
+def launch_stream(idx: int, stream=None) -> int:
+    """cudaStream_t (as int) to launch on, on the current device ``idx``: explicit, else torch's current."""
+    _native.use_device(idx)
+    if stream is None:
+        return raw_current_stream(idx)
+    return stream.cuda_stream if isinstance(stream, torch.cuda.Stream) else int(stream)
+
+
+def scratch(nbytes: int, idx: int, stream_handle: int) -> torch.Tensor:
     """Uninitialised bytes for one call on the given stream. Taken from torch's allocator on that
     stream, so a block is reused only by work behind the call (and, in a captured graph, only by
     that graph)."""
-    if stream_handle == torch.cuda.current_stream(dev).cuda_stream:
+    dev = torch.device("cuda", idx)
+    if stream_handle == raw_current_stream(idx):
         return torch.empty(nbytes, dtype=torch.uint8, device=dev)
     with torch.cuda.stream(torch.cuda.ExternalStream(stream_handle, device=dev)):
         return torch.empty(nbytes, dtype=torch.uint8, device=dev)

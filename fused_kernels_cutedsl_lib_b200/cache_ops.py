@@ -24,8 +24,8 @@ import math
 import torch
 
 from . import _native
-from ._tensors import (dtype_code, launching_on, ptr, require_float16ish, require_shape, require_tensor, same_device,
-                       scratch)
+from ._tensors import (current_device, dtype_code, launch_stream, on_device, one_device, require_dense, require_half,
+                       require_tensor, scratch)
 
 HEAD_DIMS = (64, 128)
 MAX_GROUP = 16
@@ -70,83 +70,79 @@ def cache_attention(q, k_cache, v_cache, cache_seqlens, out=None, lse=None, *, b
     ``mass_out`` defaults to ``mass``, and entries behind the lengths stay as they
     are. An empty row gives 0 and lse -inf.
     """
-    require_float16ish("q", q, strided_rows=True)
+    require_half("q", q, strided_rows=True)
     dt = q.dtype
     if q.dim() == 4 and q.shape[1] == 1:
         q = q.squeeze(1)
     if q.dim() != 3:
         raise ValueError(f"q must be [B, Hq, D] or [B, 1, Hq, D], got {tuple(q.shape)}")
     B, Hq, D = q.shape
-    require_float16ish("k_cache", k_cache, 4, dtype=dt)
-    require_float16ish("v_cache", v_cache, 4, dtype=dt)
-    if k_cache.shape != v_cache.shape:
-        raise ValueError(f"k_cache and v_cache must have the same shape, got {tuple(k_cache.shape)} and "
-                         f"{tuple(v_cache.shape)}")
-    require_tensor("cache_seqlens", cache_seqlens, torch.int32, 1)
-    rows, L, Hkv = k_cache.shape[:3]
-    if k_cache.shape[3] != D or D not in HEAD_DIMS:
-        raise ValueError(f"head_dim must be one of {HEAD_DIMS} in q and the caches, got {D} and {k_cache.shape[3]}")
+    require_half("k_cache", k_cache, 4, dtype=dt)
+    rows, L, Hkv, Dk = k_cache.shape
+    require_dense("v_cache", v_cache, dt, k_cache.shape)
+    if Dk != D or D not in HEAD_DIMS:
+        raise ValueError(f"head_dim must be one of {HEAD_DIMS} in q and the caches, got {D} and {Dk}")
     if Hkv < 1 or Hq < 1 or Hq % Hkv or Hq // Hkv > MAX_GROUP:
         raise ValueError(f"num_heads_q ({Hq}) must be a multiple of num_heads_kv ({Hkv}), ratio <= {MAX_GROUP}")
-    require_shape("cache_seqlens", cache_seqlens, (B,))
-    tensors = [q, k_cache, v_cache, cache_seqlens]
+    require_dense("cache_seqlens", cache_seqlens, torch.int32, (B,))
     page = pages = 0
     if block_table is not None:
         _check_table("block_table", block_table, B)
-        tensors.append(block_table)
         page, pages = L, rows
         L = block_table.shape[1] * page
     elif rows != B:
         raise ValueError(f"the caches hold {rows} rows but q has {B}")
     if L < 1 or (block_table is not None and pages < 1):
         raise ValueError("the cache holds no tokens")
-    if mass is None and mass_out is not None:
-        raise ValueError("mass_out needs mass")
     cap = 0
     if mass is not None:
-        mass_out = mass if mass_out is None else mass_out
         require_tensor("mass", mass, torch.float32, 3)
-        require_tensor("mass_out", mass_out, torch.float32, 3)
-        if tuple(mass.shape[:2]) != (B, Hkv) or mass.shape[2] < L or mass_out.shape != mass.shape:
-            raise ValueError(f"mass and mass_out must be [{B}, {Hkv}, >= {L}] alike, got {tuple(mass.shape)} and "
-                             f"{tuple(mass_out.shape)}")
         cap = mass.shape[2]
-        tensors += [mass, mass_out]
+        if mass.shape[0] != B or mass.shape[1] != Hkv or cap < L:
+            raise ValueError(f"mass must be [{B}, {Hkv}, >= {L}], got {tuple(mass.shape)}")
+        if mass_out is None:
+            mass_out = mass
+        else:
+            require_dense("mass_out", mass_out, torch.float32, (B, Hkv, cap))
+    elif mass_out is not None:
+        raise ValueError("mass_out needs mass")
     scale = D ** -0.5 if softmax_scale is None else float(softmax_scale)
     if not math.isfinite(scale):
         raise ValueError(f"softmax_scale must be finite, got {softmax_scale}")
     if out is None:
         out = torch.empty((B, Hq, D), dtype=dt, device=q.device)
     else:
-        require_tensor("out", out, dt)
+        require_half("out", out, dtype=dt)
         if out.numel() != B * Hq * D:
             raise ValueError(f"out must hold {B}x{Hq}x{D} elements, got shape {tuple(out.shape)}")
     if lse is None:
         lse = torch.empty((B, Hq), dtype=torch.float32, device=q.device)
     else:
-        require_tensor("lse", lse, torch.float32, 2)
-        require_shape("lse", lse, (B, Hq))
-    tensors += [out, lse]
+        require_dense("lse", lse, torch.float32, (B, Hq))
     if workspace is not None:
         require_tensor("workspace", workspace, torch.uint8, 1)
-        tensors.append(workspace)
-    dev = same_device(*tensors)
+    idx = one_device(q, k_cache, v_cache, cache_seqlens, block_table, mass, mass_out, out, lse, workspace)
     if B == 0:
         return out, lse
-    with launching_on(dev, stream) as st:
-        if workspace is None:
-            workspace = scratch(cache_attention_workspace_bytes(B, L, Hq, Hkv, D, mass is not None), dev, st)
-        _native.check(_native.load().fk_cache_attn_fwd(
-            ptr(q), q.stride(0) if B > 1 else Hq * D, ptr(k_cache), ptr(v_cache),
-            ptr(block_table) if block_table is not None else None, ptr(cache_seqlens),
-            ptr(mass) if mass is not None else None, ptr(mass_out) if mass is not None else None, cap, ptr(out),
-            ptr(lse), dtype_code(dt), B, L, page, pages, Hq, Hkv, D, scale, ptr(workspace), workspace.numel(), st))
+    if idx != current_device():
+        with on_device(idx):
+            return cache_attention(q, k_cache, v_cache, cache_seqlens, out, lse, block_table=block_table, mass=mass,
+                                   mass_out=mass_out, softmax_scale=softmax_scale, workspace=workspace, stream=stream)
+    st = launch_stream(idx, stream)
+    if workspace is None:
+        workspace = scratch(cache_attention_workspace_bytes(B, L, Hq, Hkv, D, mass is not None), idx, st)
+    _native.check(_native.load().fk_cache_attn_fwd(
+        q.data_ptr(), q.stride(0) if B > 1 else Hq * D, k_cache.data_ptr(), v_cache.data_ptr(),
+        block_table.data_ptr() if block_table is not None else None, cache_seqlens.data_ptr(),
+        mass.data_ptr() if mass is not None else None, mass_out.data_ptr() if mass is not None else None, cap,
+        out.data_ptr(), lse.data_ptr(), dtype_code(dt), B, L, page, pages, Hq, Hkv, D, scale, workspace.data_ptr(),
+        workspace.numel(), st))
     return out, lse
 
 
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    a0, b0 = a.data_ptr(), b.data_ptr()
-    return a0 < b0 + b.numel() * b.element_size() and b0 < a0 + a.numel() * a.element_size()
+def _meet(a: int, na: int, b: int, nb: int) -> bool:
+    """Whether the byte ranges [a, a + na) and [b, b + nb) meet."""
+    return a < b + nb and b < a + na
 
 
 def cache_evict(k_cache, v_cache, cache_seqlens, mass, k_out, v_out, seqlens_out, mass_out, budget: int, *,
@@ -167,41 +163,33 @@ def cache_evict(k_cache, v_cache, cache_seqlens, mass, k_out, v_out, seqlens_out
     same pools: ``out_block_table`` must name no page twice, and none that
     ``block_table`` names for a live token.
     """
-    require_float16ish("k_cache", k_cache, 4)
+    require_half("k_cache", k_cache, 4)
     dt = k_cache.dtype
-    require_float16ish("v_cache", v_cache, 4, dtype=dt)
-    require_float16ish("k_out", k_out, 4, dtype=dt)
-    require_float16ish("v_out", v_out, 4, dtype=dt)
-    if k_cache.shape != v_cache.shape or k_out.shape != v_out.shape:
-        raise ValueError("K and V caches must have the same shapes")
-    require_tensor("cache_seqlens", cache_seqlens, torch.int32, 1)
-    require_tensor("seqlens_out", seqlens_out, torch.int32, 1)
-    require_tensor("mass", mass, torch.float32, 3)
-    require_tensor("mass_out", mass_out, torch.float32, 3)
     rows, L, Hkv, D = k_cache.shape
-    rows_out, L_out = k_out.shape[:2]
-    B = cache_seqlens.shape[0]
-    if tuple(k_out.shape[2:]) != (Hkv, D):
+    require_dense("v_cache", v_cache, dt, k_cache.shape)
+    require_half("k_out", k_out, 4, dtype=dt)
+    rows_out, L_out, h_out, d_out = k_out.shape
+    if h_out != Hkv or d_out != D:
         raise ValueError(f"k_out and v_out must be [.., .., {Hkv}, {D}], got {tuple(k_out.shape)}")
+    require_dense("v_out", v_out, dt, k_out.shape)
     if Hkv < 1 or D < 8 or D % 8:
         raise ValueError(f"head_dim must be a positive multiple of 8, got {D}")
-    require_shape("seqlens_out", seqlens_out, (B,))
+    require_tensor("cache_seqlens", cache_seqlens, torch.int32, 1)
+    B = cache_seqlens.shape[0]
+    require_dense("seqlens_out", seqlens_out, torch.int32, (B,))
     budget, sinks, recent = int(budget), int(sinks), int(recent)
     if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
         raise ValueError(f"budget ({budget}) must be >= 1 and sinks ({sinks}) + recent ({recent}) must lie in "
                          f"[0, budget]")
-    tensors = [k_cache, v_cache, cache_seqlens, mass, k_out, v_out, seqlens_out, mass_out]
     page = pages = page_out = pages_out = 0
     if block_table is not None:
         _check_table("block_table", block_table, B)
-        tensors.append(block_table)
         page, pages = L, rows
         L = block_table.shape[1] * page
     elif rows != B:
         raise ValueError(f"the caches hold {rows} rows but there are {B} lengths")
     if out_block_table is not None:
         _check_table("out_block_table", out_block_table, B)
-        tensors.append(out_block_table)
         page_out, pages_out = L_out, rows_out
         L_out = out_block_table.shape[1] * page_out
     elif rows_out != B:
@@ -209,30 +197,39 @@ def cache_evict(k_cache, v_cache, cache_seqlens, mass, k_out, v_out, seqlens_out
     need = min(budget, L)
     if L < 1 or L_out < need:
         raise ValueError(f"the output cache holds {L_out} tokens per row, needs {need} (and the input at least 1)")
-    if tuple(mass.shape[:2]) != (B, Hkv) or mass.shape[2] < L:
+    require_tensor("mass", mass, torch.float32, 3)
+    require_tensor("mass_out", mass_out, torch.float32, 3)
+    cap, cap_out = mass.shape[2], mass_out.shape[2]
+    if mass.shape[0] != B or mass.shape[1] != Hkv or cap < L:
         raise ValueError(f"mass must be [{B}, {Hkv}, >= {L}], got {tuple(mass.shape)}")
-    if tuple(mass_out.shape[:2]) != (B, Hkv) or mass_out.shape[2] < need:
+    if mass_out.shape[0] != B or mass_out.shape[1] != Hkv or cap_out < need:
         raise ValueError(f"mass_out must be [{B}, {Hkv}, >= {need}], got {tuple(mass_out.shape)}")
     if kept is None:
         kept = torch.empty((B, Hkv, budget), dtype=torch.int32, device=k_cache.device)
     else:
-        require_tensor("kept", kept, torch.int32, 3)
-        require_shape("kept", kept, (B, Hkv, budget))
-    tensors.append(kept)
-    dev = same_device(*tensors)
-    same_pool = (block_table is not None and out_block_table is not None and not _overlap(block_table, out_block_table)
-                 and k_out.data_ptr() == k_cache.data_ptr() and v_out.data_ptr() == v_cache.data_ptr())
-    if not same_pool and any(_overlap(a, b) for a in (k_out, v_out) for b in (k_cache, v_cache)):
+        require_dense("kept", kept, torch.int32, (B, Hkv, budget))
+    idx = one_device(k_cache, v_cache, cache_seqlens, mass, k_out, v_out, seqlens_out, mass_out, block_table,
+                     out_block_table, kept)
+    pk, pv, pko, pvo = k_cache.data_ptr(), v_cache.data_ptr(), k_out.data_ptr(), v_out.data_ptr()
+    nb, nbo = k_cache.numel() * 2, k_out.numel() * 2  # bytes of each input and output cache
+    same_pool = (block_table is not None and out_block_table is not None and pko == pk and pvo == pv
+                 and block_table.data_ptr() != out_block_table.data_ptr())
+    if not same_pool and (_meet(pko, nbo, pk, nb) or _meet(pko, nbo, pv, nb) or _meet(pvo, nbo, pk, nb)
+                          or _meet(pvo, nbo, pv, nb)):
         raise ValueError("the output caches must not overlap the input caches")
-    if _overlap(k_out, v_out) or _overlap(mass, mass_out) or _overlap(cache_seqlens, seqlens_out):
+    pm, pmo, pl, plo = mass.data_ptr(), mass_out.data_ptr(), cache_seqlens.data_ptr(), seqlens_out.data_ptr()
+    if (_meet(pko, nbo, pvo, nbo) or _meet(pm, mass.numel() * 4, pmo, mass_out.numel() * 4)
+            or _meet(pl, B * 4, plo, B * 4)):
         raise ValueError("k_out and v_out, mass and mass_out, and the lengths must not overlap")
     if B == 0:
         return kept
-    with launching_on(dev, stream) as st:
-        _native.check(_native.load().fk_cache_evict(
-            ptr(k_cache), ptr(v_cache), ptr(block_table) if block_table is not None else None, ptr(cache_seqlens),
-            ptr(mass), mass.shape[2], ptr(k_out), ptr(v_out),
-            ptr(out_block_table) if out_block_table is not None else None, ptr(seqlens_out), ptr(mass_out),
-            mass_out.shape[2], ptr(kept), B, L, page, pages, L_out, page_out, pages_out, Hkv, D * k_cache.element_size(),
-            budget, sinks, recent, st))
+    if idx != current_device():
+        with on_device(idx):
+            return cache_evict(k_cache, v_cache, cache_seqlens, mass, k_out, v_out, seqlens_out, mass_out, budget,
+                               sinks=sinks, recent=recent, block_table=block_table, out_block_table=out_block_table,
+                               kept=kept, stream=stream)
+    _native.check(_native.load().fk_cache_evict(
+        pk, pv, block_table.data_ptr() if block_table is not None else None, pl, pm, cap, pko, pvo,
+        out_block_table.data_ptr() if out_block_table is not None else None, plo, pmo, cap_out, kept.data_ptr(), B, L,
+        page, pages, L_out, page_out, pages_out, Hkv, D * 2, budget, sinks, recent, launch_stream(idx, stream)))
     return kept

@@ -17,34 +17,40 @@ from dataclasses import dataclass
 import torch
 
 from . import _native
-from ._tensors import dtype_code, launching_on, ptr, require_float16ish, require_tensor, same_device
+from ._tensors import (current_device, dtype_code, launch_stream, on_device, one_device, require_dense, require_half,
+                       same_device)
 
 GROUP_SIZES = (32, 64, 128)
-_BLOCK_K = 128
+_BLOCK_K = 128  # inputs per block
+_SLAB = 4       # input blocks per slab
 
 
 @dataclass(frozen=True)
 class W4Weight:
     """A packed 4-bit weight [N, K]; build it with :func:`pack_w4` or :func:`quantize_w4`."""
 
-    packed: torch.Tensor      # int32 [ceil(N/16), ceil(K/128), 2, 32, 4]: codes in the kernel's order
-    scale_zero: torch.Tensor  # int32 [ceil(N/16), ceil(K/128) * 128 / group_size, 16]: scale | (16 + zero) << 16
+    packed: torch.Tensor  # int32, ceil(N/16) * ceil(K/128) blocks of 256 + 2048 / group_size: codes and scales
     n: int
     k: int
     group_size: int
-    dtype: torch.dtype        # of the scales, the activations and the output
+    dtype: torch.dtype    # of the scales, the activations and the output
 
     def nbytes(self) -> int:
-        return (self.packed.numel() + self.scale_zero.numel()) * 4
+        return self.packed.numel() * 4
 
     def dequantize(self) -> torch.Tensor:
         """The weight as fp32 [N, K] (``(q - z) * s``, exact)."""
-        nb, kb = self.packed.shape[:2]
+        nb, kb, words = -(-self.n // 16), -(-self.k // _BLOCK_K), 256 + 2048 // self.group_size
+        full = kb // _SLAB
+        head = self.packed[:full * _SLAB * nb * words].view(full, nb, _SLAB, words).transpose(0, 1)
+        tail = self.packed[full * _SLAB * nb * words:].view(nb, -1, words)
+        blocks = torch.cat([head.reshape(nb, -1, words), tail], 1)
         shifts = torch.arange(0, 32, 4, device=self.packed.device, dtype=torch.int32)
-        q = (self.packed.unsqueeze(-1) >> shifts) & 15                       # [nb, kb, half, lane, j, i]
-        q = q.view(nb, kb, 2, 8, 4, 4, 8).permute(0, 2, 3, 1, 5, 4, 6)       # [nb, half, g, kb, j, c, i]
+        q = (blocks[..., :256].unsqueeze(-1) >> shifts) & 15
+        q = q.view(nb, kb, 2, 8, 4, 4, 2, 4).permute(0, 2, 3, 1, 5, 4, 7, 6)  # [nb, half, g, kb, j, c, pair, odd]
         q = q.reshape(nb * 16, kb * _BLOCK_K)[:self.n, :self.k].float()
-        sz = self.scale_zero.transpose(1, 2).reshape(nb * 16, -1)[:self.n, :self.k // self.group_size]
+        sz = blocks[..., 256:].reshape(nb, -1, 16).transpose(1, 2).reshape(nb * 16, -1)
+        sz = sz[:self.n, :self.k // self.group_size]
         both = sz.reshape(-1).contiguous().view(self.dtype).view(self.n, -1, 2).float()
         s, z = both[..., 0], both[..., 1] - 16.0
         rep = lambda t: t.repeat_interleave(self.group_size, dim=1)  # noqa: E731
@@ -80,22 +86,26 @@ def pack_w4(q: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = 
         raise ValueError("codes and zero points must lie in [0, 15]")
     dev = q.device
     nb, kb = -(-n // 16), -(-k // _BLOCK_K)
-    packed = torch.empty(nb, kb, 2, 32, 4, dtype=torch.int32, device=dev)
+    words = 256 + 2048 // group
+    packed = torch.empty(nb, kb, words, dtype=torch.int32, device=dev)
     shifts = torch.arange(0, 32, 4, device=dev, dtype=torch.int32)
     step = max(1, (1 << 25) // (kb * _BLOCK_K * 16))  # row blocks at a time: the int32 codes are 8 times the result
     for b0 in range(0, nb, step):
         rows = q[b0 * 16:(b0 + step) * 16]
         pad = torch.zeros(-(-rows.shape[0] // 16) * 16, kb * _BLOCK_K, dtype=torch.int32, device=dev)
         pad[:rows.shape[0], :k] = rows
-        # [nb, half, g, kb, j, c, i] -> [nb, kb, half, (g, c), j], nibble i of the word
-        v = pad.view(-1, 2, 8, kb, 4, 4, 8).permute(0, 3, 1, 2, 5, 4, 6) << shifts
-        packed[b0:b0 + v.shape[0]] = v.sum(-1, dtype=torch.int32).reshape(-1, kb, 2, 32, 4)
+        # [nb, half, g, kb, j, c, pair, odd] -> [nb, kb, half, (g, c), j], nibble 4 * odd + pair of the word
+        v = pad.view(-1, 2, 8, kb, 4, 4, 4, 2).permute(0, 3, 1, 2, 5, 4, 7, 6).flatten(-2) << shifts
+        packed[b0:b0 + v.shape[0], :, :256] = v.sum(-1, dtype=torch.int32).reshape(-1, kb, 256)
     z = torch.full_like(scales, 24.0) if zeros is None else zeros.to(scales.dtype) + 16.0
     sz = torch.zeros(nb * 16, kb * _BLOCK_K // group, 2, dtype=scales.dtype, device=dev)
     sz[:n, :k // group, 0] = scales
     sz[:n, :k // group, 1] = z
-    sz = sz.view(torch.int32).view(nb, 16, -1).transpose(1, 2).contiguous()
-    return W4Weight(packed, sz, n, k, group, scales.dtype)
+    packed[..., 256:] = sz.view(torch.int32).view(nb, 16, kb, -1).permute(0, 2, 3, 1).reshape(nb, kb, -1)
+    full = kb // _SLAB
+    packed = torch.cat([packed[:, :full * _SLAB].view(nb, full, _SLAB, words).transpose(0, 1).reshape(-1),
+                        packed[:, full * _SLAB:].reshape(-1)])
+    return W4Weight(packed, n, k, group, scales.dtype)
 
 
 def quantize_w4(w: torch.Tensor, group_size: int = 128, symmetric: bool = False, dtype=None) -> W4Weight:
@@ -138,30 +148,28 @@ def w4_linear(x, weight: W4Weight, out=None, *, residual=None, stream=None):
     if not isinstance(weight, W4Weight):
         raise TypeError(f"weight must be a W4Weight (pack_w4, quantize_w4), got {type(weight).__name__}")
     n, k, dt = weight.n, weight.k, weight.dtype
-    require_float16ish("x", x, 2, dtype=dt, strided_rows=True)
-    m = x.shape[0]
-    if x.shape[1] != k:
-        raise ValueError(f"x is [M, K={x.shape[1]}] but the weight is [N={n}, K={k}]")
+    require_half("x", x, 2, dtype=dt, strided_rows=True)
+    m, xk = x.shape
+    if xk != k:
+        raise ValueError(f"x is [M, K={xk}] but the weight is [N={n}, K={k}]")
     ldx = x.stride(0) if m > 1 else k
     if ldx < k or ldx % 8:
         raise ValueError(f"x row stride must be >= K and a multiple of 8 elements, got {ldx}")
     if out is None:
         out = torch.empty((m, n), dtype=dt, device=x.device)
     else:
-        require_tensor("out", out, dt, 2)
-        if out.shape[0] != m or out.shape[1] != n:
-            raise ValueError(f"out must have shape {(m, n)}, got {tuple(out.shape)}")
+        require_dense("out", out, dt, (m, n))
     if residual is not None:
-        require_tensor("residual", residual, dt, 2)
-        if residual.shape[0] != m or residual.shape[1] != n:
-            raise ValueError(f"residual must have shape {(m, n)}, got {tuple(residual.shape)}")
-        dev = same_device(x, weight.packed, out, residual)
-    else:
-        dev = same_device(x, weight.packed, out)
+        require_dense("residual", residual, dt, (m, n))
+    packed = weight.packed
+    idx = one_device(x, packed, out, residual)
     if m == 0:
         return out
-    with launching_on(dev, stream) as st:
-        _native.check(_native.load().fk_w4_linear(
-            ptr(x), ldx, ptr(weight.packed), ptr(weight.scale_zero), ptr(residual) if residual is not None else None,
-            ptr(out), dtype_code(dt), m, n, k, weight.group_size, st))
+    if idx != current_device():
+        with on_device(idx):
+            return w4_linear(x, weight, out, residual=residual, stream=stream)
+    _native.check(_native.load().fk_w4_linear(
+        x.data_ptr(), ldx, packed.data_ptr(),
+        residual.data_ptr() if residual is not None else None, out.data_ptr(), dtype_code(dt), m, n, k,
+        weight.group_size, launch_stream(idx, stream)))
     return out

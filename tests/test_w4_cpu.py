@@ -20,8 +20,12 @@ def test_pack_and_dequantize(n, k, group, zeros, dtype):
     row, col = n - 1, k - 1
     h, g = (row % 16) // 8, row % 8
     j, c, i = (col % 128) // 32, (col % 32) // 8, col % 8
-    word = int(w.packed[row // 16, col // 128, h, 4 * g + c, j]) & 0xFFFFFFFF
-    assert (word >> (4 * i)) & 15 == int(q[row, col])
+    nb, kb, words = -(-n // 16), -(-k // 128), 256 + 2048 // group
+    slab, block = col // 512, col % 512 // 128
+    at = (slab * 4 * nb + (row // 16) * min(4, kb - 4 * slab) + block) * words
+    word = int(w.packed[at + (h * 32 + 4 * g + c) * 4 + j]) & 0xFFFFFFFF
+    nibble = (i % 2) * 4 + i // 2  # even inputs in the low half, odd ones in the high half
+    assert (word >> (4 * nibble)) & 15 == int(q[row, col])
 
 
 def test_quantize_keeps_exact_grids():
@@ -63,7 +67,7 @@ def test_entry_point_refuses_before_launch():
     lib = _native.load()
 
     def call(ldx=256, x=16, dtype=0, m=1, n=16, k=256, group=64):
-        return lib.fk_w4_linear(x, ldx, 16, 16, None, 16, dtype, m, n, k, group, None)
+        return lib.fk_w4_linear(x, ldx, 16, None, 16, dtype, m, n, k, group, None)
 
     for bad in (dict(ldx=255), dict(ldx=264 - 4), dict(x=18), dict(x=None), dict(dtype=2), dict(m=0), dict(n=0),
                 dict(k=0), dict(group=16), dict(k=224)):
