@@ -177,10 +177,8 @@ __global__ void __launch_bounds__(warps<NT>() * 32 + 32, 1) w4_linear_kernel(con
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  // No division on the device here: the few 64-bit ones that split the rows took 5 us of every
-  // call (17 warps each emulating them), more than the rest of a small call together.
+  // The host did the divisions: emulated ones in every warp cost a small call 1.4 us.
   const int cs = 1 << p.cs_log, rank = blockIdx.x & (cs - 1), cid = blockIdx.x >> p.cs_log;
-  const int kw = 1 << p.kw_log;
   const int tok0 = blockIdx.y * TOK;
   const int ntok = min(TOK, p.M - tok0);
   // This cluster's row blocks; this CTA's slabs are rank, rank + cs, ...
@@ -409,43 +407,39 @@ __global__ void __launch_bounds__(warps<NT>() * 32 + 32, 1) w4_linear_kernel(con
   }
 }
 
-// Clusters of cs CTAs that can be resident at once. The answers are kept per kernel: asking
-// takes longer than the launch.
+// Clusters of 1, 2, 4 and 8 CTAs that can be resident at once, one CTA per SM; asked once per
+// kernel and device (asking takes longer than a launch).
 template <typename T, int NT, int GROUP>
-static int resident_clusters(int cs, int smem, int* out) {
-  struct Known {
-    int dev, cs, smem, n;
-  };
-  constexpr int kKnown = 64;
+static int resident_clusters(int (&out)[4]) {
+  constexpr int kDevices = 64;
   static std::mutex mu;
-  static Known known[kKnown];
-  static int count = 0;
+  static int known[kDevices][4] = {};
   auto kern = w4_linear_kernel<T, NT, GROUP>;
   int dev = 0;
   FK_CHECK_CUDA(cudaGetDevice(&dev));
+  FK_CHECK_ARG(dev >= 0 && dev < kDevices, "device index too large");
   std::lock_guard<std::mutex> lock(mu);
-  for (int i = 0; i < count; ++i) {
-    if (known[i].dev == dev && known[i].cs == cs && known[i].smem == smem) {
-      *out = known[i].n;
-      return kOk;
+  int* k = known[dev];
+  if (k[3] == 0) {
+    FK_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    for (int i = 0; i < 4; ++i) {
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = 1 << i;
+      attr[0].val.clusterDim.y = 1;
+      attr[0].val.clusterDim.z = 1;
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(1u << i, 1, 1);
+      cfg.blockDim = dim3(warps<NT>() * 32 + 32, 1, 1);
+      cfg.dynamicSmemBytes = kSmem;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      int n = 0;
+      FK_CHECK_CUDA(cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
+      k[i] = n < 1 ? 1 : n;
     }
   }
-  FK_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cs;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)cs, 1, 1);
-  cfg.blockDim = dim3(warps<NT>() * 32 + 32, 1, 1);
-  cfg.dynamicSmemBytes = smem;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  int n = 0;
-  FK_CHECK_CUDA(cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
-  *out = n < 1 ? 1 : n;
-  if (count < kKnown) known[count++] = Known{dev, cs, smem, *out};
+  for (int i = 0; i < 4; ++i) out[i] = k[i];
   return kOk;
 }
 
@@ -453,43 +447,42 @@ template <typename T, int NT, int GROUP>
 static int launch(Params p, cudaStream_t st) {
   constexpr int W = warps<NT>();
   constexpr int kBudget = kSmem - ring_bytes<NT, GROUP>();  // for x and the partial sums
+  constexpr int kX = x_bytes<NT, GROUP>();
+  int resident[4];
+  int rc = resident_clusters<T, NT, GROUP>(resident);
+  if (rc) return rc;
   const int tiles = (p.M + NT * 8 - 1) / (NT * 8);
-  int sms = num_sms() / tiles;
-  if (sms < 1) sms = 1;
-  // CTAs per cluster: the fewest that hold all of x beside one partial sum per warp, and whose
+  // CTAs per cluster: the fewest that hold all of their x and partial sums at once, and whose
   // clusters have a row block for three quarters of the warps; at most 8 (the portable
-  // size), and no more than there are slabs.
-  int cs = 1, ncl = 0, rows = 0, slabs = 0;
-  for (;; cs *= 2) {
-    ncl = sms / cs > 0 ? sms / cs : 1;
+  // size), and no more than there are slabs. With 8, x and rows may go in several rounds.
+  int kw = 1, ncl = 0, own_bytes = 0, rows = 0, slabs = 0;
+  for (p.cs_log = 0;; ++p.cs_log) {
+    const int cs = 1 << p.cs_log;
+    ncl = resident[p.cs_log] / tiles > 0 ? resident[p.cs_log] / tiles : 1;
     if (ncl > p.nrb) ncl = p.nrb;
     rows = (p.nrb + ncl - 1) / ncl;
     slabs = (p.nslab + cs - 1) / cs;
+    // Few rows per cluster: 2 or 4 warps share a row block. Each part costs a plane of partial sums.
+    for (kw = 1; kw < kSlab && W / kw >= 2 * rows;) kw *= 2;
+    own_bytes = part_bytes<NT>() * cs * kw;  // one owned row block
     if (cs == 8 || 2 * cs > p.nslab) break;
-    if ((long long)slabs * x_bytes<NT, GROUP>() + W * part_bytes<NT>() <= kBudget && 4 * rows >= 3 * W) break;
+    if ((long long)slabs * kX + (long long)((rows + cs - 1) / cs) * own_bytes <= kBudget && 4 * rows >= 3 * W) break;
   }
-  // Few rows per cluster: 2 or 4 warps share a row block. Each part costs a plane of partial sums.
-  int kw = 1;
-  while (kw < kSlab && W / kw >= 2 * rows) kw *= 2;
-  const int own_bytes = part_bytes<NT>() * cs * kw;  // one owned row block
+  const int cs = 1 << p.cs_log;
   // x takes what is left by one round of row blocks, the partial sums what is left by x.
   int own = (W / kw + cs - 1) / cs;
-  p.chunk = (kBudget - own * own_bytes) / x_bytes<NT, GROUP>();
+  if (own > (rows + cs - 1) / cs) own = (rows + cs - 1) / cs;
+  p.chunk = (kBudget - own * own_bytes) / kX;
   if (p.chunk < 1) return fail(kErrUnsupported, "w4 linear: x does not fit into shared memory");
   if (p.chunk > slabs) p.chunk = slabs;
-  own = (kBudget - p.chunk * x_bytes<NT, GROUP>()) / own_bytes;
-  if (own > (rows + cs - 1) / cs) own = (rows + cs - 1) / cs;
-  p.tile = own * cs < rows ? own * cs : rows;
-  const int smem = ring_bytes<NT, GROUP>() + p.chunk * x_bytes<NT, GROUP>() + own * own_bytes;
-  int resident = 0;
-  int rc = resident_clusters<T, NT, GROUP>(cs, smem, &resident);
-  if (rc) return rc;
-  if (ncl * tiles > resident) ncl = resident / tiles > 0 ? resident / tiles : 1;
-  p.cs_log = cs == 8 ? 3 : cs == 4 ? 2 : cs == 2 ? 1 : 0;
+  own = (kBudget - p.chunk * kX) / own_bytes;
+  const int rounds = (rows + own * cs - 1) / (own * cs);  // of equal size
+  p.tile = (rows + rounds - 1) / rounds;
+  own = (p.tile + cs - 1) / cs;
+  const int smem = ring_bytes<NT, GROUP>() + p.chunk * kX + own * own_bytes;
   p.kw_log = kw == 4 ? 2 : kw == 2 ? 1 : 0;
   p.rb_each = p.nrb / ncl;
   p.rb_more = p.nrb % ncl;
-  auto kern = w4_linear_kernel<T, NT, GROUP>;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -504,7 +497,7 @@ static int launch(Params p, cudaStream_t st) {
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  FK_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, p));
+  FK_CHECK_CUDA(cudaLaunchKernelEx(&cfg, w4_linear_kernel<T, NT, GROUP>, p));
   return kOk;
 }
 
