@@ -52,6 +52,7 @@ struct Params {
   const void* v;
   const int* block_table;   // [B, max_blocks] or null
   int max_blocks, block_size, num_blocks;
+  FastDiv page;             // by block_size
   const int* seqlens;
   float* o_part;            // [S, B, Hq, D], normalised per split
   float* lse_part;          // [S, B, Hq], log2 domain
@@ -62,7 +63,7 @@ struct Params {
   long long mass_cap;
   void* out;                // [B, Hq, D]
   float* lse;               // [B, Hq]
-  int B, Lmax, Hq, Hkv, G, chunk;
+  int B, Lmax, Hq, Hkv, G, chunk, chunk_log;  // chunk: a power of two
   float scale_log2;
 };
 
@@ -126,7 +127,7 @@ struct TileIter {
   bool valid;
   __device__ __forceinline__ void row(const Params& p) {
     len = seq_len(p, b);
-    nb = (len + p.chunk - 1) / p.chunk;
+    nb = (len + p.chunk - 1) >> p.chunk_log;
   }
   __device__ __forceinline__ void locate(const Params& p) {
     while (true) {
@@ -201,9 +202,10 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const Params p) {
     const int t = ld.t + tw + (lane & 15);
     if (t >= ld.t1) return -1;
     if (p.block_table == nullptr) return ld.b * p.Lmax + t;
-    const int page = __ldg(p.block_table + (size_t)ld.b * p.max_blocks + t / p.block_size);
+    const int pg = p.page.div(t);
+    const int page = __ldg(p.block_table + (size_t)ld.b * p.max_blocks + pg);
     if (page < 0 || page >= p.num_blocks) return -1;
-    return page * p.block_size + t % p.block_size;
+    return page * p.block_size + (t - pg * p.block_size);
   };
   int next_row = resolve();
   int ld_stage = 0;
@@ -419,7 +421,7 @@ __global__ void __launch_bounds__(128) finish_kernel(const Params p, int merge_b
     const int row = blockIdx.x * 4 + warp;
     if (row >= p.B * p.Hq) return;
     const int b = row / p.Hq;
-    const int n = (seq_len(p, b) + p.chunk - 1) / p.chunk;
+    const int n = (seq_len(p, b) + p.chunk - 1) >> p.chunk_log;
     constexpr int PER = D / 32;  // dims per lane
     float M = -INFINITY;
     for (int s = lane; s < n; s += 32) M = fmaxf(M, __ldg(p.lse_part + s * plane + row));
@@ -471,7 +473,7 @@ __global__ void __launch_bounds__(128) finish_kernel(const Params p, int merge_b
   const int b = pair / p.Hkv, h = pair - b * p.Hkv;
   const int len = seq_len(p, b);
   if (t0 >= len) return;
-  const int n = (len + p.chunk - 1) / p.chunk;
+  const int n = (len + p.chunk - 1) >> p.chunk_log;
   for (int hh = warp; hh < p.G; hh += 4) {
     const float* src = p.lse_part + (size_t)b * p.Hq + (size_t)h * p.G + hh;
     float M = -INFINITY, W = 0.f;
@@ -626,6 +628,7 @@ extern "C" int fk_cache_attn_fwd(const void* q, long long q_batch_stride, const 
   p.v = v_cache;
   p.block_table = block_table;
   p.block_size = block_table ? block_size : 1;
+  p.page = FastDiv::of(p.block_size);
   p.max_blocks = block_table ? max_seqlen / block_size : 0;
   p.num_blocks = num_blocks;
   p.seqlens = cache_seqlens;
@@ -645,6 +648,7 @@ extern "C" int fk_cache_attn_fwd(const void* q, long long q_batch_stride, const 
   p.Hkv = num_heads_kv;
   p.G = num_heads_q / num_heads_kv;
   p.chunk = w.chunk;
+  for (p.chunk_log = 6; (1 << p.chunk_log) < w.chunk;) ++p.chunk_log;
   p.scale_log2 = softmax_scale * cattn::kLog2e;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == FK_BF16)

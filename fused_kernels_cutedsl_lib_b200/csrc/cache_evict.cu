@@ -221,50 +221,74 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const Params p) {
   cluster.sync();  // no CTA leaves while another reads its counts
 }
 
-__global__ void __launch_bounds__(256) gather_kernel(const Params p, long long pieces, int slots) {
-  constexpr int U = 4;  // copies in flight per thread
+constexpr int kGatherThreads = 256;
+constexpr int kUnroll = 4;  // 16-byte copies of K and of V in flight per thread
+
+// How the pieces of 16 bytes of one row b's output tokens are dealt to threads: piece i of a
+// block is piece in_tok of token tok, i = tok * per_tok + in_tok, heads and pieces fastest.
+struct GatherPlan {
+  FastDiv per_tok;    // pieces of a token: heads * row_bytes / 16
+  FastDiv per_row;    // pieces of a head's row
+  FastDiv page_in, page_out;
+  int tokens;         // output tokens per block
+  int slots;          // output tokens per row b at most
+};
+
+__global__ void __launch_bounds__(kGatherThreads) gather_kernel(const Params p, const GatherPlan g) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int per_row = p.row_bytes / 16;
-  uint4 kv[U], vv[U];
-  long long dst[U];
-  const long long base = (long long)blockIdx.x * (blockDim.x * U) + threadIdx.x;
+  const int b = blockIdx.y, s0 = blockIdx.x * g.tokens;
+  const int live = min(seq_len(p, b), p.budget);  // tokens of this row's output
+  const int pieces = min(g.tokens, live - s0) * g.per_tok.d;
+  const int* kept = p.kept + (size_t)b * p.Hkv * p.budget;
+  const size_t row = (size_t)p.Hkv * p.row_bytes;
+  for (int i0 = threadIdx.x; i0 < pieces; i0 += kGatherThreads * kUnroll) {
+    uint4 kv[kUnroll], vv[kUnroll];
+    long long from[kUnroll], to[kUnroll];
+    int src[kUnroll];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    dst[u] = -1;
-    const long long i = base + (long long)u * blockDim.x;
-    if (i >= pieces) continue;
-    // piece i: 16 bytes of (row b, output token s, head h), heads and pieces fastest.
-    const long long tok = i / (p.Hkv * per_row);
-    const int in_tok = (int)(i - tok * (p.Hkv * per_row));
-    const int h = in_tok / per_row;
-    const int b = (int)(tok / slots), s = (int)(tok - (long long)b * slots);
-    const int src = __ldcg(p.kept + ((size_t)b * p.Hkv + h) * p.budget + s);
-    if (src < 0) continue;
-    long long from = (long long)b * p.Lmax + src, to = (long long)b * p.out_max_seqlen + s;
-    if (p.table) {
-      const int page = __ldg(p.table + (size_t)b * p.max_blocks + src / p.block_size);
-      from = page < 0 || page >= p.num_blocks ? -1 : (long long)page * p.block_size + src % p.block_size;
+    for (int u = 0; u < kUnroll; ++u) {
+      const int i = i0 + u * kGatherThreads;
+      const int tok = g.per_tok.div(i), in_tok = i - tok * g.per_tok.d, s = s0 + tok;
+      from[u] = in_tok * 16;  // offsets in bytes; the row is added below
+      to[u] = -1;
+      if (i < pieces) {
+        src[u] = __ldcg(kept + (size_t)g.per_row.div(in_tok) * p.budget + s);
+        long long r = (long long)b * p.out_max_seqlen + s;
+        if (p.out_table) {
+          const int page = __ldg(p.out_table + (size_t)b * p.out_max_blocks + g.page_out.div(s));
+          r = page < 0 || page >= p.out_num_blocks
+                  ? -1
+                  : (long long)page * p.out_block_size + (s - g.page_out.div(s) * p.out_block_size);
+        }
+        if (r >= 0) to[u] = r * (long long)row + in_tok * 16;
+      }
     }
-    if (p.out_table) {
-      const int page = __ldg(p.out_table + (size_t)b * p.out_max_blocks + s / p.out_block_size);
-      if (page < 0 || page >= p.out_num_blocks) continue;
-      to = (long long)page * p.out_block_size + s % p.out_block_size;
-    }
-    const size_t row = (size_t)p.Hkv * p.row_bytes;
-    kv[u] = vv[u] = make_uint4(0u, 0u, 0u, 0u);
-    if (from >= 0) {
-      const size_t off = (size_t)from * row + (size_t)in_tok * 16;
-      kv[u] = *reinterpret_cast<const uint4*>(p.k + off);  // not through the read-only path: one pool may serve both sides
-      vv[u] = *reinterpret_cast<const uint4*>(p.v + off);
-    }
-    dst[u] = to * (long long)row + (long long)in_tok * 16;
-  }
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    if (dst[u] < 0) continue;
-    *reinterpret_cast<uint4*>(p.k_out + dst[u]) = kv[u];
-    *reinterpret_cast<uint4*>(p.v_out + dst[u]) = vv[u];
+    for (int u = 0; u < kUnroll; ++u) {
+      if (to[u] < 0) continue;
+      long long r = (long long)b * p.Lmax + src[u];
+      if (p.table) {
+        const int pg = g.page_in.div(src[u]);
+        const int page = __ldg(p.table + (size_t)b * p.max_blocks + pg);
+        r = page < 0 || page >= p.num_blocks ? -1 : (long long)page * p.block_size + (src[u] - pg * p.block_size);
+      }
+      from[u] = r < 0 ? -1 : from[u] + r * (long long)row;
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      kv[u] = vv[u] = make_uint4(0u, 0u, 0u, 0u);
+      if (to[u] >= 0 && from[u] >= 0) {  // not through the read-only path: one pool may serve both sides
+        kv[u] = *reinterpret_cast<const uint4*>(p.k + from[u]);
+        vv[u] = *reinterpret_cast<const uint4*>(p.v + from[u]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      if (to[u] < 0) continue;
+      *reinterpret_cast<uint4*>(p.k_out + to[u]) = kv[u];
+      *reinterpret_cast<uint4*>(p.v_out + to[u]) = vv[u];
+    }
   }
 }
 
@@ -287,12 +311,19 @@ static int launch(const Params& p, cudaStream_t st) {
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   FK_CHECK_CUDA(cudaLaunchKernelEx(&cfg, select_kernel, p));
-  const int slots = p.budget < p.Lmax ? p.budget : p.Lmax;
-  const long long pieces = (long long)p.B * slots * p.Hkv * (p.row_bytes / 16);
-  cfg.gridDim = dim3((unsigned)((pieces + 1023) / 1024), 1, 1);
-  cfg.blockDim = dim3(256, 1, 1);
+  GatherPlan g;
+  g.slots = p.budget < p.Lmax ? p.budget : p.Lmax;
+  const int per_row = p.row_bytes / 16, per_tok = p.Hkv * per_row;
+  g.per_tok = FastDiv::of(per_tok);
+  g.per_row = FastDiv::of(per_row);
+  g.page_in = FastDiv::of(p.block_size);
+  g.page_out = FastDiv::of(p.out_block_size);
+  // Tokens per block: one to four rounds of the unrolled loop.
+  g.tokens = (2 * kGatherThreads * kUnroll + per_tok - 1) / per_tok;
+  cfg.gridDim = dim3((unsigned)((g.slots + g.tokens - 1) / g.tokens), (unsigned)p.B, 1);
+  cfg.blockDim = dim3(kGatherThreads, 1, 1);
   cfg.numAttrs = 1;
-  FK_CHECK_CUDA(cudaLaunchKernelEx(&cfg, gather_kernel, p, pieces, slots));
+  FK_CHECK_CUDA(cudaLaunchKernelEx(&cfg, gather_kernel, p, g));
   return kOk;
 }
 
@@ -317,7 +348,8 @@ extern "C" int fk_cache_evict(const void* k_cache, const void* v_cache, const in
                "the output cache must hold min(budget, max_seqlen) tokens per row");
   FK_CHECK_ARG(mass_capacity >= max_seqlen && out_mass_capacity >= (budget < max_seqlen ? budget : max_seqlen),
                "mass arrays too short");
-  FK_CHECK_ARG((long long)batch * num_heads_kv <= (1 << 24) && (long long)num_heads_kv * row_bytes < (1LL << 31),
+  FK_CHECK_ARG(batch <= 65535 && (long long)batch * num_heads_kv <= (1 << 24) &&
+                   (long long)num_heads_kv * row_bytes <= (1 << 24),
                "batch or row too large");
   FK_CHECK_ARG((((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0,
                "caches must be 16-byte aligned");
@@ -333,8 +365,6 @@ extern "C" int fk_cache_evict(const void* k_cache, const void* v_cache, const in
   if (out_block_table)
     FK_CHECK_ARG(out_block_size >= 1 && out_num_blocks >= 1 && out_max_seqlen % out_block_size == 0,
                  "paged output: out_max_seqlen must be max_blocks_per_seq * out_block_size, out_num_blocks >= 1");
-  const long long slots = budget < max_seqlen ? budget : max_seqlen;
-  FK_CHECK_ARG((long long)batch * slots * num_heads_kv * (row_bytes / 16) < (1LL << 40), "cache too large");
   evict::Params p = {};
   p.k = static_cast<const uint8_t*>(k_cache);
   p.v = static_cast<const uint8_t*>(v_cache);
