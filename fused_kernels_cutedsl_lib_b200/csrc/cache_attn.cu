@@ -33,6 +33,8 @@
 #include <cuda_fp16.h>
 #include <math.h>
 
+#include <mutex>
+
 #include "common.cuh"
 #include "fk_b200.h"
 
@@ -167,6 +169,12 @@ template <int D>
 __host__ __device__ constexpr int stage_bytes() { return 2 * 16 * D * 2; }  // one warp's K and V of 16 tokens
 template <int D>
 __host__ __device__ constexpr int stages() { return D == 128 ? 3 : 5; }
+
+// The warps' rings, and room to merge their softmax states for G query heads.
+template <int D, int NT>
+__host__ __device__ constexpr size_t attend_smem(int G) {
+  return (size_t)NW * stages<D>() * stage_bytes<D>() + (size_t)(2 * NW * NT * 8 + NW * G * D) * 4;
+}
 
 template <typename E, int D, int NT, bool MASS>
 __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const Params p) {
@@ -407,33 +415,47 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const Params p) {
   cp_async_wait<0>();
 }
 
-constexpr int kMassTokens = 2048;  // tokens per mass block
+// Scores h0 .. h0 + 3 of one token (gs of them, 1 or an even number); 0 past the end.
+__device__ __forceinline__ float4 load_scores(const float* sc, int h0, int gs) {
+  if ((gs & 3) == 0) return *reinterpret_cast<const float4*>(sc + h0);
+  float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (gs == 1) {
+    f.x = *sc;
+  } else {
+    const float2 a = *reinterpret_cast<const float2*>(sc + h0);
+    f.x = a.x, f.y = a.y;
+    if (h0 + 2 < gs) {
+      const float2 c = *reinterpret_cast<const float2*>(sc + h0 + 2);
+      f.z = c.x, f.w = c.y;
+    }
+  }
+  return f;
+}
 
-// Blocks [0, merge_blocks): four (row, q head) pairs each, one per warp, merge the
-// splits. The others: one stretch of kMassTokens tokens of one (row, kv head).
+constexpr int kFinishThreads = 256;
+constexpr int kMassUnroll = 4;                                // tokens of a thread whose loads are in flight together
+constexpr int kMassTokens = kFinishThreads * kMassUnroll;     // tokens per mass block
+
+// Blocks [0, merge_blocks): eight (row, q head) pairs each, one per warp, merge the
+// splits. The others: one stretch of kMassTokens tokens of one (row, kv head). Both read
+// what pass 1 left, mostly in L2, and are short: what matters is that all loads of a
+// thread are issued before the first is used.
 template <typename E, int D>
-__global__ void __launch_bounds__(128) finish_kernel(const Params p, int merge_blocks, int stretches) {
+__global__ void __launch_bounds__(kFinishThreads) finish_kernel(const Params p, int merge_blocks, FastDiv stretches,
+                                                                FastDiv heads_q, FastDiv heads_kv) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const size_t plane = (size_t)p.B * p.Hq;
   if ((int)blockIdx.x < merge_blocks) {
-    const int row = blockIdx.x * 4 + warp;
+    const int row = blockIdx.x * (kFinishThreads / 32) + warp;
     if (row >= p.B * p.Hq) return;
-    const int b = row / p.Hq;
+    const int b = heads_q.div(row);
     const int n = (seq_len(p, b) + p.chunk - 1) >> p.chunk_log;
     constexpr int PER = D / 32;  // dims per lane
-    float M = -INFINITY;
-    for (int s = lane; s < n; s += 32) M = fmaxf(M, __ldg(p.lse_part + s * plane + row));
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-    const float ms = M == -INFINITY ? 0.f : M;
-    float W = 0.f, acc[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) acc[i] = 0.f;
-    constexpr int CH = 8;  // splits whose loads are in flight together; summed in split order
-    for (int s0 = 0; s0 < n; s0 += CH) {
-      float ls[CH], v[CH][PER];
+    constexpr int CH = 8;        // splits whose loads are in flight together; summed in split order
+    float ls[CH], v[CH][PER];
+    auto load = [&](int s0) {
 #pragma unroll
       for (int u = 0; u < CH; ++u) {
         const bool in = s0 + u < n;
@@ -447,6 +469,18 @@ __global__ void __launch_bounds__(128) finish_kernel(const Params p, int merge_b
           v[u][0] = f.x, v[u][1] = f.y;
         }
       }
+    };
+    load(0);
+    float M = -INFINITY;
+    for (int s = lane; s < n; s += 32) M = fmaxf(M, __ldg(p.lse_part + s * plane + row));
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+    const float ms = M == -INFINITY ? 0.f : M;
+    float W = 0.f, acc[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+    for (int s0 = 0; s0 < n; s0 += CH) {
+      if (s0 > 0) load(s0);
 #pragma unroll
       for (int u = 0; u < CH; ++u) {
         if (s0 + u < n) {
@@ -468,13 +502,29 @@ __global__ void __launch_bounds__(128) finish_kernel(const Params p, int merge_b
 
   __shared__ float s_lse[16];
   const int i = blockIdx.x - merge_blocks;
-  const int pair = i / stretches;
-  const int t0 = (i - pair * stretches) * kMassTokens;
-  const int b = pair / p.Hkv, h = pair - b * p.Hkv;
+  const int pair = stretches.div(i);
+  const int t0 = (i - pair * stretches.d) * kMassTokens;
+  const int b = heads_kv.div(pair), h = pair - b * p.Hkv;
   const int len = seq_len(p, b);
   if (t0 >= len) return;
   const int n = (len + p.chunk - 1) >> p.chunk_log;
-  for (int hh = warp; hh < p.G; hh += 4) {
+  const float* sc = p.scores + (size_t)pair * p.Lmax * p.gs;
+  const size_t mrow = (size_t)pair * p.mass_cap;
+  const int t1 = min(t0 + kMassTokens, len);
+  float mass[kMassUnroll], w[kMassUnroll];
+#pragma unroll
+  for (int u = 0; u < kMassUnroll; ++u) {
+    const int t = t0 + u * kFinishThreads + (int)threadIdx.x;
+    mass[u] = t < t1 ? p.mass_in[mrow + t] : 0.f;
+    w[u] = 0.f;
+  }
+  float4 first[kMassUnroll];  // scores of the first four heads, or of the only one or two
+#pragma unroll
+  for (int u = 0; u < kMassUnroll; ++u) {
+    const int t = t0 + u * kFinishThreads + (int)threadIdx.x;
+    first[u] = t < t1 ? load_scores(sc + (size_t)t * p.gs, 0, p.gs) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  for (int hh = warp; hh < p.G; hh += kFinishThreads / 32) {
     const float* src = p.lse_part + (size_t)b * p.Hq + (size_t)h * p.G + hh;
     float M = -INFINITY, W = 0.f;
     for (int s = lane; s < n; s += 32) M = fmaxf(M, __ldg(src + s * plane));
@@ -488,13 +538,23 @@ __global__ void __launch_bounds__(128) finish_kernel(const Params p, int merge_b
     if (lane == 0) s_lse[hh] = W == 0.f ? INFINITY : M + log2f(W);
   }
   __syncthreads();
-  const float* sc = p.scores + (size_t)pair * p.Lmax * p.gs;
-  const size_t mrow = (size_t)pair * p.mass_cap;
-  const int t1 = min(t0 + kMassTokens, len);
-  for (int t = t0 + (int)threadIdx.x; t < t1; t += 128) {
-    float w = 0.f;
-    for (int hh = 0; hh < p.G; ++hh) w += exp2f(__ldg(sc + (size_t)t * p.gs + hh) - s_lse[hh]);
-    p.mass_out[mrow + t] = p.mass_in[mrow + t] + w;
+  for (int h0 = 0; h0 < p.G; h0 += 4) {
+    float z[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) z[e] = h0 + e < p.G ? s_lse[h0 + e] : INFINITY;
+#pragma unroll
+    for (int u = 0; u < kMassUnroll; ++u) {
+      const int t = t0 + u * kFinishThreads + (int)threadIdx.x;
+      const float4 x = h0 == 0 ? first[u]
+                       : t < t1 ? load_scores(sc + (size_t)t * p.gs, h0, p.gs) : make_float4(0.f, 0.f, 0.f, 0.f);
+      // Heads past the group hold anything finite in the score array's padding, and z = +inf there.
+      w[u] += (exp2f(x.x - z[0]) + exp2f(x.y - z[1])) + (exp2f(x.z - z[2]) + exp2f(x.w - z[3]));
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kMassUnroll; ++u) {
+    const int t = t0 + u * kFinishThreads + (int)threadIdx.x;
+    if (t < t1) p.mass_out[mrow + t] = mass[u] + w[u];
   }
 }
 
@@ -533,14 +593,35 @@ static Layout layout(int B, int Lmax, int Hq, int Hkv, int D, bool mass) {
   return w;
 }
 
+// CTAs per SM of a kernel with this much shared memory, asked once per kernel, device and group size.
+template <typename E, int D, int NT, bool MASS>
+static int occupancy(int G, size_t smem, int* out) {
+  constexpr int kDevices = 64;
+  static std::mutex mu;
+  static int known[kDevices][17] = {};
+  int dev = 0;
+  FK_CHECK_CUDA(cudaGetDevice(&dev));
+  FK_CHECK_ARG(dev >= 0 && dev < kDevices, "device index too large");
+  std::lock_guard<std::mutex> lock(mu);
+  if (known[dev][G] == 0) {
+    auto kern = attend_kernel<E, D, NT, MASS>;
+    // The largest any group size asks for: the attribute is the kernel's, not the launch's.
+    FK_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       (int)attend_smem<D, NT>(NT * 8)));
+    int occ = 0;
+    FK_CHECK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kern, kThreads, smem));
+    known[dev][G] = occ < 1 ? 1 : occ;
+  }
+  *out = known[dev][G];
+  return kOk;
+}
+
 template <typename E, int D, int NT, bool MASS>
 static int launch_attend(const Params& p, cudaStream_t st) {
-  auto kern = attend_kernel<E, D, NT, MASS>;
-  const size_t smem = (size_t)NW * stages<D>() * stage_bytes<D>() + (size_t)(2 * NW * NT * 8 + NW * p.G * D) * 4;
-  FK_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  const size_t smem = attend_smem<D, NT>(p.G);
   int occ = 0;
-  FK_CHECK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kern, kThreads, smem));
-  if (occ < 1) occ = 1;
+  int rc = occupancy<E, D, NT, MASS>(p.G, smem, &occ);
+  if (rc) return rc;
   long long grid = (long long)num_sms() * occ;
   const long long units = (long long)p.B * p.Hkv * ((p.Lmax + p.chunk - 1) / p.chunk);
   if (grid > units) grid = units;
@@ -554,13 +635,16 @@ static int launch_attend(const Params& p, cudaStream_t st) {
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  FK_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, p));
-  const int merge_blocks = (p.B * p.Hq + 3) / 4;
+  FK_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attend_kernel<E, D, NT, MASS>, p));
+  constexpr int kRows = kFinishThreads / 32;
+  const int merge_blocks = (p.B * p.Hq + kRows - 1) / kRows;
   const int stretches = (p.Lmax + kMassTokens - 1) / kMassTokens;
   const long long blocks = merge_blocks + (MASS ? (long long)p.B * p.Hkv * stretches : 0);
   cfg.gridDim = dim3((unsigned)blocks, 1, 1);
+  cfg.blockDim = dim3(kFinishThreads, 1, 1);
   cfg.dynamicSmemBytes = 0;
-  FK_CHECK_CUDA(cudaLaunchKernelEx(&cfg, finish_kernel<E, D>, p, merge_blocks, stretches));
+  FK_CHECK_CUDA(cudaLaunchKernelEx(&cfg, finish_kernel<E, D>, p, merge_blocks, FastDiv::of(stretches),
+                                   FastDiv::of(p.Hq), FastDiv::of(p.Hkv)));
   return kOk;
 }
 

@@ -11,14 +11,20 @@
 // Bound: HBM. Every mass is read once (4 bytes), every kept token's K and V row
 // is read and written once.
 //
-// `select_kernel`: a cluster of CL CTAs per (row, kv head) finds the threshold
-// mass by radix selection: floats map to order-preserving unsigned keys, and
-// four passes narrow the key of the r-th greatest 8 bits at a time. Each CTA
-// counts the digits of its stretch in shared memory, all CTAs read all counts
-// through distributed shared memory and draw the same conclusion, so a pass is
-// one cluster barrier. Then each warp counts what it keeps, one scan over the
-// cluster's warps gives every warp its place, and kept positions and masses are
-// written in order. No atomics decide an order: results do not depend on timing.
+// `select_kernel`: a cluster of CL CTAs per (row, kv head) finds the threshold mass
+// by radix selection. Floats map to order-preserving unsigned keys, kept in
+// registers (each warp owns a contiguous stretch of the candidates). Starting from
+// the interval [least key, greatest key], a pass counts the keys in 1024 equal
+// parts of the interval and goes on with the part that holds the want-th greatest,
+// until the part is one key or holds exactly the keys still wanted: at most four
+// passes, two or three in practice. Starting from the keys' own range instead of
+// their top bits spreads the counts: masses share few exponents, and equal bins
+// serialise the shared-memory atomics. Each CTA counts its stretch, all CTAs
+// read all counts through distributed shared memory and draw the same conclusion,
+// so a pass is one cluster barrier. Then each warp counts what it keeps, one scan
+// over the cluster's warps gives every warp its place, and kept positions and
+// masses are written in order. No atomics decide an order: results do not depend
+// on timing.
 //
 // `gather_kernel` (a programmatic dependent): copies the kept rows, 16 bytes per
 // thread and cache, neighbouring threads along the heads of one output token.
@@ -34,7 +40,8 @@ namespace cg = cooperative_groups;
 
 constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
-constexpr int kBins = 256;
+constexpr int kBins = kThreads;  // one per thread
+constexpr int kBinBits = 10;
 constexpr int kMaxCluster = 8;
 
 struct Params {
@@ -54,6 +61,8 @@ struct Params {
   long long out_mass_cap;
   int* kept;                 // [B, Hkv, budget], -1 behind the new length
   int B, Lmax, Hkv, row_bytes, budget, sinks, recent;
+  FastDiv heads;             // by Hkv
+  int cl_log;                // log2 of the CTAs per cluster
 };
 
 __device__ __forceinline__ int seq_len(const Params& p, int b) {
@@ -68,18 +77,22 @@ __device__ __forceinline__ uint32_t mass_key(float f) {
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-__global__ void __launch_bounds__(kThreads) select_kernel(const Params p) {
-  __shared__ int s_hist[2][kBins];   // this CTA's digit counts, double-buffered over the passes
-  __shared__ int s_tot[kBins];       // the cluster's
-  __shared__ int s_digit, s_above;
+// KEYS: keys per lane kept in registers; 0: any number, read again from memory in every pass.
+template <int KEYS>
+__global__ void __launch_bounds__(kThreads, 1) select_kernel(const Params p) {
+  __shared__ int s_hist[2][kBins];  // this CTA's counts, double-buffered over the passes
+  __shared__ uint32_t s_min[kWarps], s_max[kWarps];
+  __shared__ uint32_t s_range[2];   // this CTA's least and greatest key
+  __shared__ int s_warp[kWarps];    // sums of the scan
+  __shared__ int s_bin, s_above, s_count;
   __shared__ int s_gt[kWarps], s_tie[kWarps];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   cg::cluster_group cluster = cg::this_cluster();
   const int cl = cluster.num_blocks(), rank = cluster.block_rank();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int pair = blockIdx.x / cl;
-  const int b = pair / p.Hkv, h = pair - b * p.Hkv;
+  const int pair = blockIdx.x >> p.cl_log;
+  const int b = p.heads.div(pair), h = pair - b * p.Hkv;
   const int len = seq_len(p, b);
   const int kept = min(len, p.budget);
   const float* mass = p.mass + (size_t)pair * p.mass_cap;
@@ -110,104 +123,148 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const Params p) {
   }
   if (want == 0) return;
 
-  // Each warp of the cluster owns a contiguous stretch of the candidates.
-  const int warps = cl * kWarps, gw = rank * kWarps + warp;
-  const int seg = ((m + warps - 1) / warps + 31) & ~31;
+  // Each warp of the cluster owns a contiguous stretch of the candidates, a whole number of
+  // rounds of 32.
+  const int gw = rank * kWarps + warp;
+  const int seg = (((m + 31) >> 5) + cl * kWarps - 1 >> (p.cl_log + 5)) << 5;
   const int w0 = min(gw * seg, m), w1 = min(w0 + seg, m);
   mass += first;
-
-  uint32_t prefix = 0, mask = 0;  // the digits of the threshold key found so far
-  int above = 0;                  // candidates with a greater key than every key with this prefix
-  for (int pass = 0; pass < 4; ++pass) {
-    const int shift = 24 - 8 * pass;
-    int* hist = s_hist[pass & 1];
-    for (int i = threadIdx.x; i < kBins; i += kThreads) hist[i] = 0;
-    __syncthreads();
-    for (int i = w0 + lane; i < w1; i += 32) {
-      const uint32_t key = mass_key(__ldg(mass + i));
-      if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1);
-    }
-    cluster.sync();
-    // The other buffer is free to be cleared in the next pass: whoever read it has
-    // passed this barrier.
-    if (threadIdx.x < kBins) {
-      int n = 0;
-      for (int q = 0; q < cl; ++q) n += cluster.map_shared_rank(hist, q)[threadIdx.x];
-      s_tot[threadIdx.x] = n;
-    }
-    __syncthreads();
-    if (warp == 0) {
-      // The digit in which the want-th greatest lies: lane l holds digits [8l, 8l + 8), suffix sums over lanes.
-      int own[8], sum = 0;
+  float reg[KEYS > 0 ? KEYS : 1];
+  if constexpr (KEYS > 0) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        own[i] = s_tot[lane * 8 + i];
-        sum += own[i];
-      }
-      int suffix = sum;  // sum over lanes >= this one
-#pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const int o = __shfl_down_sync(0xffffffffu, suffix, off);
-        if (lane + off < 32) suffix += o;
-      }
-      int over = above + suffix - sum;  // candidates of greater digits than this lane's
-      const int need = want;
-      if (over < need && need <= over + sum) {
-#pragma unroll
-        for (int i = 7; i >= 0; --i) {
-          if (over < need && need <= over + own[i]) {
-            s_digit = lane * 8 + i;
-            s_above = over;
-          }
-          over += own[i];
-        }
-      }
+    for (int u = 0; u < KEYS; ++u) {
+      const int i = w0 + u * 32 + lane;
+      reg[u] = i < w1 ? __ldg(mass + i) : 0.f;
     }
-    __syncthreads();
-    prefix |= (uint32_t)s_digit << shift;
-    mask |= 0xFFu << shift;
-    above = s_above;
   }
-  // Keys above `prefix` all stay (`above` of them); of the equal ones the first want - above.
-  const int ties = want - above;
+  // Calls f(value, index) for this lane's candidates, in order; whole warps, with `valid`.
+  auto each = [&](auto f) {
+    if constexpr (KEYS > 0) {
+#pragma unroll
+      for (int u = 0; u < KEYS; ++u) {
+        if (w0 + u * 32 < w1) f(reg[u], w0 + u * 32 + lane, w0 + u * 32 + lane < w1);
+      }
+    } else {
+      for (int i0 = w0; i0 < w1; i0 += 32) {
+        const int i = i0 + lane;
+        f(i < w1 ? __ldg(mass + i) : 0.f, i, i < w1);
+      }
+    }
+  };
+  auto sync_all = [&]() {
+    if (cl > 1) cluster.sync(); else __syncthreads();
+  };
+
+  // ---- the keys' range ----
+  uint32_t lo = 0xFFFFFFFFu, hi = 0u;
+  each([&](float f, int, bool valid) {
+    const uint32_t key = mass_key(f);
+    lo = valid ? min(lo, key) : lo;
+    hi = valid ? max(hi, key) : hi;
+  });
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  if (lane == 0) {
+    s_min[warp] = lo;
+    s_max[warp] = hi;
+  }
+  s_hist[0][threadIdx.x] = 0;
+  __syncthreads();
+  if (warp == 0) {
+    lo = __reduce_min_sync(0xffffffffu, s_min[lane]);
+    hi = __reduce_max_sync(0xffffffffu, s_max[lane]);
+    if (lane == 0) {
+      s_range[0] = lo;
+      s_range[1] = hi;
+    }
+  }
+  sync_all();
+  lo = s_range[0];
+  hi = s_range[1];
+  for (int q = 0; q < cl && cl > 1; ++q) {
+    const uint32_t* r = cluster.map_shared_rank(s_range, q);
+    lo = min(lo, r[0]);
+    hi = max(hi, r[1]);
+  }
+
+  // ---- narrow [lo, lo + 2^width) to the want-th greatest key ----
+  int width = 32 - __clz(hi - lo);  // bits of the interval
+  int above = 0;                    // candidates above the interval
+  int inside = m;                   // candidates in it
+  for (int pass = 0; width > 0 && inside > want - above; ++pass) {
+    const int shift = max(0, width - kBinBits);
+    int* hist = s_hist[pass & 1];
+    each([&](float f, int, bool valid) {
+      const uint32_t d = mass_key(f) - lo;
+      if (valid && d <= hi - lo) atomicAdd(&hist[d >> shift], 1);
+    });
+    sync_all();
+    int n = hist[threadIdx.x];
+    if (cl > 1) {
+      n = 0;
+      for (int q = 0; q < cl; ++q) n += cluster.map_shared_rank(hist, q)[threadIdx.x];
+    }
+    // The other buffer is free: whoever read it in the pass before has passed this barrier.
+    s_hist[(pass & 1) ^ 1][threadIdx.x] = 0;
+    // Candidates in greater bins: bin t of thread t, a suffix sum.
+    int suffix = n;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int o = __shfl_down_sync(0xffffffffu, suffix, off);
+      if (lane + off < 32) suffix += o;
+    }
+    if (lane == 0) s_warp[warp] = suffix;
+    __syncthreads();
+    int later = lane > warp ? s_warp[lane] : 0;
+    later = __reduce_add_sync(0xffffffffu, later);
+    const int over = above + later + suffix - n;
+    if (over < want && want <= over + n) {
+      s_bin = threadIdx.x;
+      s_above = over;
+      s_count = n;
+    }
+    __syncthreads();
+    lo += (uint32_t)s_bin << shift;
+    hi = min(hi, lo + (shift == 0 ? 0u : (0xFFFFFFFFu >> (32 - shift))));
+    width = shift;
+    above = s_above;
+    inside = s_count;
+  }
+  // All keys above the interval stay. Either all that are left in it are wanted, or it is one key,
+  // of which the earliest want - above stay.
+  const bool whole = inside == want - above;
+  const int ties = whole ? 0 : want - above;
+  const uint32_t least = whole ? lo : lo + 1;  // keys >= least stay; 0 (lo is NaN's key): none
 
   int n_gt = 0, n_tie = 0;
-  for (int i = w0 + lane; i < w1; i += 32) {
-    const uint32_t key = mass_key(__ldg(mass + i));
-    n_gt += key > prefix;
-    n_tie += key == prefix;
-  }
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    n_gt += __shfl_xor_sync(0xffffffffu, n_gt, off);
-    n_tie += __shfl_xor_sync(0xffffffffu, n_tie, off);
-  }
+  each([&](float f, int, bool valid) {
+    const uint32_t key = mass_key(f);
+    n_gt += valid && key >= least && least != 0u;
+    n_tie += valid && !whole && key == lo;
+  });
+  n_gt = __reduce_add_sync(0xffffffffu, n_gt);
+  n_tie = __reduce_add_sync(0xffffffffu, n_tie);
   if (lane == 0) {
     s_gt[warp] = n_gt;
     s_tie[warp] = n_tie;
   }
-  cluster.sync();
+  sync_all();
   // What the warps before this one hold.
   int b_gt = 0, b_tie = 0;
   for (int q = 0; q <= rank; ++q) {
-    const int* gq = cluster.map_shared_rank(s_gt, q);
-    const int* tq = cluster.map_shared_rank(s_tie, q);
+    const int* gq = cl > 1 ? cluster.map_shared_rank(s_gt, q) : s_gt;
+    const int* tq = cl > 1 ? cluster.map_shared_rank(s_tie, q) : s_tie;
     if (q < rank || lane < warp) {
       b_gt += gq[lane];
       b_tie += tq[lane];
     }
   }
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    b_gt += __shfl_xor_sync(0xffffffffu, b_gt, off);
-    b_tie += __shfl_xor_sync(0xffffffffu, b_tie, off);
-  }
+  b_gt = __reduce_add_sync(0xffffffffu, b_gt);
+  b_tie = __reduce_add_sync(0xffffffffu, b_tie);
   const uint32_t below = (1u << lane) - 1u;
-  for (int i0 = w0; i0 < w1; i0 += 32) {
-    const int i = i0 + lane;
-    const float f = i < w1 ? __ldg(mass + i) : 0.f;
+  each([&](float f, int i, bool valid) {
     const uint32_t key = mass_key(f);
-    const bool gt = i < w1 && key > prefix, tie = i < w1 && key == prefix;
+    const bool gt = valid && key >= least && least != 0u, tie = valid && !whole && key == lo;
     const uint32_t bg = __ballot_sync(0xffffffffu, gt), bt = __ballot_sync(0xffffffffu, tie);
     const int tie_rank = b_tie + __popc(bt & below);
     if (gt || (tie && tie_rank < ties)) {
@@ -217,8 +274,8 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const Params p) {
     }
     b_gt += __popc(bg);
     b_tie += __popc(bt);
-  }
-  cluster.sync();  // no CTA leaves while another reads its counts
+  });
+  if (cl > 1) cluster.sync();  // no CTA leaves while another reads its counts
 }
 
 constexpr int kGatherThreads = 256;
@@ -292,11 +349,16 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const Params p, 
   }
 }
 
-static int launch(const Params& p, cudaStream_t st) {
+static int launch(Params p, cudaStream_t st) {
   // CTAs per (row, head): enough that the pairs fill the SMs, as long as each warp
   // still has 32 candidates of the longest row.
-  int cl = 1;
-  while (cl < kMaxCluster && (long long)p.B * p.Hkv * cl < num_sms() && p.Lmax > cl * kThreads) cl *= 2;
+  p.cl_log = 0;
+  while ((1 << p.cl_log) < kMaxCluster && ((long long)p.B * p.Hkv << p.cl_log) < num_sms() &&
+         p.Lmax > (kThreads << p.cl_log))
+    ++p.cl_log;
+  const int cl = 1 << p.cl_log;
+  p.heads = FastDiv::of(p.Hkv);
+  const int keys = (p.Lmax + cl * kThreads - 1) / (cl * kThreads);  // per lane, of a row as long as can be
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -310,7 +372,12 @@ static int launch(const Params& p, cudaStream_t st) {
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  FK_CHECK_CUDA(cudaLaunchKernelEx(&cfg, select_kernel, p));
+  if (keys <= 4)
+    FK_CHECK_CUDA(cudaLaunchKernelEx(&cfg, select_kernel<4>, p));
+  else if (keys <= 32)
+    FK_CHECK_CUDA(cudaLaunchKernelEx(&cfg, select_kernel<32>, p));
+  else
+    FK_CHECK_CUDA(cudaLaunchKernelEx(&cfg, select_kernel<0>, p));
   GatherPlan g;
   g.slots = p.budget < p.Lmax ? p.budget : p.Lmax;
   const int per_row = p.row_bytes / 16, per_tok = p.Hkv * per_row;
