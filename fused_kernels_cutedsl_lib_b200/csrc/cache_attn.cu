@@ -8,21 +8,21 @@
 // Bound: HBM, 4 * D bytes per (token, kv head), plus 8 bytes of mass and the
 // scores' round trip described below.
 //
-// Pass 1 (`attend_kernel`): a persistent grid walks units (row b, kv head h,
-// split of `chunk` tokens). Four warps each take 16 tokens of every 64-token
-// tile and own a private ring of K/V stages filled by their own 16-byte
-// cp.async copies, so no barrier is needed inside a unit, and each token's
-// address comes from its own page: pages may have any size. The load side runs
-// STAGES - 1 tiles ahead of the arithmetic, across units. Tokens are the M side
-// of mma.sync m16n8k16 and the group's query heads the N side (NT tiles of 8),
-// so a K/V byte is read once for all heads that share it. Each warp keeps its
-// own running maximum and sum (fp32, log2 domain); the four are merged at the
-// end of a unit. P is multiplied as a sum of two 16-bit numbers (its rounding and
-// the rounding of the rest): the products cost nothing next to the loads, and the
-// output's error is then that of its own rounding instead of sqrt(2) times it.
-// With a mass, the raw log2-domain scores go to scratch as fp32 (4 bytes per
-// token and q head), because a token's weight is known only with the lse of the
-// whole row.
+// Pass 1 (`attend_kernel`): units (row b, kv head h, split of `chunk` tokens) are
+// dealt round-robin to the warps of a persistent grid. A warp works alone: it
+// streams its 16-token tiles through a private ring filled by its own 16-byte
+// cp.async copies and writes its unit's partial itself, so there is no barrier
+// in the kernel (a merge of four warps per unit, tried first, drained the loads
+// for 1.5 us per unit). Each token's address comes from its own page: pages may
+// have any size. The load side runs STAGES - 1 tiles ahead of the arithmetic,
+// across units. Tokens are the M side of mma.sync m16n8k16 and the group's query
+// heads the N side (NT tiles of 8), so a K/V byte is read once for all heads that
+// share it. Running maximum and sum are fp32, in the log2 domain. P is multiplied as
+// a sum of two 16-bit numbers (its rounding and the rounding of the rest): the products
+// cost nothing next to the loads, and the output's error is then that of its own
+// rounding instead of sqrt(2) times it. With a mass, the raw log2-domain scores go
+// to scratch as fp32 (4 bytes per token and q head), because a token's weight is
+// known only with the lse of the whole row.
 //
 // Pass 2 (`finish_kernel`, a programmatic dependent): blocks that merge the
 // splits of each (row, q head) into out and lse, and blocks that turn a stretch
@@ -41,8 +41,8 @@
 namespace fk {
 namespace cattn {
 
-constexpr int T = 64;   // tokens per tile
-constexpr int NW = 4;   // warps, 16 tokens of a tile each
+constexpr int T = 16;   // tokens per tile
+constexpr int NW = 4;   // warps per CTA
 constexpr int kThreads = NW * 32;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.69314718055994531f;
@@ -65,7 +65,8 @@ struct Params {
   long long mass_cap;
   void* out;                // [B, Hq, D]
   float* lse;               // [B, Hq]
-  int B, Lmax, Hq, Hkv, G, chunk, chunk_log;  // chunk: a power of two
+  int B, Lmax, Hq, Hkv, G;
+  FastDiv chunk;            // tokens per split, a multiple of 16
   float scale_log2;
 };
 
@@ -119,8 +120,10 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   return r;
 }
 
-// The tiles a CTA works on, in order: units (b, h, split) dealt round-robin over
-// the grid, and the 64-token tiles of each.
+__device__ __forceinline__ int num_splits(const Params& p, int len) { return p.chunk.div(len + p.chunk.d - 1); }
+
+// The tiles a warp works on, in order: units (b, h, split) dealt round-robin over the
+// grid's warps, and the 16-token tiles of each.
 struct TileIter {
   long long u, base;  // current unit, first unit of row b
   int b, nb, len;     // row, its splits and length
@@ -129,7 +132,7 @@ struct TileIter {
   bool valid;
   __device__ __forceinline__ void row(const Params& p) {
     len = seq_len(p, b);
-    nb = (len + p.chunk - 1) >> p.chunk_log;
+    nb = num_splits(p, len);
   }
   __device__ __forceinline__ void locate(const Params& p) {
     while (true) {
@@ -145,11 +148,11 @@ struct TileIter {
     const int r = (int)(u - base);
     h = r / nb;
     s = r - h * nb;
-    t = s * p.chunk;
-    t1 = min(t + p.chunk, len);
+    t = s * p.chunk.d;
+    t1 = min(t + p.chunk.d, len);
   }
   __device__ __forceinline__ void init(const Params& p) {
-    u = blockIdx.x;
+    u = (long long)blockIdx.x * NW + (threadIdx.x >> 5);
     base = 0;
     b = 0;
     valid = true;
@@ -159,7 +162,7 @@ struct TileIter {
   __device__ __forceinline__ void next(const Params& p) {
     t += T;
     if (t >= t1) {
-      u += gridDim.x;
+      u += (long long)gridDim.x * NW;
       locate(p);
     }
   }
@@ -167,20 +170,18 @@ struct TileIter {
 
 template <int D>
 __host__ __device__ constexpr int stage_bytes() { return 2 * 16 * D * 2; }  // one warp's K and V of 16 tokens
+// Stages of a warp's ring: 96 KB per CTA, two CTAs per SM. At D = 64 more warps with fewer stages
+// (4 CTAs of 3, 3 of 4) measured 5-10 % slower on a large batch than 2 of 6.
 template <int D>
-__host__ __device__ constexpr int stages() { return D == 128 ? 3 : 5; }
-
-// The warps' rings, and room to merge their softmax states for G query heads.
-template <int D, int NT>
-__host__ __device__ constexpr size_t attend_smem(int G) {
-  return (size_t)NW * stages<D>() * stage_bytes<D>() + (size_t)(2 * NW * NT * 8 + NW * G * D) * 4;
-}
+__host__ __device__ constexpr int stages() { return D == 128 ? 3 : 6; }
+constexpr int kCtas = 2;
+template <int D>
+__host__ __device__ constexpr int attend_smem() { return NW * stages<D>() * stage_bytes<D>(); }
 
 template <typename E, int D, int NT, bool MASS>
-__global__ void __launch_bounds__(kThreads, 2) attend_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, kCtas) attend_kernel(const Params p) {
   using El = Elem<E>;
   constexpr int S = stages<D>();
-  constexpr int HALVES = D / 64;  // 128-byte row halves of a tile row
   constexpr int KS = D / 16;
   constexpr int LPR = D / 8;      // lanes (16-byte pieces) per token row
   constexpr int RPI = 32 / LPR;   // rows per copy instruction
@@ -188,13 +189,9 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const Params p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
   const int j = lane >> 3, r = lane & 7;
-  const int tw = warp * 16;
   const float NEG_INF = -INFINITY;
   const int G = p.G;
   const uint32_t ring = smem_u32(smem) + warp * S * stage_bytes<D>();
-  float* cm = reinterpret_cast<float*>(smem + NW * S * stage_bytes<D>());  // [NW][NT * 8] row max
-  float* cl = cm + NW * NT * 8;                                            // [NW][NT * 8] row sum
-  float* co = cl + NW * NT * 8;                                            // [NW][G][D]
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -207,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const Params p) {
   // one tile ahead, so the page lookup's latency is off the copies' path.
   auto resolve = [&]() -> int {
     if (!ld.valid) return -1;
-    const int t = ld.t + tw + (lane & 15);
+    const int t = ld.t + (lane & 15);
     if (t >= ld.t1) return -1;
     if (p.block_table == nullptr) return ld.b * p.Lmax + t;
     const int pg = p.page.div(t);
@@ -291,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const Params p) {
         for (int nt = 0; nt < NT; ++nt) El::mma(sc[nt], a, qf[nt][ks][0], qf[nt][ks][1]);
       }
 
-      const int nv = t1 - (t + tw);  // valid tokens among this warp's 16
+      const int nv = t1 - t;  // valid tokens among the 16
       uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -299,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const Params p) {
         const float x2 = sc[nt][2] * p.scale_log2, x3 = sc[nt][3] * p.scale_log2;
         if (MASS) {
           const int h0 = nt * 8 + 2 * c;
-          float* dst = p.scores + (((size_t)b * p.Hkv + h) * p.Lmax + (t + tw + g)) * p.gs + h0;
+          float* dst = p.scores + (((size_t)b * p.Hkv + h) * p.Lmax + (t + g)) * p.gs + h0;
           if (p.gs > 1) {  // gs is even: a pair of heads per store
             if (h0 < p.gs) {
               if (g < nv) *reinterpret_cast<float2*>(dst) = make_float2(x0, x1);
@@ -361,7 +358,9 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const Params p) {
       it.next(p);
     } while (!last);
 
-    // ---- merge the four warps' softmax states and write the split's partial ----
+    // ---- the unit's partial: O normalised, and its lse. A sum of exactly 0 means that every
+    // score was -inf; NaN scores give a NaN sum and go on to the output. ----
+    const size_t row0 = ((size_t)split * p.B + b) * p.Hq + (size_t)h * G;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -369,48 +368,21 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const Params p) {
         l[nt][0] += __shfl_xor_sync(0xffffffffu, l[nt][0], off);
         l[nt][1] += __shfl_xor_sync(0xffffffffu, l[nt][1], off);
       }
-      const int h0 = nt * 8 + 2 * c;
-      if (g == 0) {
-        cm[warp * NT * 8 + h0] = m[nt][0];
-        cm[warp * NT * 8 + h0 + 1] = m[nt][1];
-        cl[warp * NT * 8 + h0] = l[nt][0];
-        cl[warp * NT * 8 + h0 + 1] = l[nt][1];
-      }
 #pragma unroll
-      for (int i = 0; i < KS; ++i) {
-        if (h0 < G) {
-          float* dst = co + ((size_t)warp * G + h0) * D + 16 * i + g;
-          dst[0] = o[nt][i][0];
-          dst[8] = o[nt][i][2];
+      for (int e = 0; e < 2; ++e) {
+        const int hh = nt * 8 + 2 * c + e;
+        if (hh >= G) continue;
+        const float L = l[nt][e];
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        float* dst = p.o_part + (row0 + hh) * D + g;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          dst[16 * i] = o[nt][i][e] * inv;
+          dst[16 * i + 8] = o[nt][i][e + 2] * inv;
         }
-        if (h0 + 1 < G) {
-          float* dst = co + ((size_t)warp * G + h0 + 1) * D + 16 * i + g;
-          dst[0] = o[nt][i][1];
-          dst[8] = o[nt][i][3];
-        }
+        if (g == 0) p.lse_part[row0 + hh] = L == 0.f ? NEG_INF : m[nt][e] + log2f(L);
       }
     }
-    __syncthreads();
-    const size_t row0 = ((size_t)split * p.B + b) * p.Hq + (size_t)h * G;
-    for (int e = threadIdx.x; e < G * D; e += kThreads) {
-      const int hh = e / D, d = e % D;
-      float M = NEG_INF;
-#pragma unroll
-      for (int w = 0; w < NW; ++w) M = fmaxf(M, cm[w * NT * 8 + hh]);
-      // fmaxf passes over NaN, the sums do not: NaN scores reach the output, and a
-      // sum of exactly 0 means that every score was -inf.
-      const float ms = M == NEG_INF ? 0.f : M;
-      float L = 0.f, acc = 0.f;
-#pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        const float sw = exp2f(cm[w * NT * 8 + hh] - ms);
-        L += sw * cl[w * NT * 8 + hh];
-        acc += sw * co[((size_t)w * G + hh) * D + d];
-      }
-      p.o_part[(row0 + hh) * D + d] = L == 0.f ? 0.f : acc / L;
-      if (d == 0) p.lse_part[row0 + hh] = L == 0.f ? NEG_INF : M + log2f(L);
-    }
-    __syncthreads();
   }
   cp_async_wait<0>();
 }
@@ -436,78 +408,116 @@ constexpr int kFinishThreads = 256;
 constexpr int kMassUnroll = 4;                                // tokens of a thread whose loads are in flight together
 constexpr int kMassTokens = kFinishThreads * kMassUnroll;     // tokens per mass block
 
-// Blocks [0, merge_blocks): eight (row, q head) pairs each, one per warp, merge the
-// splits. The others: one stretch of kMassTokens tokens of one (row, kv head). Both read
-// what pass 1 left, mostly in L2, and are short: what matters is that all loads of a
-// thread are issued before the first is used.
+// One (row, q head)'s lse in the log2 domain from the splits'. Whole warps.
+__device__ __forceinline__ float merge_lse(const float* src, size_t plane, int n, int lane) {
+  float M = -INFINITY, W = 0.f;
+  for (int s0 = 0; s0 < n; s0 += 128) {
+    float x[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int s = s0 + u * 32 + lane;
+      x[u] = s < n ? __ldg(src + s * plane) : -INFINITY;
+    }
+    // fmaxf passes over NaN, the sum does not.
+    const float top = fmaxf(fmaxf(M, fmaxf(x[0], x[1])), fmaxf(x[2], x[3]));
+    const float ts = top == -INFINITY ? 0.f : top;
+    W = W * exp2f(M - ts) + ((exp2f(x[0] - ts) + exp2f(x[1] - ts)) + (exp2f(x[2] - ts) + exp2f(x[3] - ts)));
+    M = top;
+  }
+  float top = M;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+  const float ts = top == -INFINITY ? 0.f : top;
+  W *= exp2f((M == -INFINITY ? ts : M) - ts);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) W += __shfl_xor_sync(0xffffffffu, W, off);
+  return W == 0.f ? -INFINITY : top + log2f(W);
+}
+
+// Blocks [0, merge_blocks) merge splits: 8 >> wpr_log (row, q head) pairs each, with
+// 1 << wpr_log warps per pair. The others: one stretch of kMassTokens tokens of one (row,
+// kv head). Both read what pass 1 left, mostly in L2, and are short: what matters is that
+// a thread's loads are issued before the first is used.
 template <typename E, int D>
-__global__ void __launch_bounds__(kFinishThreads) finish_kernel(const Params p, int merge_blocks, FastDiv stretches,
-                                                                FastDiv heads_q, FastDiv heads_kv) {
+__global__ void __launch_bounds__(kFinishThreads) finish_kernel(const Params p, int merge_blocks, int wpr_log,
+                                                                FastDiv stretches, FastDiv heads_q, FastDiv heads_kv) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  constexpr int kWarps = kFinishThreads / 32;
+  __shared__ float s_acc[kWarps][D];
+  __shared__ float s_lse[16];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const size_t plane = (size_t)p.B * p.Hq;
   if ((int)blockIdx.x < merge_blocks) {
-    const int row = blockIdx.x * (kFinishThreads / 32) + warp;
-    if (row >= p.B * p.Hq) return;
-    const int b = heads_q.div(row);
-    const int n = (seq_len(p, b) + p.chunk - 1) >> p.chunk_log;
+    const int wpr = 1 << wpr_log, part = warp & (wpr - 1);
+    const int row = blockIdx.x * (kWarps >> wpr_log) + (warp >> wpr_log);
+    const bool in_range = row < p.B * p.Hq;
     constexpr int PER = D / 32;  // dims per lane
-    constexpr int CH = 8;        // splits whose loads are in flight together; summed in split order
-    float ls[CH], v[CH][PER];
-    auto load = [&](int s0) {
-#pragma unroll
-      for (int u = 0; u < CH; ++u) {
-        const bool in = s0 + u < n;
-        ls[u] = in ? __ldg(p.lse_part + (s0 + u) * plane + row) : -INFINITY;
-        const float* src = p.o_part + ((s0 + u) * plane + row) * D + PER * lane;
-        if constexpr (PER == 4) {
-          const float4 f = in ? __ldg(reinterpret_cast<const float4*>(src)) : make_float4(0.f, 0.f, 0.f, 0.f);
-          v[u][0] = f.x, v[u][1] = f.y, v[u][2] = f.z, v[u][3] = f.w;
-        } else {
-          const float2 f = in ? __ldg(reinterpret_cast<const float2*>(src)) : make_float2(0.f, 0.f);
-          v[u][0] = f.x, v[u][1] = f.y;
-        }
-      }
-    };
-    load(0);
-    float M = -INFINITY;
-    for (int s = lane; s < n; s += 32) M = fmaxf(M, __ldg(p.lse_part + s * plane + row));
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-    const float ms = M == -INFINITY ? 0.f : M;
-    float W = 0.f, acc[PER];
+    constexpr int CH = 8;        // splits whose loads are in flight together
+    float acc[PER], lse = -INFINITY;
 #pragma unroll
     for (int i = 0; i < PER; ++i) acc[i] = 0.f;
-    for (int s0 = 0; s0 < n; s0 += CH) {
-      if (s0 > 0) load(s0);
+    if (in_range) {
+      const int n = num_splits(p, seq_len(p, heads_q.div(row)));
+      float ls[CH], v[CH][PER];
+      // Splits part, part + wpr, ..: each warp's in order, then the warps' in order.
+      auto load = [&](int s0) {
 #pragma unroll
-      for (int u = 0; u < CH; ++u) {
-        if (s0 + u < n) {
-          const float w = exp2f(ls[u] - ms);
-          W += w;
+        for (int u = 0; u < CH; ++u) {
+          const int s = s0 + u * wpr;
+          const bool in = s < n;
+          ls[u] = in ? __ldg(p.lse_part + s * plane + row) : -INFINITY;
+          const float* src = p.o_part + (s * plane + row) * D + PER * lane;
+          if constexpr (PER == 4) {
+            const float4 f = in ? __ldg(reinterpret_cast<const float4*>(src)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            v[u][0] = f.x, v[u][1] = f.y, v[u][2] = f.z, v[u][3] = f.w;
+          } else {
+            const float2 f = in ? __ldg(reinterpret_cast<const float2*>(src)) : make_float2(0.f, 0.f);
+            v[u][0] = f.x, v[u][1] = f.y;
+          }
+        }
+      };
+      load(part);
+      lse = merge_lse(p.lse_part + row, plane, n, lane);
+      // The weights add up to 1: split s has exp2(lse_s - lse).
+      const float z = lse == -INFINITY ? 0.f : lse;
+      for (int s0 = part; s0 < n; s0 += CH * wpr) {
+        if (s0 > part) load(s0);
 #pragma unroll
-          for (int i = 0; i < PER; ++i) acc[i] += w * v[u][i];
+        for (int u = 0; u < CH; ++u) {
+          if (s0 + u * wpr < n) {
+            const float w = exp2f(ls[u] - z);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) acc[i] += w * v[u][i];
+          }
         }
       }
     }
-    const bool none = W == 0.f;
-    const float inv = none ? 0.f : 1.f / W;
+    if (wpr > 1) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) s_acc[warp][PER * lane + i] = acc[i];
+      __syncthreads();
+      if (part != 0 || !in_range) return;
+      for (int w = 1; w < wpr; ++w) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) acc[i] += s_acc[warp + w][PER * lane + i];
+      }
+    }
+    if (!in_range) return;
     uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<E*>(p.out) + (size_t)row * D + PER * lane);
 #pragma unroll
-    for (int i = 0; i < PER / 2; ++i) dst[i] = Elem<E>::pack(acc[2 * i] * inv, acc[2 * i + 1] * inv);
-    if (lane == 0) p.lse[row] = none ? -INFINITY : (M + log2f(W)) * kLn2;
+    for (int i = 0; i < PER / 2; ++i) dst[i] = Elem<E>::pack(acc[2 * i], acc[2 * i + 1]);
+    if (lane == 0) p.lse[row] = lse * kLn2;
     return;
   }
 
-  __shared__ float s_lse[16];
   const int i = blockIdx.x - merge_blocks;
   const int pair = stretches.div(i);
   const int t0 = (i - pair * stretches.d) * kMassTokens;
   const int b = heads_kv.div(pair), h = pair - b * p.Hkv;
   const int len = seq_len(p, b);
   if (t0 >= len) return;
-  const int n = (len + p.chunk - 1) >> p.chunk_log;
+  const int n = num_splits(p, len);
   const float* sc = p.scores + (size_t)pair * p.Lmax * p.gs;
   const size_t mrow = (size_t)pair * p.mass_cap;
   const int t1 = min(t0 + kMassTokens, len);
@@ -524,18 +534,10 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const Params p, 
     const int t = t0 + u * kFinishThreads + (int)threadIdx.x;
     first[u] = t < t1 ? load_scores(sc + (size_t)t * p.gs, 0, p.gs) : make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  for (int hh = warp; hh < p.G; hh += kFinishThreads / 32) {
-    const float* src = p.lse_part + (size_t)b * p.Hq + (size_t)h * p.G + hh;
-    float M = -INFINITY, W = 0.f;
-    for (int s = lane; s < n; s += 32) M = fmaxf(M, __ldg(src + s * plane));
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-    const float ms = M == -INFINITY ? 0.f : M;
-    for (int s = lane; s < n; s += 32) W += exp2f(__ldg(src + s * plane) - ms);
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) W += __shfl_xor_sync(0xffffffffu, W, off);
+  for (int hh = warp; hh < p.G; hh += kWarps) {
+    const float z = merge_lse(p.lse_part + (size_t)b * p.Hq + (size_t)h * p.G + hh, plane, n, lane);
     // A head whose scores are all -inf gives no weight: +inf makes exp2(-inf - inf) = 0.
-    if (lane == 0) s_lse[hh] = W == 0.f ? INFINITY : M + log2f(W);
+    if (lane == 0) s_lse[hh] = z == -INFINITY ? INFINITY : z;
   }
   __syncthreads();
   for (int h0 = 0; h0 < p.G; h0 += 4) {
@@ -558,18 +560,17 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const Params p, 
   }
 }
 
-static int chunk_tokens(int B, int Hkv, int Lmax) {
-  // The largest of 1024..64 tokens that still gives units for three quarters of the SMs.
-  int chunk = T;
-  const long long total = (long long)B * Lmax;
-  for (int cand = 1024; cand >= T; cand >>= 1) {
-    const long long units = (long long)Hkv * ((total + cand - 1) / cand);
-    if (4 * units >= 3LL * num_sms()) {
-      chunk = cand;
-      break;
-    }
-  }
-  return chunk;
+// Tokens per split. One unit per warp of the grid where the padded batch is that small,
+// but at least kMinChunk tokens, so that a unit's partial (G * D fp32) stays small next to
+// its K and V; at most kMaxChunk, which gives a large batch units enough to even out.
+constexpr int kMinChunk = 32;
+constexpr int kMaxChunk = 256;
+static int chunk_tokens(int B, int Hkv, int Lmax, int warps) {
+  const long long total = (long long)B * Lmax * Hkv;
+  long long c = (total + warps - 1) / warps;
+  c = (c + T - 1) / T * T;
+  if (c < kMinChunk) c = kMinChunk;
+  return (int)(c > kMaxChunk ? kMaxChunk : c);
 }
 
 static int score_stride(int G) { return G == 1 ? 1 : (G + 1) & ~1; }
@@ -584,7 +585,7 @@ static size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
 
 static Layout layout(int B, int Lmax, int Hq, int Hkv, int D, bool mass) {
   Layout w;
-  w.chunk = chunk_tokens(B, Hkv, Lmax);
+  w.chunk = chunk_tokens(B, Hkv, Lmax, num_sms() * kCtas * NW);
   w.splits = (Lmax + w.chunk - 1) / w.chunk;
   const size_t rows = (size_t)w.splits * B * Hq;
   w.o_bytes = round256(rows * D * 4);
@@ -593,57 +594,58 @@ static Layout layout(int B, int Lmax, int Hq, int Hkv, int D, bool mass) {
   return w;
 }
 
-// CTAs per SM of a kernel with this much shared memory, asked once per kernel, device and group size.
+// CTAs per SM, asked once per kernel and device.
 template <typename E, int D, int NT, bool MASS>
-static int occupancy(int G, size_t smem, int* out) {
+static int occupancy(int* out) {
   constexpr int kDevices = 64;
   static std::mutex mu;
-  static int known[kDevices][17] = {};
+  static int known[kDevices] = {};
   int dev = 0;
   FK_CHECK_CUDA(cudaGetDevice(&dev));
   FK_CHECK_ARG(dev >= 0 && dev < kDevices, "device index too large");
   std::lock_guard<std::mutex> lock(mu);
-  if (known[dev][G] == 0) {
+  if (known[dev] == 0) {
     auto kern = attend_kernel<E, D, NT, MASS>;
-    // The largest any group size asks for: the attribute is the kernel's, not the launch's.
-    FK_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)attend_smem<D, NT>(NT * 8)));
+    FK_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, attend_smem<D>()));
     int occ = 0;
-    FK_CHECK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kern, kThreads, smem));
-    known[dev][G] = occ < 1 ? 1 : occ;
+    FK_CHECK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kern, kThreads, attend_smem<D>()));
+    known[dev] = occ < 1 ? 1 : occ;
   }
-  *out = known[dev][G];
+  *out = known[dev];
   return kOk;
 }
 
 template <typename E, int D, int NT, bool MASS>
 static int launch_attend(const Params& p, cudaStream_t st) {
-  const size_t smem = attend_smem<D, NT>(p.G);
   int occ = 0;
-  int rc = occupancy<E, D, NT, MASS>(p.G, smem, &occ);
+  int rc = occupancy<E, D, NT, MASS>(&occ);
   if (rc) return rc;
   long long grid = (long long)num_sms() * occ;
-  const long long units = (long long)p.B * p.Hkv * ((p.Lmax + p.chunk - 1) / p.chunk);
-  if (grid > units) grid = units;
+  const int splits = (p.Lmax + p.chunk.d - 1) / p.chunk.d;
+  const long long units = (long long)p.B * p.Hkv * splits;
+  if (grid > (units + NW - 1) / NW) grid = (units + NW - 1) / NW;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid, 1, 1);
   cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = attend_smem<D>();
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   FK_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attend_kernel<E, D, NT, MASS>, p));
-  constexpr int kRows = kFinishThreads / 32;
-  const int merge_blocks = (p.B * p.Hq + kRows - 1) / kRows;
+  // One warp per (row, q head) takes 8 splits at a time; up to 8 warps share a longer row.
+  int wpr_log = 0;
+  while (wpr_log < 3 && (8 << wpr_log) < splits) ++wpr_log;
+  const int rows = (kFinishThreads / 32) >> wpr_log;
+  const int merge_blocks = (p.B * p.Hq + rows - 1) / rows;
   const int stretches = (p.Lmax + kMassTokens - 1) / kMassTokens;
   const long long blocks = merge_blocks + (MASS ? (long long)p.B * p.Hkv * stretches : 0);
   cfg.gridDim = dim3((unsigned)blocks, 1, 1);
   cfg.blockDim = dim3(kFinishThreads, 1, 1);
   cfg.dynamicSmemBytes = 0;
-  FK_CHECK_CUDA(cudaLaunchKernelEx(&cfg, finish_kernel<E, D>, p, merge_blocks, FastDiv::of(stretches),
+  FK_CHECK_CUDA(cudaLaunchKernelEx(&cfg, finish_kernel<E, D>, p, merge_blocks, wpr_log, FastDiv::of(stretches),
                                    FastDiv::of(p.Hq), FastDiv::of(p.Hkv)));
   return kOk;
 }
@@ -731,8 +733,7 @@ extern "C" int fk_cache_attn_fwd(const void* q, long long q_batch_stride, const 
   p.Hq = num_heads_q;
   p.Hkv = num_heads_kv;
   p.G = num_heads_q / num_heads_kv;
-  p.chunk = w.chunk;
-  for (p.chunk_log = 6; (1 << p.chunk_log) < w.chunk;) ++p.chunk_log;
+  p.chunk = FastDiv::of(w.chunk);
   p.scale_log2 = softmax_scale * cattn::kLog2e;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == FK_BF16)

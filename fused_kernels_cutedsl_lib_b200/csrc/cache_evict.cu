@@ -129,25 +129,24 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const Params p) {
   const int seg = (((m + 31) >> 5) + cl * kWarps - 1 >> (p.cl_log + 5)) << 5;
   const int w0 = min(gw * seg, m), w1 = min(w0 + seg, m);
   mass += first;
-  float reg[KEYS > 0 ? KEYS : 1];
+  // Keys of places past the stretch are 0, below every mass (the key of -inf is 0x007FFFFF).
+  uint32_t reg[KEYS > 0 ? KEYS : 1];
   if constexpr (KEYS > 0) {
+    float f[KEYS];
 #pragma unroll
-    for (int u = 0; u < KEYS; ++u) {
-      const int i = w0 + u * 32 + lane;
-      reg[u] = i < w1 ? __ldg(mass + i) : 0.f;
-    }
+    for (int u = 0; u < KEYS; ++u) f[u] = w0 + u * 32 + lane < w1 ? __ldg(mass + w0 + u * 32 + lane) : 0.f;
+#pragma unroll
+    for (int u = 0; u < KEYS; ++u) reg[u] = w0 + u * 32 + lane < w1 ? mass_key(f[u]) : 0u;
   }
-  // Calls f(value, index) for this lane's candidates, in order; whole warps, with `valid`.
+  // Calls f(key, index) for this lane's candidates, in order, whole warps at a time.
   auto each = [&](auto f) {
     if constexpr (KEYS > 0) {
 #pragma unroll
-      for (int u = 0; u < KEYS; ++u) {
-        if (w0 + u * 32 < w1) f(reg[u], w0 + u * 32 + lane, w0 + u * 32 + lane < w1);
-      }
+      for (int u = 0; u < KEYS; ++u) f(reg[u], w0 + u * 32 + lane);
     } else {
       for (int i0 = w0; i0 < w1; i0 += 32) {
         const int i = i0 + lane;
-        f(i < w1 ? __ldg(mass + i) : 0.f, i, i < w1);
+        f(i < w1 ? mass_key(__ldg(mass + i)) : 0u, i);
       }
     }
   };
@@ -157,11 +156,11 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const Params p) {
 
   // ---- the keys' range ----
   uint32_t lo = 0xFFFFFFFFu, hi = 0u;
-  each([&](float f, int, bool valid) {
-    const uint32_t key = mass_key(f);
-    lo = valid ? min(lo, key) : lo;
-    hi = valid ? max(hi, key) : hi;
+  each([&](uint32_t key, int) {
+    lo = min(lo, key - 1);  // 0 wraps to the greatest
+    hi = max(hi, key);
   });
+  lo += 1;
   lo = __reduce_min_sync(0xffffffffu, lo);
   hi = __reduce_max_sync(0xffffffffu, hi);
   if (lane == 0) {
@@ -194,9 +193,9 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const Params p) {
   for (int pass = 0; width > 0 && inside > want - above; ++pass) {
     const int shift = max(0, width - kBinBits);
     int* hist = s_hist[pass & 1];
-    each([&](float f, int, bool valid) {
-      const uint32_t d = mass_key(f) - lo;
-      if (valid && d <= hi - lo) atomicAdd(&hist[d >> shift], 1);
+    each([&](uint32_t key, int) {
+      const uint32_t d = key - lo;  // wraps to a great number below the interval
+      if (d <= hi - lo) atomicAdd(&hist[d >> shift], 1);
     });
     sync_all();
     int n = hist[threadIdx.x];
@@ -234,13 +233,12 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const Params p) {
   // of which the earliest want - above stay.
   const bool whole = inside == want - above;
   const int ties = whole ? 0 : want - above;
-  const uint32_t least = whole ? lo : lo + 1;  // keys >= least stay; 0 (lo is NaN's key): none
+  const uint32_t under = whole ? lo - 1 : lo;  // greater keys stay
 
   int n_gt = 0, n_tie = 0;
-  each([&](float f, int, bool valid) {
-    const uint32_t key = mass_key(f);
-    n_gt += valid && key >= least && least != 0u;
-    n_tie += valid && !whole && key == lo;
+  each([&](uint32_t key, int) {
+    n_gt += key > under;
+    n_tie += key == lo;  // all of them are above `under` if the interval stays whole
   });
   n_gt = __reduce_add_sync(0xffffffffu, n_gt);
   n_tie = __reduce_add_sync(0xffffffffu, n_tie);
@@ -262,15 +260,14 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const Params p) {
   b_gt = __reduce_add_sync(0xffffffffu, b_gt);
   b_tie = __reduce_add_sync(0xffffffffu, b_tie);
   const uint32_t below = (1u << lane) - 1u;
-  each([&](float f, int i, bool valid) {
-    const uint32_t key = mass_key(f);
-    const bool gt = valid && key >= least && least != 0u, tie = valid && !whole && key == lo;
+  each([&](uint32_t key, int i) {
+    const bool gt = key > under, tie = !whole && key == lo;
     const uint32_t bg = __ballot_sync(0xffffffffu, gt), bt = __ballot_sync(0xffffffffu, tie);
     const int tie_rank = b_tie + __popc(bt & below);
     if (gt || (tie && tie_rank < ties)) {
       const int pos = p.sinks + b_gt + __popc(bg & below) + min(tie_rank, ties);
       out[pos] = first + i;
-      mass_out[pos] = f;
+      mass_out[pos] = __ldg(mass + i);
     }
     b_gt += __popc(bg);
     b_tie += __popc(bt);
@@ -351,10 +348,10 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const Params p, 
 
 static int launch(Params p, cudaStream_t st) {
   // CTAs per (row, head): enough that the pairs fill the SMs, as long as each warp
-  // still has 32 candidates of the longest row.
+  // still has 32 candidates of the longest row; and enough that a lane's keys fit 16 registers.
   p.cl_log = 0;
-  while ((1 << p.cl_log) < kMaxCluster && ((long long)p.B * p.Hkv << p.cl_log) < num_sms() &&
-         p.Lmax > (kThreads << p.cl_log))
+  while ((1 << p.cl_log) < kMaxCluster && p.Lmax > (kThreads << p.cl_log) &&
+         (((long long)p.B * p.Hkv << p.cl_log) < num_sms() || p.Lmax > (16 * kThreads << p.cl_log)))
     ++p.cl_log;
   const int cl = 1 << p.cl_log;
   p.heads = FastDiv::of(p.Hkv);
@@ -374,8 +371,8 @@ static int launch(Params p, cudaStream_t st) {
   cfg.numAttrs = 2;
   if (keys <= 4)
     FK_CHECK_CUDA(cudaLaunchKernelEx(&cfg, select_kernel<4>, p));
-  else if (keys <= 32)
-    FK_CHECK_CUDA(cudaLaunchKernelEx(&cfg, select_kernel<32>, p));
+  else if (keys <= 16)
+    FK_CHECK_CUDA(cudaLaunchKernelEx(&cfg, select_kernel<16>, p));
   else
     FK_CHECK_CUDA(cudaLaunchKernelEx(&cfg, select_kernel<0>, p));
   GatherPlan g;
