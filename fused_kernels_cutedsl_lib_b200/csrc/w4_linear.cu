@@ -2,41 +2,45 @@
 //   y[m, n] = sum_k x[m, k] * (q[n, k] - z[n, k / g]) * s[n, k / g]  (+ residual[m, n])
 // with q, z in [0, 15], g in {32, 64, 128} and x, s, y bf16 or fp16.
 //
-// Bound: the 4-bit weights are read once (N*K/2 bytes); everything else is small.
+// Bound: the 4-bit weights are read once (N*K/2 bytes). What it takes to keep up with
+// them is instructions: at 6.5 TB/s an SM gets 46 weights a clock, and its ALU pipe
+// issues 64 lanes a clock.
 //
-// Arithmetic. The weights never become rounded 16-bit products q*s. A nibble q
-// is or-ed into the mantissa of 16.0 (bf16: bit 3, fp16: bit 6), which is the
-// exact 16-bit number 16 + q: one shift and one logic instruction per pair.
-// Those integers go to the tensor cores as they are; per group of g inputs
-//   sum_k x (q - z) = sum_k x (16 + q) - (16 + z) * sum_k x,
-// so the zero point costs one fused multiply-add per output and group, with
-// sum_k x computed once per CTA, and the scale another, both in fp32. The
-// offset 16 (rather than the 128 or 1024 of a nibble in the lowest mantissa
-// bits) keeps the cancelled part within about 4x of the result, a relative
-// error of a few 2^-22, far below the output's rounding.
+// Arithmetic. The weights never become rounded 16-bit products q*s. Nibbles are or-ed
+// into the mantissa of fp16 256.0 (bit 2) or 16.0 (bit 6), which gives the exact numbers
+// 256 + q and 16 + q, two nibbles of a 16-bit half per rotation of the word: five ALU
+// instructions for eight weights (bf16 has too few mantissa bits for a second nibble:
+// eight). Those integers go to the tensor cores as they are; per group of g inputs
+//   sum x (q - z) = sum x (off + q) - sum x off - z sum x,
+// with both sums of x computed once per CTA, so offset and zero point cost an addition
+// and a multiply-add per output and group, and the scale another, all in fp32. bf16
+// activations become fp16 by a power of two per token and 128 inputs that brings the
+// greatest to [2^14, 2^15): exact for everything within 2^-28 of it, off by 2^-39 of it
+// below. The offsets cancel: an error of some 2^-22 * 256 / 5 of the result, under a
+// quarter of fp16's half step.
 //
 // Layout (made once by the caller, `pack_w4`): rows in blocks of 16, inputs in
-// blocks of 128 and slabs of 4 blocks (the last slab may have fewer). A block is
+// blocks of 128 and slabs of 2 blocks (the last slab may have one). A block is
 // its codes, [2][32][4] words: half h, lane l = 4*g + c, word j holds the eight
-// nibbles of row 8*h + g, inputs 32*j + 8*c + 0..7; nibble i < 4 is input 2i, nibble
-// i >= 4 input 2(i - 4) + 1, so that the pair (i, i + 4) a shift exposes is a pair
-// of neighbouring inputs; then its scales and zero points, [groups][16] words. Lane
-// l of a warp therefore reads its mma.sync A operands of both row halves as two
-// 16-byte words, the B operands are 16 bytes of x as they lie in memory, and a group
-// of 32 inputs is one word j across the four lanes of a row, so every group size is
-// a whole number of mma steps. Memory order is slab, row block, block: the rows of a
-// slab are one contiguous stream.
+// nibbles of row 8*h + g, inputs 32*j + 8*c + 0..7, as the word rotated left by 2 of
+// which nibble i < 4 is input 2i and nibble i >= 4 input 2(i - 4) + 1, so that a pair
+// (i, i + 4) is a pair of neighbouring inputs; then its scales and zero points,
+// [groups][16] words. Lane l of a warp therefore reads its mma.sync A operands of both
+// row halves as two 16-byte words, the B operands are 16 bytes of x as they lie in
+// memory, and a group of 32 inputs is one word j across the four lanes of a row, so
+// every group size is a whole number of mma steps. Memory order is slab, row block,
+// block: the rows of a slab are one contiguous stream.
 //
 // Work split. Slabs go to the CS CTAs of a cluster, row blocks to the clusters, one
 // persistent grid. A CTA stages its slabs of x in shared memory once, in operand
-// order, with the group sums. A producer thread streams W / KW row blocks of a slab
-// at a time (up to 70 KB in one bulk copy; a copy per KB block reached 1.5 TB/s only)
-// into a ring of two stages; each of the W warps multiplies one row block (or one
-// of KW parts of it). A finished row block's partial sums are stored into the shared
-// memory of the CTA of the cluster that owns the rows; after one cluster barrier
-// every owner adds what it got in a fixed order: no workspace, no atomic, and
-// results do not depend on timing. The first weight copies are issued before the
-// wait for the preceding kernel (programmatic dependent launch).
+// order, with the group sums. A producer thread streams 8 / KW row blocks of a slab per
+// bulk copy (17 KB; copies of 1 KB reached 1.5 TB/s only) into a ring of six stages; groups
+// of eight warps take turns at row blocks, each warp one row block or one of KW parts
+// of its slab. A finished row block's partial sums are stored into the shared memory of
+// the CTA of the cluster that owns the rows; when every CTA has told it so (an mbarrier
+// with one arrival per CTA), an owner adds what it got in a fixed order: no workspace, no atomic, and results do not depend on
+// timing. The first weight copies are issued before the wait for the preceding kernel
+// (programmatic dependent launch).
 #include <cuda_fp16.h>
 
 #include <mutex>
@@ -49,8 +53,10 @@ namespace fk {
 namespace w4 {
 
 constexpr int kBlockK = 128;    // inputs per packed block
-constexpr int kSlab = 4;        // blocks per slab
-constexpr int kStages = 2;
+constexpr int kSlab = 2;        // blocks per slab
+constexpr int kSlabK = kSlab * kBlockK;
+constexpr int kGroupWarps = 8;  // warps that share a stage
+constexpr int kStages = 6;
 constexpr int kSmem = 227 * 1024;
 
 struct Params {
@@ -69,36 +75,26 @@ struct Params {
   int tile;                  // row blocks per cluster whose partial sums are held at a time
 };
 
+// A word's eight nibbles as fp16 pairs of inputs (0,1) (2,3) (4,5) (6,7), offset by 256, 16, 256, 16.
+__device__ __forceinline__ void expand(uint32_t w, uint32_t (&p)[4]) {
+  const uint32_t t = __funnelshift_r(w, w, 8);
+  p[0] = (w & 0x003C003Cu) | 0x5C005C00u;
+  p[1] = (w & 0x03C003C0u) | 0x4C004C00u;
+  p[2] = (t & 0x003C003Cu) | 0x5C005C00u;
+  p[3] = (t & 0x03C003C0u) | 0x4C004C00u;
+}
+
 template <typename T>
 struct Half;
-
 template <>
 struct Half<__nv_bfloat16> {
-  static __device__ __forceinline__ void expand(uint32_t w, uint32_t (&p)[4]) {
-    constexpr uint32_t kMask = 0x00780078u, kSixteen = 0x41804180u;
-    p[0] = ((w << 3) & kMask) | kSixteen;
-    p[1] = ((w >> 1) & kMask) | kSixteen;
-    p[2] = ((w >> 5) & kMask) | kSixteen;
-    p[3] = ((w >> 9) & kMask) | kSixteen;
-  }
   static __device__ __forceinline__ float lo(uint32_t v) { return __uint_as_float(v << 16); }
   static __device__ __forceinline__ float hi(uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); }
   static __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
   static __device__ __forceinline__ __nv_bfloat16 round(float v) { return __float2bfloat16_rn(v); }
-  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    mma_bf16_16816(d, a, b0, b1);
-  }
 };
-
 template <>
 struct Half<__half> {
-  static __device__ __forceinline__ void expand(uint32_t w, uint32_t (&p)[4]) {
-    constexpr uint32_t kMask = 0x03C003C0u, kSixteen = 0x4C004C00u;
-    p[0] = ((w << 6) & kMask) | kSixteen;
-    p[1] = ((w << 2) & kMask) | kSixteen;
-    p[2] = ((w >> 2) & kMask) | kSixteen;
-    p[3] = ((w >> 6) & kMask) | kSixteen;
-  }
   static __device__ __forceinline__ float lo(uint32_t v) {
     return __half2float(__ushort_as_half((unsigned short)(v & 0xFFFFu)));
   }
@@ -107,24 +103,14 @@ struct Half<__half> {
   }
   static __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
   static __device__ __forceinline__ __half round(float v) { return __float2half_rn(v); }
-  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    mma_f16_16816(d, a, b0, b1);
-  }
 };
 
 // D = A * B: the first step of a group starts from nothing.
-template <typename T>
 __device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
-  else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar, uint64_t pol) {
@@ -148,28 +134,77 @@ __device__ __forceinline__ void ld_cluster(uint32_t addr, float& a, float& b) {
 __device__ __forceinline__ void st_cluster(uint32_t addr, float a, float b) {
   asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(addr), "f"(a), "f"(b) : "memory");
 }
+// One arrival on another CTA's mbarrier, after everything this thread has seen (its CTA's stores
+// into the cluster, ordered before it by a CTA barrier).
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// Bounded wait for arrivals from the cluster, with acquire at its scope.
+__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, int* err) {
+  const uint64_t t0 = global_timer_ns();
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if (global_timer_ns() - t0 > wait_limit_ns(err)) break;
+  }
+  record_device_error(err, kDevErrFlagWait);
+  return false;
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ float4 lds128f(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ float2 lds64f(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+  return v;
+}
 
 template <int GROUP>
 __host__ __device__ constexpr int block_bytes() { return 1024 + (kBlockK / GROUP) * 64; }
-// Warps that multiply: 16 where the registers of one CTA per SM allow it.
+constexpr int kWarps = 16;  // that multiply
+template <int GROUP>
+__host__ __device__ constexpr int stage_bytes() { return kGroupWarps * kSlab * block_bytes<GROUP>(); }
+// Bytes of shared memory: the ring with its barriers; one slab of x with the sums of its groups and the
+// scales of its blocks; one row block's partial sums from one warp.
+template <int GROUP>
+__host__ __device__ constexpr int ring_bytes() { return kStages * stage_bytes<GROUP>() + 128; }
 template <int NT>
-__host__ __device__ constexpr int warps() { return NT <= 2 ? 16 : 8; }
-// Bytes of shared memory: the ring with its barriers, one slab of x with its group sums, one row
-// block's partial sums from one warp.
+__host__ __device__ constexpr int xop_bytes() { return kSlab * 4 * NT * 32 * 16; }
 template <int NT, int GROUP>
-__host__ __device__ constexpr int stage_bytes() { return warps<NT>() * kSlab * block_bytes<GROUP>(); }
+__host__ __device__ constexpr int sum_bytes() { return kSlab * (kBlockK / GROUP) * NT * 8 * 8; }
+template <int NT>
+__host__ __device__ constexpr int inv_bytes() { return kSlab * NT * 8 * 4; }
 template <int NT, int GROUP>
-__host__ __device__ constexpr int ring_bytes() { return kStages * stage_bytes<NT, GROUP>() + 128; }
-template <int NT, int GROUP>
-__host__ __device__ constexpr int x_bytes() { return kSlab * (4 * NT * 32 * 16 + (kBlockK / GROUP) * NT * 8 * 4); }
+__host__ __device__ constexpr int x_bytes() { return xop_bytes<NT>() + sum_bytes<NT, GROUP>() + inv_bytes<NT>(); }
 template <int NT>
 __host__ __device__ constexpr int part_bytes() { return 16 * NT * 8 * 4; }
 
 // NT: tiles of 8 tokens; GROUP: inputs per scale.
 template <typename T, int NT, int GROUP>
-__global__ void __launch_bounds__(warps<NT>() * 32 + 32, 1) w4_linear_kernel(const Params p) {
+__global__ void __launch_bounds__(kWarps * 32 + 32, 1) w4_linear_kernel(const Params p) {
   using H = Half<T>;
-  constexpr int W = warps<NT>();
+  constexpr bool kScaled = std::is_same<T, __nv_bfloat16>::value;  // x goes in as fp16 times a power of two
+  constexpr int W = kWarps;
+  constexpr int NG = W / kGroupWarps;
   constexpr int GPB = kBlockK / GROUP;  // groups per input block
   constexpr int WPG = 4 / GPB;          // words of a lane per group
   constexpr int TOK = NT * 8;
@@ -184,25 +219,32 @@ __global__ void __launch_bounds__(warps<NT>() * 32 + 32, 1) w4_linear_kernel(con
   // This cluster's row blocks; this CTA's slabs are rank, rank + cs, ...
   const int rb0 = cid * p.rb_each + min(cid, p.rb_more), rb1 = rb0 + p.rb_each + (cid < p.rb_more);
   const int nsl = (p.nslab - rank + cs - 1) >> p.cs_log;
-  const int max_sl = (p.nslab + cs - 1) >> p.cs_log;  // of any CTA of the cluster
-  const int rows_stage = W >> p.kw_log;               // row blocks per stage
+  const int max_sl = (p.nslab + cs - 1) >> p.cs_log;   // of any CTA of the cluster
+  const int rows_stage = kGroupWarps >> p.kw_log;      // row blocks per stage
 
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStages * stage_bytes<NT, GROUP>());
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStages * stage_bytes<GROUP>());
   uint64_t* empty = full + kStages;
-  uint4* xs = reinterpret_cast<uint4*>(smem + ring_bytes<NT, GROUP>());               // [chunk][slab blocks][4 words j][NT][32 lanes]
-  float* xsum = reinterpret_cast<float*>(xs + (size_t)p.chunk * kSlab * 4 * NT * 32);  // [chunk][slab blocks][GPB][TOK]
-  float* part_buf = xsum + (size_t)p.chunk * kSlab * GPB * TOK;                        // [cs * kw][own][16][TOK]
+  uint64_t* done = empty + kStages;  // one arrival per CTA: its partial sums of the tile are stored
+  uint64_t* taken = done + 1;        // one arrival per CTA: it has added up the tile's
+  uint8_t* xmem = smem + ring_bytes<GROUP>();
+  uint4* xs = reinterpret_cast<uint4*>(xmem);                                           // [chunk][blocks][4 words j][NT][32 lanes]
+  float4* xsum = reinterpret_cast<float4*>(xmem + (size_t)p.chunk * xop_bytes<NT>());   // [chunk][blocks][GPB][TOK / 2]: sums of two tokens, then their offset sums
+  float* xinv = reinterpret_cast<float*>(xsum) + (size_t)p.chunk * (sum_bytes<NT, GROUP>() / 4);  // [chunk][blocks][TOK]: 1 / scale
+  float* part_buf = xinv + (size_t)p.chunk * (inv_bytes<NT>() / 4);                     // [cs * kw][own][16][TOK]
   const int own_max = (p.tile + cs - 1) >> p.cs_log;  // row blocks of a tile that one CTA owns
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], W);
+      mbar_init(&empty[i], kGroupWarps);
     }
+    mbar_init(done, cs);
+    mbar_init(taken, cs);
     fence_barrier_init();
   }
   __syncthreads();
-  // The other CTAs must have started before anything is stored into their shared memory.
+  // The other CTAs must have started, their barriers included, before anything is stored into their
+  // shared memory. The only phase of the cluster's own barrier.
   cluster_arrive();
 
   auto slab_blocks = [&](int s) { return min(kSlab, p.nkb - s * kSlab); };
@@ -212,37 +254,37 @@ __global__ void __launch_bounds__(warps<NT>() * 32 + 32, 1) w4_linear_kernel(con
     const uint64_t pol = l2_policy_evict_first();
     int stage = 0, filled = 0;
     uint32_t phase = 0;
-    cluster_wait();
     for (int r0 = rb0; r0 < rb1; r0 += p.tile) {
       const int nr = min(p.tile, rb1 - r0);
       if (lane == 0) {
         for (int c0 = 0; c0 < max_sl; c0 += p.chunk) {
           const int c1 = min(c0 + p.chunk, nsl);
-          for (int rg = 0; rg < nr; rg += rows_stage) {
+          for (int rg = 0; rg < nr; rg += NG * rows_stage) {
             for (int sl = c0; sl < c1; ++sl) {
               const int s = rank + sl * cs, nb = slab_blocks(s);
-              const uint32_t bytes = (uint32_t)min(rows_stage, nr - rg) * nb * BB;
-              if (filled >= kStages) mbar_wait(&empty[stage], phase ^ 1, p.err, kDevErrEmptyWait);
-              mbar_arrive_expect_tx(&full[stage], bytes);
-              bulk_load(smem_u32(smem + stage * stage_bytes<NT, GROUP>()),
-                        p.packed + ((size_t)s * kSlab * p.nrb + (size_t)(r0 + rg) * nb) * BB, bytes, &full[stage], pol);
-              ++filled;
-              if (++stage == kStages) {
-                stage = 0;
-                phase ^= 1;
+              const uint8_t* src = p.packed + ((size_t)s * kSlab * p.nrb + (size_t)(r0 + rg) * nb) * BB;
+#pragma unroll
+              for (int q = 0; q < NG; ++q) {
+                const int n = min(rows_stage, nr - rg - q * rows_stage);
+                if (n <= 0) break;
+                const uint32_t bytes = (uint32_t)(n * nb) * BB;
+                if (filled >= kStages) mbar_wait(&empty[stage], phase ^ 1, p.err, kDevErrEmptyWait);
+                mbar_arrive_expect_tx(&full[stage], bytes);
+                bulk_load(smem_u32(smem + stage * stage_bytes<GROUP>()), src + (size_t)(q * rows_stage * nb) * BB, bytes,
+                          &full[stage], pol);
+                ++filled;
+                if (++stage == kStages) {
+                  stage = 0;
+                  phase ^= 1;
+                }
               }
             }
           }
         }
       }
-      __syncwarp();
-      cluster_arrive();
-      cluster_wait();
-      if (r0 + p.tile < rb1) {
-        cluster_arrive();
-        cluster_wait();
-      }
     }
+    __syncwarp();
+    cluster_wait();
     // No copy may be in flight when the CTA ends, also when a multiplying warp gave up waiting for one.
     if (lane == 0) {
       for (int f = max(0, filled - kStages); f < filled; ++f)
@@ -253,62 +295,149 @@ __global__ void __launch_bounds__(warps<NT>() * 32 + 32, 1) w4_linear_kernel(con
 
   // ------------------------------ multiply ------------------------------
   const int g = lane >> 2, c = lane & 3;
-  const int wrow = warp & (rows_stage - 1), wk = warp >> (__ffs(W) - 1 - p.kw_log);  // row block of a stage, part of its slab
+  const int gid = warp / kGroupWarps, gw = warp % kGroupWarps;
+  const int wrow = gw & (rows_stage - 1), wk = gw >> (3 - p.kw_log);  // row block of a stage, part of its slab
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  int stage = 0;
+  // Where a lane reads its tokens' operands: columns past the last token read the last one's, whose
+  // bytes the shared memory serves once (one token: a quarter of the wavefronts).
+  uint32_t xlane[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) xlane[t] = (min(g, max(0, ntok - 1 - t * 8)) * 4 + c) * 16;
+  int stage = 0;  // of the next fill of the current round of row blocks
   uint32_t phase = 0;
+  auto advance = [&](int& st, uint32_t& ph, int n) {  // n <= kStages
+    st += n;
+    if (st >= kStages) {
+      st -= kStages;
+      ph ^= 1;
+    }
+  };
   bool ok = true;
 
-  for (int r0 = rb0; r0 < rb1; r0 += p.tile) {
+  uint32_t tile_phase = 0;
+  // All of this CTA's multiplying warps have come here, and one of them tells the cluster.
+  auto tell = [&](uint64_t* bar) {
+    named_bar_sync(1, W * 32);
+    if (warp == 0 && lane < cs) arrive_cluster(map_to(smem_u32(bar), lane));
+  };
+  for (int r0 = rb0; r0 < rb1; r0 += p.tile, tile_phase ^= 1) {
     const int nr = min(p.tile, rb1 - r0);
     for (int c0 = 0; c0 < max_sl; c0 += p.chunk) {
       const int c1 = min(c0 + p.chunk, nsl);  // c0 >= c1 in a CTA with one slab less
-      // ---- stage x of these slabs: 8 inputs of a token per thread and iteration. Columns past the
-      // last token stay whatever they are: they reach only sums that nobody reads. ----
+      // ---- stage x of these slabs: a warp takes a token's slab, a lane 8 inputs; four such loads in
+      // flight. Columns past the last token stay whatever they are: they reach only sums that nobody reads. ----
       if (r0 == rb0 || p.chunk < max_sl) {
         if (c0 > 0 || r0 > rb0) named_bar_sync(1, W * 32);  // the previous chunk has been used
-        constexpr int kPieces = kSlab * 16;  // of a token and slab; whole warps share a token (shuffles below)
-        const int q = threadIdx.x % kPieces;
-        const int kb = q >> 4, j = (q >> 2) & 3, cc = q & 3;
-        for (int sl = 0; sl < c1 - c0; ++sl) {
-          const int k = (rank + (c0 + sl) * cs) * (kSlab * kBlockK) + q * 8;
-          for (int n = threadIdx.x / kPieces; n < ntok; n += W * 32 / kPieces) {
-            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-            if (k < p.K)
-              v = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + (size_t)(tok0 + n) * p.ldx + k);
-            float sum = ((H::lo(v.x) + H::hi(v.x)) + (H::lo(v.y) + H::hi(v.y))) +
-                        ((H::lo(v.z) + H::hi(v.z)) + (H::lo(v.w) + H::hi(v.w)));
+        const int j = (lane >> 2) & 3, cc = lane & 3, kb = lane >> 4;
+        constexpr int U = 4;
+        int sl = c0, n = warp;  // item (slab, token)
+        while (sl < c1 && n >= ntok) n -= ntok, ++sl;
+        while (sl < c1) {
+          uint4 v[U];
+          int isl[U], in[U];
 #pragma unroll
-            for (int off = 1; off < GROUP / 8; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-            xs[(((sl * kSlab + kb) * 4 + j) * NT + (n >> 3)) * 32 + (n & 7) * 4 + cc] = v;
-            if (q % (GROUP / 8) == 0) xsum[(sl * (kPieces * 8 / GROUP) + q / (GROUP / 8)) * TOK + n] = sum;
+          for (int u = 0; u < U; ++u) {
+            isl[u] = sl;
+            in[u] = n;
+            v[u] = make_uint4(0u, 0u, 0u, 0u);
+            if (sl < c1) {
+              const int k = (rank + sl * cs) * kSlabK + lane * 8;
+              if (k < p.K)
+                v[u] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + (size_t)(tok0 + n) * p.ldx + k);
+              n += W;
+              while (sl < c1 && n >= ntok) n -= ntok, ++sl;
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            if (isl[u] >= c1) break;
+            const int lsl = isl[u] - c0, nn = in[u];
+            uint4 w = v[u];
+            float inv = 1.f;
+            if constexpr (kScaled) {
+              // The greatest magnitude of the token's 128 inputs, by the bits without signs.
+              uint32_t m = __vmaxu2(__vmaxu2(w.x & 0x7FFF7FFFu, w.y & 0x7FFF7FFFu),
+                                    __vmaxu2(w.z & 0x7FFF7FFFu, w.w & 0x7FFF7FFFu));
+              m = max(m & 0xFFFFu, m >> 16);
+#pragma unroll
+              for (int off = 1; off < 16; off <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, off));
+              const int e = min(141 - (int)(m >> 7), 126);  // x * 2^e is below 2^15
+              const float scale = __uint_as_float((uint32_t)(127 + e) << 23);
+              inv = __uint_as_float((uint32_t)(127 - e) << 23);
+              uint32_t* wp = &w.x;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const __half2 hh = __floats2half2_rn(H::lo(wp[i]) * scale, H::hi(wp[i]) * scale);
+                wp[i] = *reinterpret_cast<const uint32_t*>(&hh);
+              }
+            }
+            xs[(((lsl * kSlab + kb) * 4 + j) * NT + (nn >> 3)) * 32 + (nn & 7) * 4 + cc] = w;
+            if (kScaled && (lane & 15) == 0) xinv[(lsl * kSlab + kb) * TOK + nn] = inv;
+          }
+        }
+        named_bar_sync(1, W * 32);
+        // The groups' sums, by the tensor cores: a matrix whose row 0 is all ones and whose row 1 has the
+        // offsets (256 256 16 16 per lane and step) times the operands just stored. A warp takes
+        // a block's 8 tokens; lanes 0..3 end up with the sums of tokens 2c, 2c + 1 and lanes 4..7 with
+        // their offset sums.
+        const uint32_t one = g == 0 ? 0x3C003C00u : g == 1 ? 0x5C005C00u : 0u;
+        const uint32_t two = g == 0 ? 0x3C003C00u : g == 1 ? 0x4C004C00u : 0u;
+        const uint32_t af[4] = {one, 0u, two, 0u};
+        for (int i = warp; i < (c1 - c0) * kSlab * NT; i += W) {
+          const int blk = i / NT, t = i % NT;
+#pragma unroll
+          for (int gi = 0; gi < GPB; ++gi) {
+            float d[4];
+#pragma unroll
+            for (int jj = 0; jj < WPG; ++jj) {
+              const uint4 b = xs[((blk * 4 + gi * WPG + jj) * NT + t) * 32 + lane];
+              if (jj == 0)
+                mma_first(d, af, b.x, b.y);
+              else
+                mma_f16_16816(d, af, b.x, b.y);
+              mma_f16_16816(d, af, b.z, b.w);
+            }
+            if (lane < 8)
+              reinterpret_cast<float2*>(xsum + (blk * GPB + gi) * (TOK / 2) + t * 4 + c)[g] = make_float2(d[0], d[1]);
           }
         }
         named_bar_sync(1, W * 32);
       }
-      if (r0 == rb0 && c0 == 0) cluster_wait();
+      if (c0 == 0) {
+        if (r0 == rb0)
+          cluster_wait();
+        else if (ok)  // the owners are done with the tile before
+          ok = wait_cluster(taken, tile_phase ^ 1, p.err);
+        __syncwarp();
+      }
 
-      for (int rg = 0; rg < nr; rg += rows_stage) {
-        const int lr = rg + wrow;  // this warp's row block of the tile
+      for (int rg = 0; rg < nr; rg += NG * rows_stage) {
+        const int lr = rg + gid * rows_stage + wrow;                      // this warp's row block of the tile
+        const int groups = min(NG, (nr - rg + rows_stage - 1) >> (3 - p.kw_log));  // warp groups with rows in this round
+        const bool mine = gid < groups, live = lr < nr;
         float acc[NT][4];
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
+        int st = stage;
+        uint32_t ph = phase;
+        if (gid) advance(st, ph, gid);
         for (int sl = c0; sl < c1; ++sl) {
-          if (ok && !mbar_wait(&full[stage], phase, p.err, kDevErrFullWait)) ok = false;
-          if (lr < nr) {
+          advance(stage, phase, groups);
+          if (!mine) continue;
+          if (ok && !mbar_wait(&full[st], ph, p.err, kDevErrFullWait)) ok = false;
+          if (live) {
             const int nb = slab_blocks(rank + sl * cs);
-            const uint8_t* sb = smem + stage * stage_bytes<NT, GROUP>() + (size_t)wrow * nb * BB;
-            const int b_end = min(nb, (wk + 1) * (kSlab >> p.kw_log));
+            const int b0 = wk * (kSlab >> p.kw_log), b1 = min(nb, b0 + (kSlab >> p.kw_log));
+            const int lb0 = (sl - c0) * kSlab + b0;
+            uint32_t wa = smem_u32(smem + st * stage_bytes<GROUP>() + (wrow * nb + b0) * BB) + lane * 16;
+            uint32_t xa = smem_u32(xs + (size_t)lb0 * (4 * NT * 32));
+            uint32_t sa = smem_u32(xsum + (size_t)lb0 * (GPB * (TOK / 2)) + c);
+            uint32_t va = smem_u32(xinv + lb0 * TOK + 2 * c);
 #pragma unroll 1
-            for (int bl = wk * (kSlab >> p.kw_log); bl < b_end; ++bl) {
-              const uint8_t* bb = sb + bl * BB;
-              const uint4 lo4 = *reinterpret_cast<const uint4*>(bb + lane * 16);
-              const uint4 hi4 = *reinterpret_cast<const uint4*>(bb + 512 + lane * 16);
-              const uint32_t* sz = reinterpret_cast<const uint32_t*>(bb + 1024) + g;
-              const int lb = (sl - c0) * kSlab + bl;
-              const uint4* xb = xs + (size_t)lb * 4 * NT * 32 + lane;
-              const float* xg = xsum + lb * GPB * TOK + 2 * c;
+            for (int bl = b0; bl < b1; ++bl) {
+              const uint4 lo4 = lds128(wa), hi4 = lds128(wa + 512);
+              const uint32_t za = wa - lane * 16 + 1024 + g * 4;
               const uint32_t wlo[4] = {lo4.x, lo4.y, lo4.z, lo4.w};
               const uint32_t whi[4] = {hi4.x, hi4.y, hi4.z, hi4.w};
 #pragma unroll
@@ -317,48 +446,52 @@ __global__ void __launch_bounds__(warps<NT>() * 32 + 32, 1) w4_linear_kernel(con
 #pragma unroll
                 for (int jj = 0; jj < WPG; ++jj) {
                   const int j = i * WPG + jj;
-                  uint32_t pl[4], ph[4];
-                  H::expand(wlo[j], pl);
-                  H::expand(whi[j], ph);
-                  const uint32_t a0[4] = {pl[0], ph[0], pl[1], ph[1]};
-                  const uint32_t a1[4] = {pl[2], ph[2], pl[3], ph[3]};
+                  uint32_t pl[4], ph4[4];
+                  expand(wlo[j], pl);
+                  expand(whi[j], ph4);
+                  const uint32_t a0[4] = {pl[0], ph4[0], pl[1], ph4[1]};
+                  const uint32_t a1[4] = {pl[2], ph4[2], pl[3], ph4[3]};
 #pragma unroll
                   for (int t = 0; t < NT; ++t) {
-                    const uint4 b = xb[(j * NT + t) * 32];
+                    const uint4 b = lds128(xa + (j * NT + t) * 512 + xlane[t]);
                     if (jj == 0)
-                      mma_first<T>(part[t], a0, b.x, b.y);
+                      mma_first(part[t], a0, b.x, b.y);
                     else
-                      H::mma(part[t], a0, b.x, b.y);
-                    H::mma(part[t], a1, b.z, b.w);
+                      mma_f16_16816(part[t], a0, b.x, b.y);
+                    mma_f16_16816(part[t], a1, b.z, b.w);
                   }
                 }
-                const uint32_t z0 = sz[i * 16], z1 = sz[i * 16 + 8];
+                const uint32_t z0 = lds32(za + i * 64), z1 = lds32(za + i * 64 + 32);
                 const float s_lo = H::lo(z0), z_lo = H::hi(z0);
                 const float s_hi = H::lo(z1), z_hi = H::hi(z1);
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                  const float2 xx = *reinterpret_cast<const float2*>(xg + i * TOK + t * 8);
-                  acc[t][0] = fmaf(s_lo, fmaf(-z_lo, xx.x, part[t][0]), acc[t][0]);
-                  acc[t][1] = fmaf(s_lo, fmaf(-z_lo, xx.y, part[t][1]), acc[t][1]);
-                  acc[t][2] = fmaf(s_hi, fmaf(-z_hi, xx.x, part[t][2]), acc[t][2]);
-                  acc[t][3] = fmaf(s_hi, fmaf(-z_hi, xx.y, part[t][3]), acc[t][3]);
+                  const float4 xx = lds128f(sa + (i * (TOK / 2) + t * 4) * 16);
+                  const float2 iv = kScaled ? lds64f(va + t * 32) : make_float2(1.f, 1.f);
+                  const float s0 = kScaled ? s_lo * iv.x : s_lo, s1 = kScaled ? s_lo * iv.y : s_lo;
+                  const float s2 = kScaled ? s_hi * iv.x : s_hi, s3 = kScaled ? s_hi * iv.y : s_hi;
+                  acc[t][0] = fmaf(s0, fmaf(-z_lo, xx.x, part[t][0] - xx.z), acc[t][0]);
+                  acc[t][1] = fmaf(s1, fmaf(-z_lo, xx.y, part[t][1] - xx.w), acc[t][1]);
+                  acc[t][2] = fmaf(s2, fmaf(-z_hi, xx.x, part[t][2] - xx.z), acc[t][2]);
+                  acc[t][3] = fmaf(s3, fmaf(-z_hi, xx.y, part[t][3] - xx.w), acc[t][3]);
                 }
               }
+              wa += BB;
+              xa += 4 * NT * 512;
+              sa += GPB * (TOK / 2) * 16;
+              va += TOK * 4;
             }
           }
           __syncwarp();
-          if (lane == 0) mbar_arrive(&empty[stage]);
-          if (++stage == kStages) {
-            stage = 0;
-            phase ^= 1;
-          }
+          if (lane == 0) mbar_arrive(&empty[st]);
+          advance(st, ph, groups);
         }
         // The row block's partial sums go to the CTA that owns the rows. A warp whose CTA has no
         // slab in the first chunk leaves zeros; a later chunk adds to what this lane stored before.
-        if (lr < nr && (c0 == 0 || c0 < c1)) {
+        if (live && (c0 == 0 || c0 < c1)) {
           const int owner = lr & (cs - 1), slot = lr >> p.cs_log;
-          float* mine = part_buf + (size_t)((((rank << p.kw_log) + wk) * own_max + slot) * 16 + g) * TOK + 2 * c;
-          const uint32_t to = map_to(smem_u32(mine), owner);
+          float* dst = part_buf + (size_t)((((rank << p.kw_log) + wk) * own_max + slot) * 16 + g) * TOK + 2 * c;
+          const uint32_t to = map_to(smem_u32(dst), owner);
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
             if (t * 8 + 2 * c < ntok) {
@@ -378,32 +511,38 @@ __global__ void __launch_bounds__(warps<NT>() * 32 + 32, 1) w4_linear_kernel(con
     }
 
     // ---- every owner adds up its rows' partial sums, in order ----
-    __syncwarp();
-    cluster_arrive();
-    cluster_wait();
+    tell(done);
+    if (ok) ok = wait_cluster(done, tile_phase, p.err);
     {
-      // Row block lr of the tile belongs to CTA lr mod cs; 16 lanes take its rows, for one token.
+      // Row block lr of the tile belongs to CTA lr mod cs; 16 lanes take its rows, for four tokens.
       const int n_own = (nr - rank + cs - 1) >> p.cs_log, parts = cs << p.kw_log;
       const int plane = own_max * 16 * TOK;
       const int r = lane & 15;
-      for (int i = warp * 2 + (lane >> 4); i < n_own * TOK; i += W * 2) {
-        const int slot = i / TOK, n = i % TOK;  // TOK is a power of two
+      for (int i = warp * 2 + (lane >> 4); i < n_own * (TOK / 4); i += W * 2) {
+        const int slot = i / (TOK / 4), n = (i % (TOK / 4)) * 4;  // TOK is a power of two
         const int row = (r0 + (slot << p.cs_log) + rank) * 16 + r;
         if (n >= ntok || row >= p.N) continue;
-        const float* from = part_buf + (slot * 16 + r) * TOK + n;
-        float v = 0.f;
-#pragma unroll 8
-        for (int q = 0; q < parts; ++q) v += from[q * plane];
         const size_t off = (size_t)(tok0 + n) * p.N + row;
-        if (p.residual) v += H::to_float(static_cast<const T*>(p.residual)[off]);
-        static_cast<T*>(p.y)[off] = H::round(v);
+        float res[4] = {0.f, 0.f, 0.f, 0.f};
+        if (p.residual) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (n + e < ntok) res[e] = H::to_float(static_cast<const T*>(p.residual)[off + (size_t)e * p.N]);
+        }
+        const float* from = part_buf + (slot * 16 + r) * TOK + n;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+        for (int q = 0; q < parts; ++q) {
+          const float4 f = *reinterpret_cast<const float4*>(from + q * plane);
+          v.x += f.x, v.y += f.y, v.z += f.z, v.w += f.w;
+        }
+        const float out[4] = {v.x + res[0], v.y + res[1], v.z + res[2], v.w + res[3]};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n + e < ntok) static_cast<T*>(p.y)[off + (size_t)e * p.N] = H::round(out[e]);
       }
     }
-    if (r0 + p.tile < rb1) {  // the next tile's partial sums overwrite these
-      __syncwarp();
-      cluster_arrive();
-      cluster_wait();
-    }
+    if (r0 + p.tile < rb1) tell(taken);  // the next tile's partial sums overwrite these
   }
 }
 
@@ -430,7 +569,7 @@ static int resident_clusters(int (&out)[4]) {
       attr[0].val.clusterDim.z = 1;
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3(1u << i, 1, 1);
-      cfg.blockDim = dim3(warps<NT>() * 32 + 32, 1, 1);
+      cfg.blockDim = dim3(kWarps * 32 + 32, 1, 1);
       cfg.dynamicSmemBytes = kSmem;
       cfg.attrs = attr;
       cfg.numAttrs = 1;
@@ -445,54 +584,45 @@ static int resident_clusters(int (&out)[4]) {
 
 template <typename T, int NT, int GROUP>
 static int launch(Params p, cudaStream_t st) {
-  constexpr int W = warps<NT>();
-  constexpr int kBudget = kSmem - ring_bytes<NT, GROUP>();  // for x and the partial sums
+  constexpr int kBudget = kSmem - ring_bytes<GROUP>();  // for x and the partial sums
   constexpr int kX = x_bytes<NT, GROUP>();
+  static_assert(kX + 8 * part_bytes<NT>() <= kBudget, "a slab of x and one owned row block must fit");
   int resident[4];
   int rc = resident_clusters<T, NT, GROUP>(resident);
   if (rc) return rc;
   const int tiles = (p.M + NT * 8 - 1) / (NT * 8);
-  // CTAs per cluster: the fewest that hold all of their x and partial sums at once, and whose
-  // clusters have a row block for three quarters of the warps; at most 8 (the portable
-  // size), and no more than there are slabs. With 8, x and rows may go in several rounds.
-  int kw = 1, ncl = 0, own_bytes = 0, rows = 0, slabs = 0;
-  for (p.cs_log = 0;; ++p.cs_log) {
-    const int cs = 1 << p.cs_log;
-    ncl = resident[p.cs_log] / tiles > 0 ? resident[p.cs_log] / tiles : 1;
-    if (ncl > p.nrb) ncl = p.nrb;
-    rows = (p.nrb + ncl - 1) / ncl;
-    slabs = (p.nslab + cs - 1) / cs;
-    // Few rows per cluster: 2 or 4 warps share a row block. Each part costs a plane of partial sums.
-    for (kw = 1; kw < kSlab && W / kw >= 2 * rows;) kw *= 2;
-    own_bytes = part_bytes<NT>() * cs * kw;  // one owned row block
-    if (cs == 8 || 2 * cs > p.nslab) break;
-    if ((long long)slabs * kX + (long long)((rows + cs - 1) / cs) * own_bytes <= kBudget && 4 * rows >= 3 * W) break;
-  }
+  // Four CTAs per cluster where there are slabs for them: measured best or within 2 % of it from one
+  // token on 4096 rows to 64 on 14336 inputs. Two or one leave too many slabs of x to every CTA, eight
+  // leave SMs idle (15 clusters of 8, 36 of 4 are resident on 148 SMs).
+  p.cs_log = p.nslab >= 4 ? 2 : p.nslab >= 2 ? 1 : 0;
   const int cs = 1 << p.cs_log;
-  // x takes what is left by one round of row blocks, the partial sums what is left by x.
-  int own = (W / kw + cs - 1) / cs;
-  if (own > (rows + cs - 1) / cs) own = (rows + cs - 1) / cs;
+  int ncl = resident[p.cs_log] / tiles;
+  ncl = ncl < 1 ? 1 : ncl > p.nrb ? p.nrb : ncl;
+  const int rows = (p.nrb + ncl - 1) / ncl, slabs = (p.nslab + cs - 1) / cs;
+  // Few rows per cluster: two warps share a row block. Each part costs a plane of partial sums.
+  p.kw_log = 2 * rows <= kWarps ? 1 : 0;
+  const int own_bytes = part_bytes<NT>() * cs << p.kw_log;  // one owned row block
+  // All partial sums at once if they leave room for a slab of x, which takes the rest.
+  int own = (rows + cs - 1) / cs;
+  if ((long long)own * own_bytes > kBudget - kX) own = (kBudget - kX) / own_bytes;
   p.chunk = (kBudget - own * own_bytes) / kX;
-  if (p.chunk < 1) return fail(kErrUnsupported, "w4 linear: x does not fit into shared memory");
   if (p.chunk > slabs) p.chunk = slabs;
-  own = (kBudget - p.chunk * kX) / own_bytes;
   const int rounds = (rows + own * cs - 1) / (own * cs);  // of equal size
   p.tile = (rows + rounds - 1) / rounds;
   own = (p.tile + cs - 1) / cs;
-  const int smem = ring_bytes<NT, GROUP>() + p.chunk * kX + own * own_bytes;
-  p.kw_log = kw == 4 ? 2 : kw == 2 ? 1 : 0;
+  const int smem = ring_bytes<GROUP>() + p.chunk * kX + own * own_bytes;
   p.rb_each = p.nrb / ncl;
   p.rb_more = p.nrb % ncl;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = cs;
+  attr[1].val.clusterDim.x = 1 << p.cs_log;
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(ncl * cs), (unsigned)tiles, 1);
-  cfg.blockDim = dim3(W * 32 + 32, 1, 1);
+  cfg.gridDim = dim3((unsigned)(ncl << p.cs_log), (unsigned)tiles, 1);
+  cfg.blockDim = dim3(kWarps * 32 + 32, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;

@@ -22,7 +22,7 @@ from ._tensors import (current_device, dtype_code, launch_stream, on_device, one
 
 GROUP_SIZES = (32, 64, 128)
 _BLOCK_K = 128  # inputs per block
-_SLAB = 4       # input blocks per slab
+_SLAB = 2       # input blocks per slab
 
 
 @dataclass(frozen=True)
@@ -46,15 +46,21 @@ class W4Weight:
         tail = self.packed[full * _SLAB * nb * words:].view(nb, -1, words)
         blocks = torch.cat([head.reshape(nb, -1, words), tail], 1)
         shifts = torch.arange(0, 32, 4, device=self.packed.device, dtype=torch.int32)
-        q = (blocks[..., :256].unsqueeze(-1) >> shifts) & 15
+        words = _rotate_left(blocks[..., :256], 30)
+        q = (words.unsqueeze(-1) >> shifts) & 15
         q = q.view(nb, kb, 2, 8, 4, 4, 2, 4).permute(0, 2, 3, 1, 5, 4, 7, 6)  # [nb, half, g, kb, j, c, pair, odd]
         q = q.reshape(nb * 16, kb * _BLOCK_K)[:self.n, :self.k].float()
         sz = blocks[..., 256:].reshape(nb, -1, 16).transpose(1, 2).reshape(nb * 16, -1)
         sz = sz[:self.n, :self.k // self.group_size]
         both = sz.reshape(-1).contiguous().view(self.dtype).view(self.n, -1, 2).float()
-        s, z = both[..., 0], both[..., 1] - 16.0
+        s, z = both[..., 0], both[..., 1]
         rep = lambda t: t.repeat_interleave(self.group_size, dim=1)  # noqa: E731
         return (q - rep(z)) * rep(s)
+
+
+def _rotate_left(words: torch.Tensor, n: int) -> torch.Tensor:
+    """int32 words rotated by n bits (the shift right of a negative int32 is arithmetic: masked)."""
+    return (words << n) | ((words >> (32 - n)) & ((1 << n) - 1))
 
 
 def pack_w4(q: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None) -> W4Weight:
@@ -96,8 +102,8 @@ def pack_w4(q: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = 
         pad[:rows.shape[0], :k] = rows
         # [nb, half, g, kb, j, c, pair, odd] -> [nb, kb, half, (g, c), j], nibble 4 * odd + pair of the word
         v = pad.view(-1, 2, 8, kb, 4, 4, 4, 2).permute(0, 3, 1, 2, 5, 4, 7, 6).flatten(-2) << shifts
-        packed[b0:b0 + v.shape[0], :, :256] = v.sum(-1, dtype=torch.int32).reshape(-1, kb, 256)
-    z = torch.full_like(scales, 24.0) if zeros is None else zeros.to(scales.dtype) + 16.0
+        packed[b0:b0 + v.shape[0], :, :256] = _rotate_left(v.sum(-1, dtype=torch.int32), 2).reshape(-1, kb, 256)
+    z = torch.full_like(scales, 8.0) if zeros is None else zeros.to(scales.dtype)
     sz = torch.zeros(nb * 16, kb * _BLOCK_K // group, 2, dtype=scales.dtype, device=dev)
     sz[:n, :k // group, 0] = scales
     sz[:n, :k // group, 1] = z

@@ -376,13 +376,13 @@ FK_API int fk_skinny_gemm_noalloc(const void* x, const void* w, void* y, int M, 
  * rounding. Weights never become 16-bit products: integers are multiplied and the
  * scale is applied in fp32, so a non-finite x gives non-finite y.
  *   packed  blocks of 16 rows x 128 inputs, 1024 + 8192 / group_size bytes each,
- *           16-byte aligned, ceil(N/16) x ceil(K/128) of them, ordered by slab of 4
- *           input blocks (the last may have fewer), row block, input block. As
- *           uint32 a block is [2][32][4] codes, then [128 / group_size][16] scales:
- *           word j of lane 4g + c in half h holds q of row 8 h + g, inputs
- *           32 j + 8 c + {0, 2, 4, 6, 1, 3, 5, 7}, lowest nibble first (anything
- *           past N or K); the scale word of a row has s in the low half and 16 + z
- *           (as dtype) in the high half (0 past N or K).
+ *           16-byte aligned, ceil(N/16) x ceil(K/128) of them, ordered by slab of 2
+ *           input blocks (the last may have one), row block, input block. As uint32 a
+ *           block is [2][32][4] codes, then [128 / group_size][16] scales: word j of
+ *           lane 4g + c in half h is, rotated left by 2, the word that holds q of row
+ *           8 h + g, inputs 32 j + 8 c + {0, 2, 4, 6, 1, 3, 5, 7}, lowest nibble first
+ *           (anything past N or K); the scale word of a row has s in the low half and
+ *           z (as dtype) in the high half (0 past N or K).
  * No workspace. As for every GEMM here, the weights must not be written by the
  * kernel of this library that precedes the call on its stream. */
 FK_API int fk_w4_linear(const void* x, long long ldx, const void* packed, const void* residual, void* y, int dtype,

@@ -21,9 +21,10 @@ def test_pack_and_dequantize(n, k, group, zeros, dtype):
     h, g = (row % 16) // 8, row % 8
     j, c, i = (col % 128) // 32, (col % 32) // 8, col % 8
     nb, kb, words = -(-n // 16), -(-k // 128), 256 + 2048 // group
-    slab, block = col // 512, col % 512 // 128
-    at = (slab * 4 * nb + (row // 16) * min(4, kb - 4 * slab) + block) * words
+    slab, block = col // 256, col % 256 // 128
+    at = (slab * 2 * nb + (row // 16) * min(2, kb - 2 * slab) + block) * words
     word = int(w.packed[at + (h * 32 + 4 * g + c) * 4 + j]) & 0xFFFFFFFF
+    word = (word >> 2) | (word & 3) << 30
     nibble = (i % 2) * 4 + i // 2  # even inputs in the low half, odd ones in the high half
     assert (word >> (4 * nibble)) & 15 == int(q[row, col])
 
