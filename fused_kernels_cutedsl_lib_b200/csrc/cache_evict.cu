@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const Params p) {
   // Each warp of the cluster owns a contiguous stretch of the candidates, a whole number of
   // rounds of 32.
   const int gw = rank * kWarps + warp;
-  const int seg = (((m + 31) >> 5) + cl * kWarps - 1 >> (p.cl_log + 5)) << 5;
+  const int seg = ((((m + 31) >> 5) + cl * kWarps - 1) >> (p.cl_log + 5)) << 5;
   const int w0 = min(gw * seg, m), w1 = min(w0 + seg, m);
   mass += first;
   // Keys of places past the stretch are 0, below every mass (the key of -inf is 0x007FFFFF).
@@ -348,10 +348,12 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const Params p, 
 
 static int launch(Params p, cudaStream_t st) {
   // CTAs per (row, head): enough that the pairs fill the SMs, as long as each warp
-  // still has 32 candidates of the longest row; and enough that a lane's keys fit 16 registers.
+  // still has 32 candidates of the longest row; and enough that a lane's keys fit 32 registers (at
+  // 32 rows of up to 32768 tokens one CTA with 32 keys per lane measured 47 us, two with 16 each 55:
+  // a pass is latency, and a cluster's barrier costs more than a CTA's).
   p.cl_log = 0;
   while ((1 << p.cl_log) < kMaxCluster && p.Lmax > (kThreads << p.cl_log) &&
-         (((long long)p.B * p.Hkv << p.cl_log) < num_sms() || p.Lmax > (16 * kThreads << p.cl_log)))
+         (((long long)p.B * p.Hkv << p.cl_log) < num_sms() || p.Lmax > (32 * kThreads << p.cl_log)))
     ++p.cl_log;
   const int cl = 1 << p.cl_log;
   p.heads = FastDiv::of(p.Hkv);
@@ -373,6 +375,8 @@ static int launch(Params p, cudaStream_t st) {
     FK_CHECK_CUDA(cudaLaunchKernelEx(&cfg, select_kernel<4>, p));
   else if (keys <= 16)
     FK_CHECK_CUDA(cudaLaunchKernelEx(&cfg, select_kernel<16>, p));
+  else if (keys <= 32)
+    FK_CHECK_CUDA(cudaLaunchKernelEx(&cfg, select_kernel<32>, p));
   else
     FK_CHECK_CUDA(cudaLaunchKernelEx(&cfg, select_kernel<0>, p));
   GatherPlan g;
@@ -382,8 +386,8 @@ static int launch(Params p, cudaStream_t st) {
   g.per_row = FastDiv::of(per_row);
   g.page_in = FastDiv::of(p.block_size);
   g.page_out = FastDiv::of(p.out_block_size);
-  // Tokens per block: one to four rounds of the unrolled loop.
-  g.tokens = (2 * kGatherThreads * kUnroll + per_tok - 1) / per_tok;
+  // Tokens per block: one round of the unrolled loop, or a token.
+  g.tokens = (kGatherThreads * kUnroll + per_tok - 1) / per_tok;
   cfg.gridDim = dim3((unsigned)((g.slots + g.tokens - 1) / g.tokens), (unsigned)p.B, 1);
   cfg.blockDim = dim3(kGatherThreads, 1, 1);
   cfg.numAttrs = 1;

@@ -154,21 +154,30 @@ def w4_linear(x, weight: W4Weight, out=None, *, residual=None, stream=None):
     if not isinstance(weight, W4Weight):
         raise TypeError(f"weight must be a W4Weight (pack_w4, quantize_w4), got {type(weight).__name__}")
     n, k, dt = weight.n, weight.k, weight.dtype
-    require_half("x", x, 2, dtype=dt, strided_rows=True)
-    m, xk = x.shape
-    if xk != k:
-        raise ValueError(f"x is [M, K={xk}] but the weight is [N={n}, K={k}]")
-    ldx = x.stride(0) if m > 1 else k
-    if ldx < k or ldx % 8:
-        raise ValueError(f"x row stride must be >= K and a multiple of 8 elements, got {ldx}")
-    if out is None:
-        out = torch.empty((m, n), dtype=dt, device=x.device)
-    else:
-        require_dense("out", out, dt, (m, n))
-    if residual is not None:
-        require_dense("residual", residual, dt, (m, n))
     packed = weight.packed
-    idx = one_device(x, packed, out, residual)
+    idx = packed.get_device()
+    # The shortest tests first: nothing more to ask if all of them hold.
+    if not (isinstance(x, torch.Tensor) and x.dtype == dt and x.dim() == 2 and x.shape[1] == k and x.get_device() == idx
+            and idx >= 0 and x.is_contiguous() and k % 8 == 0 and isinstance(out, torch.Tensor)
+            and out.dtype == dt and out.get_device() == idx and out.is_contiguous() and out.shape == (x.shape[0], n)
+            and (residual is None or (isinstance(residual, torch.Tensor) and residual.dtype == dt
+                                      and residual.get_device() == idx and residual.is_contiguous()
+                                      and residual.shape == out.shape))):
+        require_half("x", x, 2, dtype=dt, strided_rows=True)
+        m, xk = x.shape
+        if xk != k:
+            raise ValueError(f"x is [M, K={xk}] but the weight is [N={n}, K={k}]")
+        if m > 1 and (x.stride(0) < k or x.stride(0) % 8):
+            raise ValueError(f"x row stride must be >= K and a multiple of 8 elements, got {x.stride(0)}")
+        if out is None:
+            out = torch.empty((m, n), dtype=dt, device=x.device)
+        else:
+            require_dense("out", out, dt, (m, n))
+        if residual is not None:
+            require_dense("residual", residual, dt, (m, n))
+        idx = one_device(x, packed, out, residual)
+    m = x.shape[0]
+    ldx = x.stride(0) if m > 1 else k
     if m == 0:
         return out
     if idx != current_device():
