@@ -1,0 +1,121 @@
+// What the two forms of the 4-bit linear layer share: the packed weight's constants and
+// expansion, element conversions, bulk copies, and the hand-over of partial sums within a
+// cluster.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace fk {
+namespace w4 {
+
+constexpr int kBlockK = 128;    // inputs per packed block
+constexpr int kSlab = 2;        // blocks per slab
+
+// A checked call of the layer.
+struct Call {
+  const void* x;
+  long long ldx;
+  const uint8_t* packed;
+  const void* residual;
+  void* y;
+  int* err;
+  bool bf16;
+  int M, N, K, group;
+};
+// The form for more than 16 tokens (w4_tc.cu).
+int linear_tc(const Call& c, cudaStream_t st);
+
+// A word's eight nibbles as fp16 pairs of inputs (0,1) (2,3) (4,5) (6,7), offset by 256, 16, 256, 16.
+__device__ __forceinline__ void expand(uint32_t w, uint32_t (&p)[4]) {
+  const uint32_t t = __funnelshift_r(w, w, 8);
+  p[0] = (w & 0x003C003Cu) | 0x5C005C00u;
+  p[1] = (w & 0x03C003C0u) | 0x4C004C00u;
+  p[2] = (t & 0x003C003Cu) | 0x5C005C00u;
+  p[3] = (t & 0x03C003C0u) | 0x4C004C00u;
+}
+
+template <typename T>
+struct Half;
+template <>
+struct Half<__nv_bfloat16> {
+  static __device__ __forceinline__ float lo(uint32_t v) { return __uint_as_float(v << 16); }
+  static __device__ __forceinline__ float hi(uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); }
+  static __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+  static __device__ __forceinline__ __nv_bfloat16 round(float v) { return __float2bfloat16_rn(v); }
+};
+template <>
+struct Half<__half> {
+  static __device__ __forceinline__ float lo(uint32_t v) {
+    return __half2float(__ushort_as_half((unsigned short)(v & 0xFFFFu)));
+  }
+  static __device__ __forceinline__ float hi(uint32_t v) {
+    return __half2float(__ushort_as_half((unsigned short)(v >> 16)));
+  }
+  static __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+  static __device__ __forceinline__ __half round(float v) { return __float2half_rn(v); }
+};
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar, uint64_t pol) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(
+          dst),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar)), "l"(pol)
+      : "memory");
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// Shared-memory address of the same place in another CTA of the cluster.
+__device__ __forceinline__ uint32_t map_to(uint32_t addr, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void ld_cluster(uint32_t addr, float& a, float& b) {
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(a), "=f"(b) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void st_cluster(uint32_t addr, float a, float b) {
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(addr), "f"(a), "f"(b) : "memory");
+}
+__device__ __forceinline__ void st_cluster4(uint32_t addr, float a, float b, float c, float d) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
+}
+// One arrival on another CTA's mbarrier, after everything this thread has seen (its CTA's stores
+// into the cluster, ordered before it by a CTA barrier).
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// Bounded wait for arrivals from the cluster, with acquire at its scope.
+__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, int* err) {
+  const uint64_t t0 = global_timer_ns();
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if (global_timer_ns() - t0 > wait_limit_ns(err)) break;
+  }
+  record_device_error(err, kDevErrFlagWait);
+  return false;
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+  return v;
+}
+
+template <int GROUP>
+__host__ __device__ constexpr int block_bytes() { return 1024 + (kBlockK / GROUP) * 64; }
+}  // namespace w4
+}  // namespace fk

@@ -1,4 +1,4 @@
-// Linear layer with 4-bit weights and group scales for a few tokens:
+// Linear layer with 4-bit weights and group scales for up to 16 tokens (more: w4_tc.cu):
 //   y[m, n] = sum_k x[m, k] * (q[n, k] - z[n, k / g]) * s[n, k / g]  (+ residual[m, n])
 // with q, z in [0, 15], g in {32, 64, 128} and x, s, y bf16 or fp16.
 //
@@ -48,12 +48,11 @@
 
 #include "common.cuh"
 #include "fk_b200.h"
+#include "w4.cuh"
 
 namespace fk {
 namespace w4 {
 
-constexpr int kBlockK = 128;    // inputs per packed block
-constexpr int kSlab = 2;        // blocks per slab
 constexpr int kSlabK = kSlab * kBlockK;
 constexpr int kGroupWarps = 8;  // warps that share a stage
 constexpr int kStages = 6;
@@ -75,36 +74,6 @@ struct Params {
   int tile;                  // row blocks per cluster whose partial sums are held at a time
 };
 
-// A word's eight nibbles as fp16 pairs of inputs (0,1) (2,3) (4,5) (6,7), offset by 256, 16, 256, 16.
-__device__ __forceinline__ void expand(uint32_t w, uint32_t (&p)[4]) {
-  const uint32_t t = __funnelshift_r(w, w, 8);
-  p[0] = (w & 0x003C003Cu) | 0x5C005C00u;
-  p[1] = (w & 0x03C003C0u) | 0x4C004C00u;
-  p[2] = (t & 0x003C003Cu) | 0x5C005C00u;
-  p[3] = (t & 0x03C003C0u) | 0x4C004C00u;
-}
-
-template <typename T>
-struct Half;
-template <>
-struct Half<__nv_bfloat16> {
-  static __device__ __forceinline__ float lo(uint32_t v) { return __uint_as_float(v << 16); }
-  static __device__ __forceinline__ float hi(uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); }
-  static __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-  static __device__ __forceinline__ __nv_bfloat16 round(float v) { return __float2bfloat16_rn(v); }
-};
-template <>
-struct Half<__half> {
-  static __device__ __forceinline__ float lo(uint32_t v) {
-    return __half2float(__ushort_as_half((unsigned short)(v & 0xFFFFu)));
-  }
-  static __device__ __forceinline__ float hi(uint32_t v) {
-    return __half2float(__ushort_as_half((unsigned short)(v >> 16)));
-  }
-  static __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-  static __device__ __forceinline__ __half round(float v) { return __float2half_rn(v); }
-};
-
 // D = A * B: the first step of a group starts from nothing.
 __device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -113,55 +82,6 @@ __device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4],
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar, uint64_t pol) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(
-          dst),
-      "l"(src), "r"(bytes), "r"(smem_u32(bar)), "l"(pol)
-      : "memory");
-}
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-// Shared-memory address of the same place in another CTA of the cluster.
-__device__ __forceinline__ uint32_t map_to(uint32_t addr, int rank) {
-  uint32_t r;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void ld_cluster(uint32_t addr, float& a, float& b) {
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(a), "=f"(b) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void st_cluster(uint32_t addr, float a, float b) {
-  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(addr), "f"(a), "f"(b) : "memory");
-}
-// One arrival on another CTA's mbarrier, after everything this thread has seen (its CTA's stores
-// into the cluster, ordered before it by a CTA barrier).
-__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-// Bounded wait for arrivals from the cluster, with acquire at its scope.
-__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, int* err) {
-  const uint64_t t0 = global_timer_ns();
-  while (true) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    if (ok) return true;
-    if (global_timer_ns() - t0 > wait_limit_ns(err)) break;
-  }
-  record_device_error(err, kDevErrFlagWait);
-  return false;
-}
-__device__ __forceinline__ uint4 lds128(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-  return v;
-}
 __device__ __forceinline__ float4 lds128f(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
@@ -172,14 +92,6 @@ __device__ __forceinline__ float2 lds64f(uint32_t addr) {
   asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr));
   return v;
 }
-__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
-  return v;
-}
-
-template <int GROUP>
-__host__ __device__ constexpr int block_bytes() { return 1024 + (kBlockK / GROUP) * 64; }
 constexpr int kWarps = 16;  // that multiply
 template <int GROUP>
 __host__ __device__ constexpr int stage_bytes() { return kGroupWarps * kSlab * block_bytes<GROUP>(); }
@@ -214,8 +126,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, 1) w4_linear_kernel(const Pa
 
   // The host did the divisions: emulated ones in every warp cost a small call 1.4 us.
   const int cs = 1 << p.cs_log, rank = blockIdx.x & (cs - 1), cid = blockIdx.x >> p.cs_log;
-  const int tok0 = blockIdx.y * TOK;
-  const int ntok = min(TOK, p.M - tok0);
+  const int ntok = p.M;  // at most TOK
   // This cluster's row blocks; this CTA's slabs are rank, rank + cs, ...
   const int rb0 = cid * p.rb_each + min(cid, p.rb_more), rb1 = rb0 + p.rb_each + (cid < p.rb_more);
   const int nsl = (p.nslab - rank + cs - 1) >> p.cs_log;
@@ -344,7 +255,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, 1) w4_linear_kernel(const Pa
             if (sl < c1) {
               const int k = (rank + sl * cs) * kSlabK + lane * 8;
               if (k < p.K)
-                v[u] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + (size_t)(tok0 + n) * p.ldx + k);
+                v[u] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + (size_t)n * p.ldx + k);
               n += W;
               while (sl < c1 && n >= ntok) n -= ntok, ++sl;
             }
@@ -522,7 +433,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, 1) w4_linear_kernel(const Pa
         const int slot = i / (TOK / 4), n = (i % (TOK / 4)) * 4;  // TOK is a power of two
         const int row = (r0 + (slot << p.cs_log) + rank) * 16 + r;
         if (n >= ntok || row >= p.N) continue;
-        const size_t off = (size_t)(tok0 + n) * p.N + row;
+        const size_t off = (size_t)n * p.N + row;
         float res[4] = {0.f, 0.f, 0.f, 0.f};
         if (p.residual) {
 #pragma unroll
@@ -590,14 +501,12 @@ static int launch(Params p, cudaStream_t st) {
   int resident[4];
   int rc = resident_clusters<T, NT, GROUP>(resident);
   if (rc) return rc;
-  const int tiles = (p.M + NT * 8 - 1) / (NT * 8);
   // Four CTAs per cluster where there are slabs for them: measured best or within 2 % of it from one
-  // token on 4096 rows to 64 on 14336 inputs. Two or one leave too many slabs of x to every CTA, eight
+  // token on 4096 rows to 16 on 28672. Two or one leave too many slabs of x to every CTA, eight
   // leave SMs idle (15 clusters of 8, 36 of 4 are resident on 148 SMs).
   p.cs_log = p.nslab >= 4 ? 2 : p.nslab >= 2 ? 1 : 0;
   const int cs = 1 << p.cs_log;
-  int ncl = resident[p.cs_log] / tiles;
-  ncl = ncl < 1 ? 1 : ncl > p.nrb ? p.nrb : ncl;
+  const int ncl = resident[p.cs_log] > p.nrb ? p.nrb : resident[p.cs_log];
   const int rows = (p.nrb + ncl - 1) / ncl, slabs = (p.nslab + cs - 1) / cs;
   // Few rows per cluster: two warps share a row block. Each part costs a plane of partial sums.
   p.kw_log = 2 * rows <= kWarps ? 1 : 0;
@@ -621,7 +530,7 @@ static int launch(Params p, cudaStream_t st) {
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(ncl << p.cs_log), (unsigned)tiles, 1);
+  cfg.gridDim = dim3((unsigned)(ncl << p.cs_log), 1, 1);
   cfg.blockDim = dim3(kWarps * 32 + 32, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
@@ -638,12 +547,9 @@ static int by_group(const Params& p, int group, cudaStream_t st) {
   return launch<T, NT, 128>(p, st);
 }
 
-// 8, 16 or 32 tokens share one pass over the weight; more go in passes of 32, side by side.
 template <typename T>
 static int by_tokens(const Params& p, int group, cudaStream_t st) {
-  if (p.M <= 8) return by_group<T, 1>(p, group, st);
-  if (p.M <= 16) return by_group<T, 2>(p, group, st);
-  return by_group<T, 4>(p, group, st);
+  return p.M <= 8 ? by_group<T, 1>(p, group, st) : by_group<T, 2>(p, group, st);
 }
 
 }  // namespace w4
@@ -664,12 +570,18 @@ extern "C" int fk_w4_linear(const void* x, long long ldx, const void* packed, co
   FK_CHECK_ARG(((uintptr_t)x & 15) == 0 && ((uintptr_t)packed & 15) == 0,
                "x and packed must be 16-byte aligned");
   FK_CHECK_ARG(((uintptr_t)y & 1) == 0 && ((uintptr_t)residual & 1) == 0, "y and residual must be 2-byte aligned");
+  int* err = device_error_word();
+  if (!err) return fail(kErrCuda, "device error word unavailable");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (M > 16) {
+    const w4::Call c{x, ldx, static_cast<const uint8_t*>(packed), residual, y, err, dtype == FK_BF16, M, N, K, group_size};
+    return w4::linear_tc(c, st);
+  }
   w4::Params p = {};
   p.x = x;
   p.ldx = ldx;
   p.packed = static_cast<const uint8_t*>(packed);
-  p.err = device_error_word();
-  if (!p.err) return fail(kErrCuda, "device error word unavailable");
+  p.err = err;
   p.residual = residual;
   p.y = y;
   p.M = M;
@@ -678,7 +590,6 @@ extern "C" int fk_w4_linear(const void* x, long long ldx, const void* packed, co
   p.nrb = (N + 15) / 16;
   p.nkb = (K + w4::kBlockK - 1) / w4::kBlockK;
   p.nslab = (p.nkb + w4::kSlab - 1) / w4::kSlab;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == FK_BF16) return w4::by_tokens<__nv_bfloat16>(p, group_size, st);
   return w4::by_tokens<__half>(p, group_size, st);
 }

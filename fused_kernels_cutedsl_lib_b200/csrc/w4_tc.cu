@@ -1,0 +1,507 @@
+// Linear layer with 4-bit weights and group scales for more than 16 tokens, on tcgen05:
+//   y[m, n] = sum_k x[m, k] * (q[n, k] - z[n, k / g]) * s[n, k / g]  (+ residual[m, n])
+// (the layout of the weight and the form for up to 16 tokens are in w4_linear.cu).
+//
+// Bound: up to 64 tokens share one pass over the weight, so a weight is expanded once
+// and the products cost the tensor cores a fraction of the time that the expansion
+// costs the ALU. mma.sync, which the form for few tokens uses, pays 32 products and 16
+// shared-memory reads per KB of weight at 32 tokens: 61 us for 64 tokens on 4096 x 14336
+// against 16 us here.
+//
+// One CTA: 128 output rows, a slice of the inputs, N tokens (32 or 64). Per slab of 256
+// inputs
+//   * warp 8 copies the rows' packed blocks (one bulk copy, contiguous) and x (TMA,
+//     128B-swizzled boxes of 64 inputs x N tokens) into a ring of stages;
+//   * warps 0-3 take the slab's first 128 inputs, warps 4-7 the others. Thread = row =
+//     TMEM lane: it expands its row's 16 words to the exact integers q - z (bf16: 128 + q
+//     from one rotation and one logic instruction per pair, minus 128 + z; fp16: 256 + q
+//     and 16 + q) and stores them to TMEM as the A operand (two buffers);
+//   * warp 9 issues D = A x^T, one accumulator per group of g inputs, and commits;
+//   * while it runs, the threads expand the next block; then each reads its row of D and
+//     adds s * D to its fp32 sums, N registers. Integers and x are exact, so the only
+//     roundings are those of fp32 sums and the output.
+// The inputs are split over the CS CTAs of a cluster; each warp group's sums go to the
+// shared memory of the CTA that owns the rows (mbarrier with one arrival per CTA), which
+// adds them in a fixed order: no workspace, no atomic.
+#include <cuda_fp16.h>
+
+#include <mutex>
+#include <type_traits>
+
+#include "common.cuh"
+#include "fk_b200.h"
+#include "w4.cuh"
+
+namespace fk {
+namespace w4tc {
+
+using w4::kBlockK;
+using w4::kSlab;
+
+constexpr int kRows = 128;     // output rows per CTA (UMMA M, TMEM lanes)
+constexpr int kRowBlocks = 8;  // of 16 rows
+constexpr int kThreads = 320;
+constexpr int kLoadWarp = 8, kMmaWarp = 9;
+constexpr int kSmem = 227 * 1024;
+constexpr uint32_t kACol = 256;  // TMEM: D of warp group w at 128 w, its A buffers at 256 + 128 w + 64 buf
+
+struct Params {
+  const uint8_t* packed;
+  const void* residual;
+  void* y;
+  int* err;
+  int M, N;
+  int nrb, nkb, nslab;
+  int cs_log;
+};
+
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// K-major operand, 128B swizzle, 8-row groups 1024 B apart.
+__device__ __forceinline__ uint64_t desc_k_sw128(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+// kind::f16, A and B both bf16 or both fp16, D fp32, M = 128, N = n.
+template <typename T>
+__host__ __device__ constexpr uint32_t idesc(int n) {
+  constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  return (1u << 4) | (kType << 7) | (kType << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+}
+// D (+)= A . B with A (M = 128 x K = 16, 16-bit pairs packed per 32-bit column) in TMEM.
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(db), "r"(id), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+// 32 consecutive TMEM columns of this thread's lane (no wait).
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+      "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]),
+      "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]),
+      "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// One row's word as the exact 16-bit integers q - z, four pairs of neighbouring inputs.
+template <typename T>
+struct Expand;
+template <>
+struct Expand<__nv_bfloat16> {
+  __nv_bfloat162 c;  // 128 + z, twice
+  __device__ __forceinline__ void zero(uint32_t sz) {
+    const float z = __uint_as_float(sz & 0xFFFF0000u);
+    c = __float2bfloat162_rn(128.f + z);
+  }
+  __device__ __forceinline__ void word(uint32_t w, uint32_t* p) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t v = (__funnelshift_r(w, w, 4 * i + 2) & 0x000F000Fu) | 0x43004300u;
+      const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), c);
+      p[i] = *reinterpret_cast<const uint32_t*>(&d);
+    }
+  }
+};
+template <>
+struct Expand<__half> {
+  __half2 c256, c16;
+  __device__ __forceinline__ void zero(uint32_t sz) {
+    const float z = __half2float(__ushort_as_half((unsigned short)(sz >> 16)));
+    c256 = __float2half2_rn(256.f + z);
+    c16 = __float2half2_rn(16.f + z);
+  }
+  __device__ __forceinline__ void word(uint32_t w, uint32_t* p) const {
+    uint32_t v[4];
+    w4::expand(w, v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&v[i]), i & 1 ? c16 : c256);
+      p[i] = *reinterpret_cast<const uint32_t*>(&d);
+    }
+  }
+};
+
+template <int GROUP>
+__host__ __device__ constexpr int weight_bytes() { return (kRowBlocks * kSlab * w4::block_bytes<GROUP>() + 1023) / 1024 * 1024; }
+template <int NTOK, int GROUP>
+__host__ __device__ constexpr int stage_bytes() { return weight_bytes<GROUP>() + kSlab * 2 * NTOK * 128; }
+// Partial sums of the rows a CTA owns, from two warp groups of every CTA of the cluster; 4 floats of padding per
+// row keep a warp's 16-byte stores on distinct banks.
+template <int NTOK>
+__host__ __device__ constexpr int part_bytes() { return 2 * kRows * (NTOK + 4) * 4; }
+template <int NTOK, int GROUP>
+__host__ __device__ constexpr int stages() {
+  constexpr int s = (kSmem - 2048 - part_bytes<NTOK>()) / stage_bytes<NTOK, GROUP>();
+  return s > 6 ? 6 : s;
+}
+
+template <typename T, int NTOK, int GROUP>
+__global__ void __launch_bounds__(kThreads, 1)
+    w4_tc_kernel(const __grid_constant__ CUtensorMap tmX, const Params p) {
+  constexpr int S = stages<NTOK, GROUP>();
+  static_assert(S >= 2, "");
+  constexpr int GPB = kBlockK / GROUP;
+  static_assert(GPB * NTOK <= 128, "a warp group's accumulators have 128 columns");
+  constexpr int BB = w4::block_bytes<GROUP>();
+  constexpr int STAGE = stage_bytes<NTOK, GROUP>();
+  constexpr int XOFF = weight_bytes<GROUP>();
+  constexpr int PR = NTOK + 4;  // floats per row of partial sums
+  extern __shared__ uint8_t smem_raw[];
+  // Aligned by the shared-window address: the same in every CTA of the cluster.
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  float* part_buf = reinterpret_cast<float*>(smem + S * STAGE);  // [2 cs][128 / cs][PR]
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S * STAGE + part_bytes<NTOK>());
+  uint64_t* empty = full + S;    // 8 warps have read the weights, the MMAs have read x
+  uint64_t* a_full = empty + S;  // [2 groups][2 buffers]
+  uint64_t* d_full = a_full + 4; // [2]
+  uint64_t* d_empty = d_full + 2;
+  uint64_t* done = d_empty + 2;  // one arrival per CTA: its partial sums are stored
+  uint64_t* tmem_done = done + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_done + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int cs = 1 << p.cs_log, rank = blockIdx.x & (cs - 1), tile = blockIdx.x >> p.cs_log;
+  const int tok0 = blockIdx.y * NTOK;
+  const int nsl = (p.nslab - rank + cs - 1) >> p.cs_log;  // slabs rank, rank + cs, ..
+  auto slab_blocks = [&](int s) { return min(kSlab, p.nkb - s * kSlab); };
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 9);
+    }
+    for (int i = 0; i < 4; ++i) mbar_init(&a_full[i], 4);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&d_full[i], 1);
+      mbar_init(&d_empty[i], 4);
+    }
+    mbar_init(done, cs);
+    mbar_init(tmem_done, 8);
+    fence_barrier_init();
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  // The other CTAs must have started, their barriers included, before anything is stored into their
+  // shared memory. The only phase of the cluster's own barrier.
+  w4::cluster_arrive();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  if (warp == kLoadWarp) {
+    // ------------------------------ loads ------------------------------
+    if (lane == 0) {
+      tma_prefetch_desc(&tmX);
+      const uint64_t pol_w = l2_policy_evict_first(), pol_x = l2_policy_evict_last();
+      const int rows = min(kRowBlocks, p.nrb - tile * kRowBlocks);
+      auto load_w = [&](int i) {
+        const int st = i % S, s = rank + i * cs, nb = slab_blocks(s);
+        const uint32_t bytes = (uint32_t)(rows * nb) * BB;
+        mbar_arrive_expect_tx(&full[st], bytes + nb * 2 * NTOK * 128);
+        w4::bulk_load(smem_u32(smem + st * STAGE),
+                      p.packed + ((size_t)s * kSlab * p.nrb + (size_t)tile * kRowBlocks * nb) * BB, bytes, &full[st], pol_w);
+      };
+      auto load_x = [&](int i) {
+        const int st = i % S, s = rank + i * cs, nb = slab_blocks(s);
+        for (int q = 0; q < nb * 2; ++q)
+          tma_load_2d(smem + st * STAGE + XOFF + q * (NTOK * 128), &tmX, &full[st], s * kSlab * kBlockK + q * 64, tok0,
+                      pol_x);
+      };
+      // The weights' first copies do not wait for the preceding kernel, x does.
+      const int ahead = min(S, nsl);
+      for (int i = 0; i < ahead; ++i) load_w(i);
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      for (int i = 0; i < ahead; ++i) load_x(i);
+      for (int i = ahead; i < nsl; ++i) {
+        if (!mbar_wait(&empty[i % S], ((i / S) & 1) ^ 1, p.err, kDevErrEmptyWait)) break;
+        load_w(i);
+        load_x(i);
+      }
+    }
+    __syncwarp();
+    w4::cluster_wait();
+    return;
+  }
+
+  if (warp == kMmaWarp) {
+    // ------------------------------ products ------------------------------
+    if (lane == 0) {
+      constexpr uint32_t ID = idesc<T>(NTOK);
+      bool ok = true;
+      for (int i = 0; i < nsl && ok; ++i) {
+        const int st = i % S, nb = slab_blocks(rank + i * cs);
+        ok = mbar_wait(&full[st], (i / S) & 1, p.err, kDevErrFullWait);
+        for (int w = 0; w < nb && ok; ++w) {
+          // The group's block i: its A buffer is i & 1, used before for block i - 2. (Only the last slab
+          // can lack a block, so both groups count alike.)
+          ok = mbar_wait(&a_full[w * 2 + (i & 1)], (i >> 1) & 1, p.err, kDevErrMmaWait) &&
+               (i == 0 || mbar_wait(&d_empty[w], (i - 1) & 1, p.err, kDevErrMmaWait));
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t xb = smem_u32(smem + st * STAGE + XOFF) + w * (2 * NTOK * 128);
+          const uint32_t a = tmem + kACol + w * 128 + (i & 1) * 64, d = tmem + w * 128;
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk) {
+            const int gi = kk * 16 / GROUP;
+            umma_ts(d + gi * NTOK, a + kk * 8, desc_k_sw128(xb + (kk >> 2) * (NTOK * 128) + (kk & 3) * 32), ID,
+                    kk * 16 % GROUP ? 1u : 0u);
+          }
+          umma_commit(&d_full[w]);
+        }
+        if (ok) umma_commit(&empty[st]);
+      }
+    }
+    __syncwarp();
+    mbar_wait(tmem_done, 0, p.err, kDevErrMmaWait);  // D has been read
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    w4::cluster_wait();
+    return;
+  }
+
+  // ------------------------------ expand and add up ------------------------------
+  const int wg = warp >> 2, quarter = warp & 3;
+  const int r = 32 * quarter + lane;  // this thread's row of the tile, its TMEM lane
+  const uint32_t tlane = tmem + ((uint32_t)(32 * quarter) << 16);
+  const uint32_t d_addr = tlane + wg * 128, a_addr = tlane + kACol + wg * 128;
+  float acc[NTOK];
+#pragma unroll
+  for (int n = 0; n < NTOK; ++n) acc[n] = 0.f;
+  float scale[GPB];  // of the block whose D is awaited
+  bool ok = true;
+  // acc += scale * D of block i.
+  auto collect = [&](int i) {
+    if (!__all_sync(~0u, mbar_wait(&d_full[wg], i & 1, p.err, kDevErrMmaWait))) return false;
+    tc_fence_after();
+#pragma unroll
+    for (int gi = 0; gi < GPB; ++gi) {
+      uint32_t d[NTOK];
+#pragma unroll
+      for (int c = 0; c < NTOK / 32; ++c) tmem_ld32(d_addr + gi * NTOK + c * 32, d + c * 32);
+      tmem_ld_wait();
+#pragma unroll
+      for (int n = 0; n < NTOK; ++n) acc[n] = fmaf(scale[gi], __uint_as_float(d[n]), acc[n]);
+    }
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&d_empty[wg]);
+    return true;
+  };
+  int mine = 0;  // blocks this group has expanded
+  for (int i = 0; i < nsl; ++i) {
+    const int st = i % S, nb = slab_blocks(rank + i * cs);
+    ok = __all_sync(~0u, mbar_wait(&full[st], (i / S) & 1, p.err, kDevErrFullWait));
+    if (!ok) break;
+    float next[GPB];
+    if (wg < nb) {
+      const uint32_t ba = smem_u32(smem + st * STAGE) + ((r >> 4) * nb + wg) * BB + (r & 15) * 64;
+      const uint32_t sa = ba - (r & 15) * 60 + 1024;
+      uint32_t words[4][4];  // [c][j]: inputs 32 j + 8 c
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const uint4 v = w4::lds128(ba + c * 16);
+        words[c][0] = v.x, words[c][1] = v.y, words[c][2] = v.z, words[c][3] = v.w;
+      }
+      Expand<T> ex[GPB];
+#pragma unroll
+      for (int gi = 0; gi < GPB; ++gi) {
+        const uint32_t sz = w4::lds32(sa + gi * 64);
+        next[gi] = w4::Half<T>::lo(sz);
+        ex[gi].zero(sz);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {  // 64 inputs: 32 columns
+        uint32_t a[32];
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) ex[(2 * h + jj) * 32 / GROUP].word(words[c][2 * h + jj], a + jj * 16 + c * 4);
+        tmem_st32(a_addr + (i & 1) * 64 + h * 32, a);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&a_full[wg * 2 + (i & 1)]);
+    }
+    if (lane == 0) mbar_arrive(&empty[st]);
+    if (i > 0) ok = collect(i - 1);
+    if (!ok) break;
+    if (wg < nb) {
+      mine = i + 1;
+#pragma unroll
+      for (int gi = 0; gi < GPB; ++gi) scale[gi] = next[gi];
+    }
+  }
+  if (ok && mine == nsl) ok = collect(nsl - 1);
+  __syncwarp();
+  if (lane == 0) mbar_arrive(tmem_done);
+
+  // ---- the sums go to the CTAs that own the rows, 128 / cs each ----
+  w4::cluster_wait();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  {
+    const int rows_log = 7 - p.cs_log, owner = r >> rows_log, slot = r & ((1 << rows_log) - 1);
+    const uint32_t to =
+        w4::map_to(smem_u32(part_buf + ((size_t)((rank * 2 + wg) << rows_log) + slot) * PR), owner);
+#pragma unroll
+    for (int n = 0; n < NTOK; n += 4) w4::st_cluster4(to + n * 4, acc[n], acc[n + 1], acc[n + 2], acc[n + 3]);
+    named_bar_sync(1, 256);
+    if (warp == 0 && lane < cs) w4::arrive_cluster(w4::map_to(smem_u32(done), lane));
+    if (!w4::wait_cluster(done, 0, p.err)) return;
+    const int rows = 1 << rows_log, plane = rows * PR;
+    // Lanes along the rows: a token's outputs are contiguous.
+    for (int e = threadIdx.x; e < rows * (NTOK / 4); e += 256) {
+      const int row_in = e & (rows - 1), n = (e >> rows_log) * 4;
+      const int row = tile * kRows + rank * rows + row_in;
+      if (row >= p.N || tok0 + n >= p.M) continue;
+      const float* from = part_buf + row_in * PR + n;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int q = 0; q < 2 * cs; ++q) {
+        const float4 f = *reinterpret_cast<const float4*>(from + q * plane);
+        v.x += f.x, v.y += f.y, v.z += f.z, v.w += f.w;
+      }
+      const float out[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (tok0 + n + i >= p.M) break;
+        const size_t off = (size_t)(tok0 + n + i) * p.N + row;
+        float o = out[i];
+        if (p.residual) o += w4::Half<T>::to_float(static_cast<const T*>(p.residual)[off]);
+        static_cast<T*>(p.y)[off] = w4::Half<T>::round(o);
+      }
+    }
+  }
+}
+
+// Clusters of 1, 2, 4 and 8 CTAs that can be resident at once, asked once per kernel and device.
+template <typename T, int NTOK, int GROUP>
+static int resident_clusters(int smem, int (&out)[4]) {
+  constexpr int kDevices = 64;
+  static std::mutex mu;
+  static int known[kDevices][4] = {};
+  auto kern = w4_tc_kernel<T, NTOK, GROUP>;
+  int dev = 0;
+  FK_CHECK_CUDA(cudaGetDevice(&dev));
+  FK_CHECK_ARG(dev >= 0 && dev < kDevices, "device index too large");
+  std::lock_guard<std::mutex> lock(mu);
+  int* k = known[dev];
+  if (k[3] == 0) {
+    FK_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    for (int i = 0; i < 4; ++i) {
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = 1 << i;
+      attr[0].val.clusterDim.y = 1;
+      attr[0].val.clusterDim.z = 1;
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(1u << i, 1, 1);
+      cfg.blockDim = dim3(kThreads, 1, 1);
+      cfg.dynamicSmemBytes = smem;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      int n = 0;
+      FK_CHECK_CUDA(cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
+      k[i] = n < 1 ? 1 : n;
+    }
+  }
+  for (int i = 0; i < 4; ++i) out[i] = k[i];
+  return kOk;
+}
+
+template <typename T, int NTOK, int GROUP>
+static int launch(const w4::Call& c, cudaStream_t st) {
+  constexpr int smem = 1024 + stages<NTOK, GROUP>() * stage_bytes<NTOK, GROUP>() + part_bytes<NTOK>() + 512;
+  static_assert(smem <= kSmem, "shared memory budget");
+  int resident[4];
+  int rc = resident_clusters<T, NTOK, GROUP>(smem, resident);
+  if (rc) return rc;
+  Params p;
+  p.packed = c.packed;
+  p.residual = c.residual;
+  p.y = c.y;
+  p.err = c.err;
+  p.M = c.M;
+  p.N = c.N;
+  p.nrb = (c.N + 15) / 16;
+  p.nkb = (c.K + kBlockK - 1) / kBlockK;
+  p.nslab = (p.nkb + kSlab - 1) / kSlab;
+  const long long row_tiles = (c.N + kRows - 1) / kRows, tok_tiles = (c.M + NTOK - 1) / NTOK;
+  // CTAs per cluster: the least waves x (slabs of the busiest CTA + what a CTA costs besides, as much as
+  // six slabs).
+  long long best = -1;
+  for (int l = 0; l < 4 && (1 << l) <= p.nslab; ++l) {
+    const long long waves = (row_tiles * tok_tiles + resident[l] - 1) / resident[l];
+    const long long cost = waves * ((p.nslab + (1 << l) - 1) / (1 << l) + 6);
+    if (best < 0 || cost < best) {
+      best = cost;
+      p.cs_log = l;
+    }
+  }
+  FK_CHECK_ARG(row_tiles << p.cs_log < (1LL << 31), "N too large");
+  CUtensorMap tmX;
+  const uint64_t dims[2] = {(uint64_t)c.K, (uint64_t)c.M};
+  const uint64_t strides[1] = {(uint64_t)c.ldx * 2};
+  const uint32_t box[2] = {64, NTOK};
+  rc = encode_tma(&tmX,
+                  std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                        : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                  2, const_cast<void*>(c.x), dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc) return rc;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 1 << p.cs_log;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(row_tiles << p.cs_log), (unsigned)tok_tiles, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  FK_CHECK_CUDA(cudaLaunchKernelEx(&cfg, w4_tc_kernel<T, NTOK, GROUP>, tmX, p));
+  return kOk;
+}
+
+template <typename T>
+static int by_group(const w4::Call& c, cudaStream_t st) {
+  // Tokens per pass: 64, or 32 where that is enough or the groups' accumulators need the columns.
+  if (c.group == 32) return launch<T, 32, 32>(c, st);
+  if (c.M <= 32) return c.group == 64 ? launch<T, 32, 64>(c, st) : launch<T, 32, 128>(c, st);
+  return c.group == 64 ? launch<T, 64, 64>(c, st) : launch<T, 64, 128>(c, st);
+}
+
+}  // namespace w4tc
+
+int w4::linear_tc(const Call& c, cudaStream_t st) {
+  return c.bf16 ? w4tc::by_group<__nv_bfloat16>(c, st) : w4tc::by_group<__half>(c, st);
+}
+
+}  // namespace fk
