@@ -10,18 +10,18 @@
 //
 // One CTA: 128 output rows, a slice of the inputs, N tokens (32 or 64). Per slab of 256
 // inputs
-//   * warp 8 copies the rows' packed blocks (one bulk copy, contiguous) and x (TMA,
+//   * warp 16 copies the rows' packed blocks (one bulk copy, contiguous) and x (TMA,
 //     128B-swizzled boxes of 64 inputs x N tokens) into a ring of stages;
 //   * warps 0-3 take the slab's first 128 inputs, warps 4-7 the others. Thread = row =
 //     TMEM lane: it expands its row's 16 words to the exact integers q - z (bf16: 128 + q
 //     from one rotation and one logic instruction per pair, minus 128 + z; fp16: 256 + q
 //     and 16 + q) and stores them to TMEM as the A operand (two buffers);
-//   * warp 9 issues D = A x^T, one accumulator per group of g inputs, and commits;
-//   * while it runs, the threads expand the next block; then each reads its row of D and
-//     adds s * D to its fp32 sums, N registers. Integers and x are exact, so the only
-//     roundings are those of fp32 sums and the output.
-// The inputs are split over the CS CTAs of a cluster; each warp group's sums go to the
-// shared memory of the CTA that owns the rows (mbarrier with one arrival per CTA), which
+//   * warp 17 issues D = A x^T, one accumulator per group of g inputs, and commits;
+//   * warps 8-15 (thread = row and half of the tokens) read D and add s * D to their fp32
+//     sums. Integers and x are exact, so the only roundings are those of fp32 sums and
+//     the output. (The expanding warps adding up themselves: XX us.)
+// The inputs are split over the CS CTAs of a cluster; their sums go to the shared memory
+// of the CTA that owns the rows (mbarrier with one arrival per CTA), which
 // adds them in a fixed order: no workspace, no atomic.
 #include <cuda_fp16.h>
 
@@ -40,8 +40,8 @@ using w4::kSlab;
 
 constexpr int kRows = 128;     // output rows per CTA (UMMA M, TMEM lanes)
 constexpr int kRowBlocks = 8;  // of 16 rows
-constexpr int kThreads = 320;
-constexpr int kLoadWarp = 8, kMmaWarp = 9;
+constexpr int kThreads = 608;
+constexpr int kLoadWarp = 16, kMmaWarp = 17;  // 0-7 expand, 8-15 add up, 17 and 18 issue the products
 constexpr int kSmem = 227 * 1024;
 constexpr uint32_t kACol = 256;  // TMEM: D of warp group w at 128 w, its A buffers at 256 + 128 w + 64 buf
 
@@ -101,6 +101,13 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
         "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr));
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -146,10 +153,10 @@ template <int GROUP>
 __host__ __device__ constexpr int weight_bytes() { return (kRowBlocks * kSlab * w4::block_bytes<GROUP>() + 1023) / 1024 * 1024; }
 template <int NTOK, int GROUP>
 __host__ __device__ constexpr int stage_bytes() { return weight_bytes<GROUP>() + kSlab * 2 * NTOK * 128; }
-// Partial sums of the rows a CTA owns, from two warp groups of every CTA of the cluster; 4 floats of padding per
-// row keep a warp's 16-byte stores on distinct banks.
+// Partial sums of the rows a CTA owns, from every CTA of the cluster; 4 floats of padding per row keep a warp's
+// 16-byte stores on distinct banks.
 template <int NTOK>
-__host__ __device__ constexpr int part_bytes() { return 2 * kRows * (NTOK + 4) * 4; }
+__host__ __device__ constexpr int part_bytes() { return kRows * (NTOK + 4) * 4; }
 template <int NTOK, int GROUP>
 __host__ __device__ constexpr int stages() {
   constexpr int s = (kSmem - 2048 - part_bytes<NTOK>()) / stage_bytes<NTOK, GROUP>();
@@ -162,7 +169,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int S = stages<NTOK, GROUP>();
   static_assert(S >= 2, "");
   constexpr int GPB = kBlockK / GROUP;
-  static_assert(GPB * NTOK <= 128, "a warp group's accumulators have 128 columns");
+  static_assert(GPB * NTOK <= 128, "the accumulators of a slab's first and second blocks have 128 columns each");
+  constexpr int DB = GPB * NTOK <= 64 ? 2 : 1;  // accumulator buffers
   constexpr int BB = w4::block_bytes<GROUP>();
   constexpr int STAGE = stage_bytes<NTOK, GROUP>();
   constexpr int XOFF = weight_bytes<GROUP>();
@@ -170,13 +178,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   // Aligned by the shared-window address: the same in every CTA of the cluster.
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  float* part_buf = reinterpret_cast<float*>(smem + S * STAGE);  // [2 cs][128 / cs][PR]
+  float* part_buf = reinterpret_cast<float*>(smem + S * STAGE);  // [cs][128 / cs][PR]
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + S * STAGE + part_bytes<NTOK>());
-  uint64_t* empty = full + S;    // 8 warps have read the weights, the MMAs have read x
-  uint64_t* a_full = empty + S;  // [2 groups][2 buffers]
-  uint64_t* d_full = a_full + 4; // [2]
-  uint64_t* d_empty = d_full + 2;
-  uint64_t* done = d_empty + 2;  // one arrival per CTA: its partial sums are stored
+  uint64_t* empty = full + S;    // 8 warps have read codes, 8 have scales and know that x has been read
+  uint64_t* a_full = empty + S;  // [2 blocks of the slab][slab & 1]
+  uint64_t* d_full = a_full + 4; // same: the products are done, A's buffer is free
+  uint64_t* d_empty = d_full + 4;
+  uint64_t* done = d_empty + 4;  // one arrival per CTA: its partial sums are stored
   uint64_t* tmem_done = done + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_done + 1);
 
@@ -189,15 +197,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 9);
+      mbar_init(&empty[i], 16);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(&a_full[i], 4);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&a_full[i], 4);
       mbar_init(&d_full[i], 1);
-      mbar_init(&d_empty[i], 4);
+      mbar_init(&d_empty[i], 8);
     }
     mbar_init(done, cs);
-    mbar_init(tmem_done, 8);
+    mbar_init(tmem_done, 9);
     fence_barrier_init();
   }
   if (warp == kMmaWarp) {
@@ -248,35 +256,35 @@ __global__ void __launch_bounds__(kThreads, 1)
     return;
   }
 
-  if (warp == kMmaWarp) {
+  if (warp >= kMmaWarp) {
     // ------------------------------ products ------------------------------
+    const int w = warp - kMmaWarp;  // of the slab's two blocks
     if (lane == 0) {
       constexpr uint32_t ID = idesc<T>(NTOK);
-      bool ok = true;
-      for (int i = 0; i < nsl && ok; ++i) {
-        const int st = i % S, nb = slab_blocks(rank + i * cs);
-        ok = mbar_wait(&full[st], (i / S) & 1, p.err, kDevErrFullWait);
-        for (int w = 0; w < nb && ok; ++w) {
-          // The group's block i: its A buffer is i & 1, used before for block i - 2. (Only the last slab
-          // can lack a block, so both groups count alike.)
-          ok = mbar_wait(&a_full[w * 2 + (i & 1)], (i >> 1) & 1, p.err, kDevErrMmaWait) &&
-               (i == 0 || mbar_wait(&d_empty[w], (i - 1) & 1, p.err, kDevErrMmaWait));
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t xb = smem_u32(smem + st * STAGE + XOFF) + w * (2 * NTOK * 128);
-          const uint32_t a = tmem + kACol + w * 128 + (i & 1) * 64, d = tmem + w * 128;
+      for (int i = 0; i < nsl; ++i) {
+        if (w >= slab_blocks(rank + i * cs)) break;  // (only the last slab can lack its second block)
+        const int st = i % S, ab = w * 2 + (i & 1), db = w * 2 + i % DB;
+        if (!mbar_wait(&full[st], (i / S) & 1, p.err, kDevErrFullWait) ||
+            (i >= DB && !mbar_wait(&d_empty[db], (i / DB - 1) & 1, p.err, kDevErrMmaWait)) ||
+            !mbar_wait(&a_full[ab], (i >> 1) & 1, p.err, kDevErrMmaWait))
+          break;
+        tc_fence_after();
+        const uint64_t xd = desc_k_sw128(smem_u32(smem + st * STAGE + XOFF) + w * (2 * NTOK * 128));
+        const uint32_t a = tmem + kACol + ab * 64, d = tmem + w * 128 + i % DB * 64;
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk) {
-            const int gi = kk * 16 / GROUP;
-            umma_ts(d + gi * NTOK, a + kk * 8, desc_k_sw128(xb + (kk >> 2) * (NTOK * 128) + (kk & 3) * 32), ID,
-                    kk * 16 % GROUP ? 1u : 0u);
-          }
-          umma_commit(&d_full[w]);
-        }
-        if (ok) umma_commit(&empty[st]);
+        for (int kk = 0; kk < 8; ++kk)
+          umma_ts(d + kk * 16 / GROUP * NTOK, a + kk * 8, xd + (((kk >> 2) * (NTOK * 128) + (kk & 3) * 32) >> 4), ID,
+                  kk * 16 % GROUP ? 1u : 0u);
+        umma_commit(&d_full[ab]);
       }
     }
     __syncwarp();
+    if (w == 1) {
+      if (lane == 0) mbar_arrive(tmem_done);
+      __syncwarp();
+      w4::cluster_wait();
+      return;
+    }
     mbar_wait(tmem_done, 0, p.err, kDevErrMmaWait);  // D has been read
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
@@ -284,42 +292,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     return;
   }
 
-  // ------------------------------ expand and add up ------------------------------
-  const int wg = warp >> 2, quarter = warp & 3;
-  const int r = 32 * quarter + lane;  // this thread's row of the tile, its TMEM lane
+  const int quarter = warp & 3, r = 32 * quarter + lane;  // this thread's row of the tile, its TMEM lane
   const uint32_t tlane = tmem + ((uint32_t)(32 * quarter) << 16);
-  const uint32_t d_addr = tlane + wg * 128, a_addr = tlane + kACol + wg * 128;
-  float acc[NTOK];
-#pragma unroll
-  for (int n = 0; n < NTOK; ++n) acc[n] = 0.f;
-  float scale[GPB];  // of the block whose D is awaited
-  bool ok = true;
-  // acc += scale * D of block i.
-  auto collect = [&](int i) {
-    if (!__all_sync(~0u, mbar_wait(&d_full[wg], i & 1, p.err, kDevErrMmaWait))) return false;
-    tc_fence_after();
-#pragma unroll
-    for (int gi = 0; gi < GPB; ++gi) {
-      uint32_t d[NTOK];
-#pragma unroll
-      for (int c = 0; c < NTOK / 32; ++c) tmem_ld32(d_addr + gi * NTOK + c * 32, d + c * 32);
-      tmem_ld_wait();
-#pragma unroll
-      for (int n = 0; n < NTOK; ++n) acc[n] = fmaf(scale[gi], __uint_as_float(d[n]), acc[n]);
-    }
-    tc_fence_before();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&d_empty[wg]);
-    return true;
-  };
-  int mine = 0;  // blocks this group has expanded
-  for (int i = 0; i < nsl; ++i) {
-    const int st = i % S, nb = slab_blocks(rank + i * cs);
-    ok = __all_sync(~0u, mbar_wait(&full[st], (i / S) & 1, p.err, kDevErrFullWait));
-    if (!ok) break;
-    float next[GPB];
-    if (wg < nb) {
-      const uint32_t ba = smem_u32(smem + st * STAGE) + ((r >> 4) * nb + wg) * BB + (r & 15) * 64;
+  if (warp < 8) {
+    // ------------------------------ expand ------------------------------
+    const int w = warp >> 2;  // of the slab's two blocks
+    for (int i = 0; i < nsl; ++i) {
+      const int st = i % S, nb = slab_blocks(rank + i * cs);
+      if (!__all_sync(~0u, mbar_wait(&full[st], (i / S) & 1, p.err, kDevErrFullWait))) break;
+      if (w >= nb) {
+        if (lane == 0) mbar_arrive(&empty[st]);
+        continue;
+      }
+      const uint32_t ba = smem_u32(smem + st * STAGE) + ((r >> 4) * nb + w) * BB + (r & 15) * 64;
       const uint32_t sa = ba - (r & 15) * 60 + 1024;
       uint32_t words[4][4];  // [c][j]: inputs 32 j + 8 c
 #pragma unroll
@@ -329,11 +314,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       Expand<T> ex[GPB];
 #pragma unroll
-      for (int gi = 0; gi < GPB; ++gi) {
-        const uint32_t sz = w4::lds32(sa + gi * 64);
-        next[gi] = w4::Half<T>::lo(sz);
-        ex[gi].zero(sz);
-      }
+      for (int gi = 0; gi < GPB; ++gi) ex[gi].zero(w4::lds32(sa + gi * 64));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
+      const int ab = w * 2 + (i & 1);
+      if (i >= 2 && !__all_sync(~0u, mbar_wait(&d_full[ab], ((i >> 1) - 1) & 1, p.err, kDevErrMmaWait))) break;
+      tc_fence_after();
 #pragma unroll
       for (int h = 0; h < 2; ++h) {  // 64 inputs: 32 columns
         uint32_t a[32];
@@ -341,23 +327,61 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int jj = 0; jj < 2; ++jj)
 #pragma unroll
           for (int c = 0; c < 4; ++c) ex[(2 * h + jj) * 32 / GROUP].word(words[c][2 * h + jj], a + jj * 16 + c * 4);
-        tmem_st32(a_addr + (i & 1) * 64 + h * 32, a);
+        tmem_st32(tlane + kACol + ab * 64 + h * 32, a);
       }
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&a_full[wg * 2 + (i & 1)]);
+      if (lane == 0) mbar_arrive(&a_full[ab]);
     }
-    if (lane == 0) mbar_arrive(&empty[st]);
-    if (i > 0) ok = collect(i - 1);
-    if (!ok) break;
-    if (wg < nb) {
-      mine = i + 1;
+    __syncwarp();
+    w4::cluster_wait();
+    return;
+  }
+
+  // ------------------------------ add up ------------------------------
+  constexpr int HT = NTOK / 2;  // tokens of this warp: warps 8-11 the first half
+  const int half = (warp >> 2) & 1;
+  float acc[HT];
 #pragma unroll
-      for (int gi = 0; gi < GPB; ++gi) scale[gi] = next[gi];
+  for (int n = 0; n < HT; ++n) acc[n] = 0.f;
+  bool ok = true;
+  for (int i = 0; i < nsl && ok; ++i) {
+    const int st = i % S, nb = slab_blocks(rank + i * cs);
+    ok = __all_sync(~0u, mbar_wait(&full[st], (i / S) & 1, p.err, kDevErrFullWait));
+    if (!ok) break;
+    const uint32_t sa = smem_u32(smem + st * STAGE) + (r >> 4) * nb * BB + (r & 15) * 4 + 1024;
+    float scale[kSlab][GPB];
+#pragma unroll
+    for (int w = 0; w < kSlab; ++w)
+#pragma unroll
+      for (int gi = 0; gi < GPB; ++gi) scale[w][gi] = w < nb ? w4::Half<T>::lo(w4::lds32(sa + w * BB + gi * 64)) : 0.f;
+#pragma unroll
+    for (int w = 0; w < kSlab; ++w) {
+      if (w >= nb || !ok) break;
+      const int db = w * 2 + i % DB;
+      ok = __all_sync(~0u, mbar_wait(&d_full[w * 2 + (i & 1)], (i >> 1) & 1, p.err, kDevErrMmaWait));
+      if (!ok) break;
+      tc_fence_after();
+      if (w == nb - 1 && lane == 0) mbar_arrive(&empty[st]);  // both blocks' products are done: x is free
+#pragma unroll
+      for (int gi = 0; gi < GPB; ++gi) {
+        uint32_t d[HT];
+        const uint32_t from = tlane + w * 128 + i % DB * 64 + gi * NTOK + half * HT;
+        if constexpr (HT == 32) {
+          tmem_ld32(from, d);
+        } else {
+          tmem_ld16(from, d);
+        }
+        tmem_ld_wait();
+#pragma unroll
+        for (int n = 0; n < HT; ++n) acc[n] = fmaf(scale[w][gi], __uint_as_float(d[n]), acc[n]);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&d_empty[db]);
     }
   }
-  if (ok && mine == nsl) ok = collect(nsl - 1);
   __syncwarp();
   if (lane == 0) mbar_arrive(tmem_done);
 
@@ -365,23 +389,24 @@ __global__ void __launch_bounds__(kThreads, 1)
   w4::cluster_wait();
   asm volatile("griddepcontrol.wait;" ::: "memory");
   {
+    const int tid = threadIdx.x - 256;
     const int rows_log = 7 - p.cs_log, owner = r >> rows_log, slot = r & ((1 << rows_log) - 1);
     const uint32_t to =
-        w4::map_to(smem_u32(part_buf + ((size_t)((rank * 2 + wg) << rows_log) + slot) * PR), owner);
+        w4::map_to(smem_u32(part_buf + ((size_t)(rank << rows_log) + slot) * PR + half * HT), owner);
 #pragma unroll
-    for (int n = 0; n < NTOK; n += 4) w4::st_cluster4(to + n * 4, acc[n], acc[n + 1], acc[n + 2], acc[n + 3]);
+    for (int n = 0; n < HT; n += 4) w4::st_cluster4(to + n * 4, acc[n], acc[n + 1], acc[n + 2], acc[n + 3]);
     named_bar_sync(1, 256);
-    if (warp == 0 && lane < cs) w4::arrive_cluster(w4::map_to(smem_u32(done), lane));
+    if (warp == 8 && lane < cs) w4::arrive_cluster(w4::map_to(smem_u32(done), lane));
     if (!w4::wait_cluster(done, 0, p.err)) return;
     const int rows = 1 << rows_log, plane = rows * PR;
     // Lanes along the rows: a token's outputs are contiguous.
-    for (int e = threadIdx.x; e < rows * (NTOK / 4); e += 256) {
+    for (int e = tid; e < rows * (NTOK / 4); e += 256) {
       const int row_in = e & (rows - 1), n = (e >> rows_log) * 4;
       const int row = tile * kRows + rank * rows + row_in;
       if (row >= p.N || tok0 + n >= p.M) continue;
       const float* from = part_buf + row_in * PR + n;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int q = 0; q < 2 * cs; ++q) {
+      for (int q = 0; q < cs; ++q) {
         const float4 f = *reinterpret_cast<const float4*>(from + q * plane);
         v.x += f.x, v.y += f.y, v.z += f.z, v.w += f.w;
       }
