@@ -86,7 +86,22 @@ __device__ __forceinline__ void st_cluster4(uint32_t addr, float a, float b, flo
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// Bounded wait for arrivals from the cluster, with acquire at its scope.
+// Bounded wait for a phase. The bound itself lies in global memory and is looked at only when a
+// wait has lasted some time: its latency would be paid after every wait that does not succeed at once.
+constexpr uint64_t kPatienceNs = 50000;
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* err, int code) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = global_timer_ns();
+  while (!mbar_try_wait(bar, parity)) {
+    const uint64_t t = global_timer_ns() - t0;
+    if (t > kPatienceNs && t > wait_limit_ns(err)) {
+      record_device_error(err, code);
+      return false;
+    }
+  }
+  return true;
+}
+// The same for arrivals from the cluster, with acquire at its scope.
 __device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, int* err) {
   const uint64_t t0 = global_timer_ns();
   while (true) {
@@ -99,7 +114,8 @@ __device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, int
         : "r"(smem_u32(bar)), "r"(parity)
         : "memory");
     if (ok) return true;
-    if (global_timer_ns() - t0 > wait_limit_ns(err)) break;
+    const uint64_t t = global_timer_ns() - t0;
+    if (t > kPatienceNs && t > wait_limit_ns(err)) break;
   }
   record_device_error(err, kDevErrFlagWait);
   return false;

@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, 1) w4_linear_kernel(const Pa
                 const int n = min(rows_stage, nr - rg - q * rows_stage);
                 if (n <= 0) break;
                 const uint32_t bytes = (uint32_t)(n * nb) * BB;
-                if (filled >= kStages) mbar_wait(&empty[stage], phase ^ 1, p.err, kDevErrEmptyWait);
+                if (filled >= kStages) w4::wait(&empty[stage], phase ^ 1, p.err, kDevErrEmptyWait);
                 mbar_arrive_expect_tx(&full[stage], bytes);
                 bulk_load(smem_u32(smem + stage * stage_bytes<GROUP>()), src + (size_t)(q * rows_stage * nb) * BB, bytes,
                           &full[stage], pol);
@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, 1) w4_linear_kernel(const Pa
     // No copy may be in flight when the CTA ends, also when a multiplying warp gave up waiting for one.
     if (lane == 0) {
       for (int f = max(0, filled - kStages); f < filled; ++f)
-        mbar_wait(&full[f % kStages], (f / kStages) & 1, p.err, kDevErrFullWait);
+        w4::wait(&full[f % kStages], (f / kStages) & 1, p.err, kDevErrFullWait);
     }
     return;
   }
@@ -336,7 +336,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, 1) w4_linear_kernel(const Pa
         for (int sl = c0; sl < c1; ++sl) {
           advance(stage, phase, groups);
           if (!mine) continue;
-          if (ok && !mbar_wait(&full[st], ph, p.err, kDevErrFullWait)) ok = false;
+          if (ok && !w4::wait(&full[st], ph, p.err, kDevErrFullWait)) ok = false;
           if (live) {
             const int nb = slab_blocks(rank + sl * cs);
             const int b0 = wk * (kSlab >> p.kw_log), b1 = min(nb, b0 + (kSlab >> p.kw_log));

@@ -13,9 +13,9 @@
 //   * warp 16 copies the rows' packed blocks (one bulk copy, contiguous) and x (TMA,
 //     128B-swizzled boxes of 64 inputs x N tokens) into a ring of stages;
 //   * warps 0-3 take the slab's first 128 inputs, warps 4-7 the others. Thread = row =
-//     TMEM lane: it expands its row's 16 words to the exact integers q - z (bf16: 128 + q
-//     from one rotation and one logic instruction per pair, minus 128 + z; fp16: 256 + q
-//     and 16 + q) and stores them to TMEM as the A operand (two buffers);
+//     TMEM lane: it expands its row's 16 words to the exact integers q - z (bf16: 32 + q
+//     from a rotation and a logic instruction per pair, minus 32 + z; fp16: 256 + q and
+//     16 + q) and stores them to TMEM as the A operand (two buffers);
 //   * warp 17 issues D = A x^T, one accumulator per group of g inputs, and commits;
 //   * warps 8-15 (thread = row and half of the tokens) read D and add s * D to their fp32
 //     sums. Integers and x are exact, so the only roundings are those of fp32 sums and
@@ -80,6 +80,17 @@ __device__ __forceinline__ void umma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                : "memory");
 }
+// One lane of the warp, in a form that the compiler knows to be a single one: the operands of the
+// products stay in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xFFFFFFFF;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
 // 32 consecutive TMEM columns of this thread's lane (no wait).
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
   asm volatile(
@@ -116,15 +127,15 @@ template <typename T>
 struct Expand;
 template <>
 struct Expand<__nv_bfloat16> {
-  __nv_bfloat162 c;  // 128 + z, twice
+  __nv_bfloat162 c;  // 32 + z, twice
   __device__ __forceinline__ void zero(uint32_t sz) {
     const float z = __uint_as_float(sz & 0xFFFF0000u);
-    c = __float2bfloat162_rn(128.f + z);
+    c = __float2bfloat162_rn(32.f + z);
   }
   __device__ __forceinline__ void word(uint32_t w, uint32_t* p) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t v = (__funnelshift_r(w, w, 4 * i + 2) & 0x000F000Fu) | 0x43004300u;
+      const uint32_t v = (__funnelshift_r(w, w, 4 * i) & 0x003C003Cu) | 0x42004200u;
       const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), c);
       p[i] = *reinterpret_cast<const uint32_t*>(&d);
     }
@@ -246,7 +257,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       asm volatile("griddepcontrol.wait;" ::: "memory");
       for (int i = 0; i < ahead; ++i) load_x(i);
       for (int i = ahead; i < nsl; ++i) {
-        if (!mbar_wait(&empty[i % S], ((i / S) & 1) ^ 1, p.err, kDevErrEmptyWait)) break;
+        if (!w4::wait(&empty[i % S], ((i / S) & 1) ^ 1, p.err, kDevErrEmptyWait)) break;
         load_w(i);
         load_x(i);
       }
@@ -259,24 +270,27 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp >= kMmaWarp) {
     // ------------------------------ products ------------------------------
     const int w = warp - kMmaWarp;  // of the slab's two blocks
-    if (lane == 0) {
-      constexpr uint32_t ID = idesc<T>(NTOK);
-      for (int i = 0; i < nsl; ++i) {
-        if (w >= slab_blocks(rank + i * cs)) break;  // (only the last slab can lack its second block)
-        const int st = i % S, ab = w * 2 + (i & 1), db = w * 2 + i % DB;
-        if (!mbar_wait(&full[st], (i / S) & 1, p.err, kDevErrFullWait) ||
-            (i >= DB && !mbar_wait(&d_empty[db], (i / DB - 1) & 1, p.err, kDevErrMmaWait)) ||
-            !mbar_wait(&a_full[ab], (i >> 1) & 1, p.err, kDevErrMmaWait))
-          break;
-        tc_fence_after();
-        const uint64_t xd = desc_k_sw128(smem_u32(smem + st * STAGE + XOFF) + w * (2 * NTOK * 128));
-        const uint32_t a = tmem + kACol + ab * 64, d = tmem + w * 128 + i % DB * 64;
+    constexpr uint32_t ID = idesc<T>(NTOK);
+    const bool leader = elect_one();
+    const uint64_t x0 = desc_k_sw128(smem_u32(smem) + XOFF + w * (2 * NTOK * 128));
+    for (int i = 0; i < nsl; ++i) {
+      if (w >= slab_blocks(rank + i * cs)) break;  // (only the last slab can lack its second block)
+      const int st = i % S, ab = w * 2 + (i & 1), db = w * 2 + i % DB;
+      if (!__all_sync(~0u, w4::wait(&full[st], (i / S) & 1, p.err, kDevErrFullWait) &&
+                               (i < DB || w4::wait(&d_empty[db], (i / DB - 1) & 1, p.err, kDevErrMmaWait)) &&
+                               w4::wait(&a_full[ab], (i >> 1) & 1, p.err, kDevErrMmaWait)))
+        break;
+      tc_fence_after();
+      const uint64_t xd = x0 + (st * STAGE >> 4);
+      const uint32_t a = tmem + kACol + ab * 64, d = tmem + w * 128 + i % DB * 64;
+      if (leader) {
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)
           umma_ts(d + kk * 16 / GROUP * NTOK, a + kk * 8, xd + (((kk >> 2) * (NTOK * 128) + (kk & 3) * 32) >> 4), ID,
                   kk * 16 % GROUP ? 1u : 0u);
         umma_commit(&d_full[ab]);
       }
+      __syncwarp();
     }
     __syncwarp();
     if (w == 1) {
@@ -285,7 +299,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       w4::cluster_wait();
       return;
     }
-    mbar_wait(tmem_done, 0, p.err, kDevErrMmaWait);  // D has been read
+    w4::wait(tmem_done, 0, p.err, kDevErrMmaWait);  // D has been read
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
     w4::cluster_wait();
@@ -299,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int w = warp >> 2;  // of the slab's two blocks
     for (int i = 0; i < nsl; ++i) {
       const int st = i % S, nb = slab_blocks(rank + i * cs);
-      if (!__all_sync(~0u, mbar_wait(&full[st], (i / S) & 1, p.err, kDevErrFullWait))) break;
+      if (!__all_sync(~0u, w4::wait(&full[st], (i / S) & 1, p.err, kDevErrFullWait))) break;
       if (w >= nb) {
         if (lane == 0) mbar_arrive(&empty[st]);
         continue;
@@ -318,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[st]);
       const int ab = w * 2 + (i & 1);
-      if (i >= 2 && !__all_sync(~0u, mbar_wait(&d_full[ab], ((i >> 1) - 1) & 1, p.err, kDevErrMmaWait))) break;
+      if (i >= 2 && !__all_sync(~0u, w4::wait(&d_full[ab], ((i >> 1) - 1) & 1, p.err, kDevErrMmaWait))) break;
       tc_fence_after();
 #pragma unroll
       for (int h = 0; h < 2; ++h) {  // 64 inputs: 32 columns
@@ -348,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   bool ok = true;
   for (int i = 0; i < nsl && ok; ++i) {
     const int st = i % S, nb = slab_blocks(rank + i * cs);
-    ok = __all_sync(~0u, mbar_wait(&full[st], (i / S) & 1, p.err, kDevErrFullWait));
+    ok = __all_sync(~0u, w4::wait(&full[st], (i / S) & 1, p.err, kDevErrFullWait));
     if (!ok) break;
     const uint32_t sa = smem_u32(smem + st * STAGE) + (r >> 4) * nb * BB + (r & 15) * 4 + 1024;
     float scale[kSlab][GPB];
@@ -360,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int w = 0; w < kSlab; ++w) {
       if (w >= nb || !ok) break;
       const int db = w * 2 + i % DB;
-      ok = __all_sync(~0u, mbar_wait(&d_full[w * 2 + (i & 1)], (i >> 1) & 1, p.err, kDevErrMmaWait));
+      ok = __all_sync(~0u, w4::wait(&d_full[w * 2 + (i & 1)], (i >> 1) & 1, p.err, kDevErrMmaWait));
       if (!ok) break;
       tc_fence_after();
       if (w == nb - 1 && lane == 0) mbar_arrive(&empty[st]);  // both blocks' products are done: x is free
