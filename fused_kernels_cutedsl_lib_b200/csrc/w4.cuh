@@ -89,10 +89,21 @@ __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
 // Bounded wait for a phase. The bound itself lies in global memory and is looked at only when a
 // wait has lasted some time: its latency would be paid after every wait that does not succeed at once.
 constexpr uint64_t kPatienceNs = 50000;
-__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* err, int code) {
-  if (mbar_try_wait(bar, parity)) return true;
+__device__ __forceinline__ bool try_wait_at(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool wait_at(uint32_t bar, uint32_t parity, int* err, int code) {
+  if (try_wait_at(bar, parity)) return true;
   const uint64_t t0 = global_timer_ns();
-  while (!mbar_try_wait(bar, parity)) {
+  while (!try_wait_at(bar, parity)) {
     const uint64_t t = global_timer_ns() - t0;
     if (t > kPatienceNs && t > wait_limit_ns(err)) {
       record_device_error(err, code);
@@ -100,6 +111,12 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* err, i
     }
   }
   return true;
+}
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* err, int code) {
+  return wait_at(smem_u32(bar), parity, err, code);
+}
+__device__ __forceinline__ void arrive_at(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 // The same for arrivals from the cluster, with acquire at its scope.
 __device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, int* err) {

@@ -273,24 +273,27 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr uint32_t ID = idesc<T>(NTOK);
     const bool leader = elect_one();
     const uint64_t x0 = desc_k_sw128(smem_u32(smem) + XOFF + w * (2 * NTOK * 128));
-    for (int i = 0; i < nsl; ++i) {
-      if (w >= slab_blocks(rank + i * cs)) break;  // (only the last slab can lack its second block)
-      const int st = i % S, ab = w * 2 + (i & 1), db = w * 2 + i % DB;
-      if (!__all_sync(~0u, w4::wait(&full[st], (i / S) & 1, p.err, kDevErrFullWait) &&
-                               (i < DB || w4::wait(&d_empty[db], (i / DB - 1) & 1, p.err, kDevErrMmaWait)) &&
-                               w4::wait(&a_full[ab], (i >> 1) & 1, p.err, kDevErrMmaWait)))
+    const uint32_t full0 = smem_u32(full), a_full0 = smem_u32(a_full) + w * 16, d_empty0 = smem_u32(d_empty) + w * 16;
+    const int blocks = nsl > 0 && w >= slab_blocks(rank + (nsl - 1) * cs) ? nsl - 1 : nsl;
+    uint32_t st = 0, ph = 0;
+    for (int i = 0; i < blocks; ++i) {
+      const int b = i & 1;
+      if (!__all_sync(~0u, w4::wait_at(full0 + st * 8, ph, p.err, kDevErrFullWait) &&
+                               (i < DB || w4::wait_at(d_empty0 + i % DB * 8, (i / DB - 1) & 1, p.err, kDevErrMmaWait)) &&
+                               w4::wait_at(a_full0 + b * 8, (i >> 1) & 1, p.err, kDevErrMmaWait)))
         break;
       tc_fence_after();
       const uint64_t xd = x0 + (st * STAGE >> 4);
-      const uint32_t a = tmem + kACol + ab * 64, d = tmem + w * 128 + i % DB * 64;
+      const uint32_t a = tmem + kACol + w * 128 + b * 64, d = tmem + w * 128 + i % DB * 64;
       if (leader) {
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)
           umma_ts(d + kk * 16 / GROUP * NTOK, a + kk * 8, xd + (((kk >> 2) * (NTOK * 128) + (kk & 3) * 32) >> 4), ID,
                   kk * 16 % GROUP ? 1u : 0u);
-        umma_commit(&d_full[ab]);
+        umma_commit(&d_full[w * 2 + b]);
       }
       __syncwarp();
+      if (++st == S) st = 0, ph ^= 1;
     }
     __syncwarp();
     if (w == 1) {
@@ -306,19 +309,26 @@ __global__ void __launch_bounds__(kThreads, 1)
     return;
   }
 
+  // In the loops below every instruction counts (a block's expansion is some 180): stage, parities and
+  // addresses are carried along, not derived from the slab's index.
   const int quarter = warp & 3, r = 32 * quarter + lane;  // this thread's row of the tile, its TMEM lane
   const uint32_t tlane = tmem + ((uint32_t)(32 * quarter) << 16);
+  const uint32_t smem0 = smem_u32(smem), full0 = smem_u32(full), empty0 = smem_u32(empty);
+  const bool short_tail = nsl > 0 && slab_blocks(rank + (nsl - 1) * cs) < kSlab;  // the last slab has one block
+  uint32_t st = 0, ph = 0;  // stage, its parity
   if (warp < 8) {
     // ------------------------------ expand ------------------------------
     const int w = warp >> 2;  // of the slab's two blocks
+    const uint32_t a_full0 = smem_u32(a_full) + w * 16, d_full0 = smem_u32(d_full) + w * 16;
+    const uint32_t a0 = tlane + kACol + w * 128;
     for (int i = 0; i < nsl; ++i) {
-      const int st = i % S, nb = slab_blocks(rank + i * cs);
-      if (!__all_sync(~0u, w4::wait(&full[st], (i / S) & 1, p.err, kDevErrFullWait))) break;
-      if (w >= nb) {
-        if (lane == 0) mbar_arrive(&empty[st]);
-        continue;
+      const bool tail = short_tail && i == nsl - 1;
+      if (!__all_sync(~0u, w4::wait_at(full0 + st * 8, ph, p.err, kDevErrFullWait))) break;
+      if (w == 1 && tail) {
+        if (lane == 0) w4::arrive_at(empty0 + st * 8);
+        break;
       }
-      const uint32_t ba = smem_u32(smem + st * STAGE) + ((r >> 4) * nb + w) * BB + (r & 15) * 64;
+      const uint32_t ba = smem0 + st * STAGE + (tail ? (r >> 4) * BB : ((r >> 4) * kSlab + w) * BB) + (r & 15) * 64;
       const uint32_t sa = ba - (r & 15) * 60 + 1024;
       uint32_t words[4][4];  // [c][j]: inputs 32 j + 8 c
 #pragma unroll
@@ -329,10 +339,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       Expand<T> ex[GPB];
 #pragma unroll
       for (int gi = 0; gi < GPB; ++gi) ex[gi].zero(w4::lds32(sa + gi * 64));
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[st]);
-      const int ab = w * 2 + (i & 1);
-      if (i >= 2 && !__all_sync(~0u, w4::wait(&d_full[ab], ((i >> 1) - 1) & 1, p.err, kDevErrMmaWait))) break;
+      const uint32_t b8 = (i & 1) * 8;
+      if (i >= 2 && !__all_sync(~0u, w4::wait_at(d_full0 + b8, ((i >> 1) & 1) ^ 1, p.err, kDevErrMmaWait))) break;
       tc_fence_after();
 #pragma unroll
       for (int h = 0; h < 2; ++h) {  // 64 inputs: 32 columns
@@ -341,12 +349,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int jj = 0; jj < 2; ++jj)
 #pragma unroll
           for (int c = 0; c < 4; ++c) ex[(2 * h + jj) * 32 / GROUP].word(words[c][2 * h + jj], a + jj * 16 + c * 4);
-        tmem_st32(tlane + kACol + ab * 64 + h * 32, a);
+        tmem_st32(a0 + b8 * 8 + h * 32, a);
       }
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&a_full[ab]);
+      if (lane == 0) {
+        w4::arrive_at(a_full0 + b8);
+        w4::arrive_at(empty0 + st * 8);
+      }
+      if (++st == S) st = 0, ph ^= 1;
     }
     __syncwarp();
     w4::cluster_wait();
@@ -356,45 +368,48 @@ __global__ void __launch_bounds__(kThreads, 1)
   // ------------------------------ add up ------------------------------
   constexpr int HT = NTOK / 2;  // tokens of this warp: warps 8-11 the first half
   const int half = (warp >> 2) & 1;
+  const uint32_t d_full0 = smem_u32(d_full), d_empty0 = smem_u32(d_empty);
   float acc[HT];
 #pragma unroll
   for (int n = 0; n < HT; ++n) acc[n] = 0.f;
   bool ok = true;
   for (int i = 0; i < nsl && ok; ++i) {
-    const int st = i % S, nb = slab_blocks(rank + i * cs);
-    ok = __all_sync(~0u, w4::wait(&full[st], (i / S) & 1, p.err, kDevErrFullWait));
+    const bool tail = short_tail && i == nsl - 1;
+    ok = __all_sync(~0u, w4::wait_at(full0 + st * 8, ph, p.err, kDevErrFullWait));
     if (!ok) break;
-    const uint32_t sa = smem_u32(smem + st * STAGE) + (r >> 4) * nb * BB + (r & 15) * 4 + 1024;
+    const uint32_t sa = smem0 + st * STAGE + (r >> 4) * (tail ? BB : kSlab * BB) + (r & 15) * 4 + 1024;
     float scale[kSlab][GPB];
 #pragma unroll
     for (int w = 0; w < kSlab; ++w)
 #pragma unroll
-      for (int gi = 0; gi < GPB; ++gi) scale[w][gi] = w < nb ? w4::Half<T>::lo(w4::lds32(sa + w * BB + gi * 64)) : 0.f;
+      for (int gi = 0; gi < GPB; ++gi) scale[w][gi] = w4::Half<T>::lo(w4::lds32(sa + w * BB + gi * 64));
+    const uint32_t b8 = (i & 1) * 8, db8 = DB == 2 ? b8 : 0;
 #pragma unroll
     for (int w = 0; w < kSlab; ++w) {
-      if (w >= nb || !ok) break;
-      const int db = w * 2 + i % DB;
-      ok = __all_sync(~0u, w4::wait(&d_full[w * 2 + (i & 1)], (i >> 1) & 1, p.err, kDevErrMmaWait));
-      if (!ok) break;
-      tc_fence_after();
-      if (w == nb - 1 && lane == 0) mbar_arrive(&empty[st]);  // both blocks' products are done: x is free
+      if (w == 0 || !tail) {
+        ok = __all_sync(~0u, w4::wait_at(d_full0 + w * 16 + b8, (i >> 1) & 1, p.err, kDevErrMmaWait));
+        if (!ok) break;
+        tc_fence_after();
+        if ((w == kSlab - 1 || tail) && lane == 0) w4::arrive_at(empty0 + st * 8);  // x has been read
 #pragma unroll
-      for (int gi = 0; gi < GPB; ++gi) {
-        uint32_t d[HT];
-        const uint32_t from = tlane + w * 128 + i % DB * 64 + gi * NTOK + half * HT;
-        if constexpr (HT == 32) {
-          tmem_ld32(from, d);
-        } else {
-          tmem_ld16(from, d);
+        for (int gi = 0; gi < GPB; ++gi) {
+          uint32_t d[HT];
+          const uint32_t from = tlane + w * 128 + db8 * 8 + gi * NTOK + half * HT;
+          if constexpr (HT == 32) {
+            tmem_ld32(from, d);
+          } else {
+            tmem_ld16(from, d);
+          }
+          tmem_ld_wait();
+#pragma unroll
+          for (int n = 0; n < HT; ++n) acc[n] = fmaf(scale[w][gi], __uint_as_float(d[n]), acc[n]);
         }
-        tmem_ld_wait();
-#pragma unroll
-        for (int n = 0; n < HT; ++n) acc[n] = fmaf(scale[w][gi], __uint_as_float(d[n]), acc[n]);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) w4::arrive_at(d_empty0 + w * 16 + db8);
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&d_empty[db]);
     }
+    if (++st == S) st = 0, ph ^= 1;
   }
   __syncwarp();
   if (lane == 0) mbar_arrive(tmem_done);
