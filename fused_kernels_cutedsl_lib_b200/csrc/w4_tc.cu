@@ -40,8 +40,8 @@ using w4::kSlab;
 
 constexpr int kRows = 128;     // output rows per CTA (UMMA M, TMEM lanes)
 constexpr int kRowBlocks = 8;  // of 16 rows
-constexpr int kThreads = 608;
-constexpr int kLoadWarp = 16, kMmaWarp = 17;  // 0-7 expand, 8-15 add up, 17 and 18 issue the products
+constexpr int kThreads = 576;
+constexpr int kLoadWarp = 16, kMmaWarp = 17;  // 0-7 expand, 8-15 add up
 constexpr int kSmem = 227 * 1024;
 constexpr uint32_t kACol = 256;  // TMEM: D of warp group w at 128 w, its A buffers at 256 + 128 w + 64 buf
 
@@ -122,6 +122,19 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// (a & b) | c in one instruction.
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+// A constant that stays in a register: a logic instruction has room for one immediate only, and the
+// compiler would load the other one before every use.
+__device__ __forceinline__ uint32_t in_register(uint32_t v) {
+  uint32_t d;
+  asm volatile("mov.b32 %0, %1;" : "=r"(d) : "r"(v));
+  return d;
+}
 // One row's word as the exact 16-bit integers q - z, four pairs of neighbouring inputs.
 template <typename T>
 struct Expand;
@@ -132,10 +145,13 @@ struct Expand<__nv_bfloat16> {
     const float z = __uint_as_float(sz & 0xFFFF0000u);
     c = __float2bfloat162_rn(32.f + z);
   }
-  __device__ __forceinline__ void word(uint32_t w, uint32_t* p) const {
+  struct Consts {
+    uint32_t mask = in_register(0x003C003Cu), one = in_register(0x42004200u);
+  };
+  __device__ __forceinline__ void word(uint32_t w, uint32_t* p, const Consts& k) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t v = (__funnelshift_r(w, w, 4 * i) & 0x003C003Cu) | 0x42004200u;
+      const uint32_t v = and_or(__funnelshift_r(w, w, 4 * i), k.mask, k.one);
       const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), c);
       p[i] = *reinterpret_cast<const uint32_t*>(&d);
     }
@@ -149,9 +165,14 @@ struct Expand<__half> {
     c256 = __float2half2_rn(256.f + z);
     c16 = __float2half2_rn(16.f + z);
   }
-  __device__ __forceinline__ void word(uint32_t w, uint32_t* p) const {
-    uint32_t v[4];
-    w4::expand(w, v);
+  struct Consts {
+    uint32_t mask0 = in_register(0x003C003Cu), one0 = in_register(0x5C005C00u);
+    uint32_t mask1 = in_register(0x03C003C0u), one1 = in_register(0x4C004C00u);
+  };
+  __device__ __forceinline__ void word(uint32_t w, uint32_t* p, const Consts& k) const {
+    const uint32_t t = __funnelshift_r(w, w, 8);
+    const uint32_t v[4] = {and_or(w, k.mask0, k.one0), and_or(w, k.mask1, k.one1), and_or(t, k.mask0, k.one0),
+                           and_or(t, k.mask1, k.one1)};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&v[i]), i & 1 ? c16 : c256);
@@ -192,10 +213,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   float* part_buf = reinterpret_cast<float*>(smem + S * STAGE);  // [cs][128 / cs][PR]
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + S * STAGE + part_bytes<NTOK>());
   uint64_t* empty = full + S;    // 8 warps have read codes, 8 have scales and know that x has been read
-  uint64_t* a_full = empty + S;  // [2 blocks of the slab][slab & 1]
-  uint64_t* d_full = a_full + 4; // same: the products are done, A's buffer is free
-  uint64_t* d_empty = d_full + 4;
-  uint64_t* done = d_empty + 4;  // one arrival per CTA: its partial sums are stored
+  uint64_t* a_full = empty + S;  // [slab & 1]
+  uint64_t* d_full = a_full + 2; // the products are done, A's buffer is free
+  uint64_t* d_empty = d_full + 2;
+  uint64_t* done = d_empty + 2;  // one arrival per CTA: its partial sums are stored
   uint64_t* tmem_done = done + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_done + 1);
 
@@ -210,13 +231,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 16);
     }
-    for (int i = 0; i < 4; ++i) {
-      mbar_init(&a_full[i], 4);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&a_full[i], 8);
       mbar_init(&d_full[i], 1);
       mbar_init(&d_empty[i], 8);
     }
     mbar_init(done, cs);
-    mbar_init(tmem_done, 9);
+    mbar_init(tmem_done, 8);
     fence_barrier_init();
   }
   if (warp == kMmaWarp) {
@@ -267,41 +288,37 @@ __global__ void __launch_bounds__(kThreads, 1)
     return;
   }
 
-  if (warp >= kMmaWarp) {
+  if (warp == kMmaWarp) {
     // ------------------------------ products ------------------------------
-    const int w = warp - kMmaWarp;  // of the slab's two blocks
     constexpr uint32_t ID = idesc<T>(NTOK);
     const bool leader = elect_one();
-    const uint64_t x0 = desc_k_sw128(smem_u32(smem) + XOFF + w * (2 * NTOK * 128));
-    const uint32_t full0 = smem_u32(full), a_full0 = smem_u32(a_full) + w * 16, d_empty0 = smem_u32(d_empty) + w * 16;
-    const int blocks = nsl > 0 && w >= slab_blocks(rank + (nsl - 1) * cs) ? nsl - 1 : nsl;
+    const uint64_t x0 = desc_k_sw128(smem_u32(smem) + XOFF);
+    const uint32_t full0 = smem_u32(full), a_full0 = smem_u32(a_full), d_empty0 = smem_u32(d_empty);
     uint32_t st = 0, ph = 0;
-    for (int i = 0; i < blocks; ++i) {
-      const int b = i & 1;
+    for (int i = 0; i < nsl; ++i) {
+      const int b = i & 1, nb = slab_blocks(rank + i * cs);
       if (!__all_sync(~0u, w4::wait_at(full0 + st * 8, ph, p.err, kDevErrFullWait) &&
                                (i < DB || w4::wait_at(d_empty0 + i % DB * 8, (i / DB - 1) & 1, p.err, kDevErrMmaWait)) &&
                                w4::wait_at(a_full0 + b * 8, (i >> 1) & 1, p.err, kDevErrMmaWait)))
         break;
       tc_fence_after();
       const uint64_t xd = x0 + (st * STAGE >> 4);
-      const uint32_t a = tmem + kACol + w * 128 + b * 64, d = tmem + w * 128 + i % DB * 64;
+      const uint32_t a = tmem + kACol + b * 64, d = tmem + i % DB * 64;
       if (leader) {
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          umma_ts(d + kk * 16 / GROUP * NTOK, a + kk * 8, xd + (((kk >> 2) * (NTOK * 128) + (kk & 3) * 32) >> 4), ID,
-                  kk * 16 % GROUP ? 1u : 0u);
-        umma_commit(&d_full[w * 2 + b]);
+        for (int w = 0; w < kSlab; ++w) {
+          if (w >= nb) break;
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk)
+            umma_ts(d + w * 128 + kk * 16 / GROUP * NTOK, a + w * 128 + kk * 8,
+                    xd + (((w * 2 + (kk >> 2)) * (NTOK * 128) + (kk & 3) * 32) >> 4), ID, kk * 16 % GROUP ? 1u : 0u);
+        }
+        umma_commit(&d_full[b]);
       }
       __syncwarp();
       if (++st == S) st = 0, ph ^= 1;
     }
     __syncwarp();
-    if (w == 1) {
-      if (lane == 0) mbar_arrive(tmem_done);
-      __syncwarp();
-      w4::cluster_wait();
-      return;
-    }
     w4::wait(tmem_done, 0, p.err, kDevErrMmaWait);  // D has been read
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
@@ -315,19 +332,26 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tlane = tmem + ((uint32_t)(32 * quarter) << 16);
   const uint32_t smem0 = smem_u32(smem), full0 = smem_u32(full), empty0 = smem_u32(empty);
   const bool short_tail = nsl > 0 && slab_blocks(rank + (nsl - 1) * cs) < kSlab;  // the last slab has one block
-  uint32_t st = 0, ph = 0;  // stage, its parity
+  uint32_t st = 0;  // stage
   if (warp < 8) {
     // ------------------------------ expand ------------------------------
     const int w = warp >> 2;  // of the slab's two blocks
-    const uint32_t a_full0 = smem_u32(a_full) + w * 16, d_full0 = smem_u32(d_full) + w * 16;
+    const uint32_t a_full0 = smem_u32(a_full), d_full0 = smem_u32(d_full);
     const uint32_t a0 = tlane + kACol + w * 128;
+    uint32_t ph = 0;  // parity of the stage
+    const typename Expand<T>::Consts consts;
     for (int i = 0; i < nsl; ++i) {
       const bool tail = short_tail && i == nsl - 1;
-      if (!__all_sync(~0u, w4::wait_at(full0 + st * 8, ph, p.err, kDevErrFullWait))) break;
+      const uint32_t b8 = (i & 1) * 8;
+      // The buffer's last products: their phase over, this warp's next arrival counts for slab i.
+      auto buffer_free = [&] {
+        return i < 2 || __all_sync(~0u, w4::wait_at(d_full0 + b8, ((i >> 1) & 1) ^ 1, p.err, kDevErrMmaWait));
+      };
       if (w == 1 && tail) {
-        if (lane == 0) w4::arrive_at(empty0 + st * 8);
+        if (buffer_free() && lane == 0) w4::arrive_at(a_full0 + b8);
         break;
       }
+      if (!__all_sync(~0u, w4::wait_at(full0 + st * 8, ph, p.err, kDevErrFullWait))) break;
       const uint32_t ba = smem0 + st * STAGE + (tail ? (r >> 4) * BB : ((r >> 4) * kSlab + w) * BB) + (r & 15) * 64;
       const uint32_t sa = ba - (r & 15) * 60 + 1024;
       uint32_t words[4][4];  // [c][j]: inputs 32 j + 8 c
@@ -339,8 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       Expand<T> ex[GPB];
 #pragma unroll
       for (int gi = 0; gi < GPB; ++gi) ex[gi].zero(w4::lds32(sa + gi * 64));
-      const uint32_t b8 = (i & 1) * 8;
-      if (i >= 2 && !__all_sync(~0u, w4::wait_at(d_full0 + b8, ((i >> 1) & 1) ^ 1, p.err, kDevErrMmaWait))) break;
+      if (!buffer_free()) break;
       tc_fence_after();
 #pragma unroll
       for (int h = 0; h < 2; ++h) {  // 64 inputs: 32 columns
@@ -348,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int jj = 0; jj < 2; ++jj)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) ex[(2 * h + jj) * 32 / GROUP].word(words[c][2 * h + jj], a + jj * 16 + c * 4);
+          for (int c = 0; c < 4; ++c) ex[(2 * h + jj) * 32 / GROUP].word(words[c][2 * h + jj], a + jj * 16 + c * 4, consts);
         tmem_st32(a0 + b8 * 8 + h * 32, a);
       }
       tmem_st_wait();
@@ -375,41 +398,36 @@ __global__ void __launch_bounds__(kThreads, 1)
   bool ok = true;
   for (int i = 0; i < nsl && ok; ++i) {
     const bool tail = short_tail && i == nsl - 1;
-    ok = __all_sync(~0u, w4::wait_at(full0 + st * 8, ph, p.err, kDevErrFullWait));
-    if (!ok) break;
-    const uint32_t sa = smem0 + st * STAGE + (r >> 4) * (tail ? BB : kSlab * BB) + (r & 15) * 4 + 1024;
-    float scale[kSlab][GPB];
-#pragma unroll
-    for (int w = 0; w < kSlab; ++w)
-#pragma unroll
-      for (int gi = 0; gi < GPB; ++gi) scale[w][gi] = w4::Half<T>::lo(w4::lds32(sa + w * BB + gi * 64));
     const uint32_t b8 = (i & 1) * 8, db8 = DB == 2 ? b8 : 0;
+    ok = __all_sync(~0u, w4::wait_at(d_full0 + b8, (i >> 1) & 1, p.err, kDevErrMmaWait));
+    if (!ok) break;
+    tc_fence_after();
+    const uint32_t sa = smem0 + st * STAGE + (r >> 4) * (tail ? BB : kSlab * BB) + (r & 15) * 4 + 1024;
 #pragma unroll
     for (int w = 0; w < kSlab; ++w) {
-      if (w == 0 || !tail) {
-        ok = __all_sync(~0u, w4::wait_at(d_full0 + w * 16 + b8, (i >> 1) & 1, p.err, kDevErrMmaWait));
-        if (!ok) break;
-        tc_fence_after();
-        if ((w == kSlab - 1 || tail) && lane == 0) w4::arrive_at(empty0 + st * 8);  // x has been read
+      if (w == 1 && tail) break;
 #pragma unroll
-        for (int gi = 0; gi < GPB; ++gi) {
-          uint32_t d[HT];
-          const uint32_t from = tlane + w * 128 + db8 * 8 + gi * NTOK + half * HT;
-          if constexpr (HT == 32) {
-            tmem_ld32(from, d);
-          } else {
-            tmem_ld16(from, d);
-          }
-          tmem_ld_wait();
-#pragma unroll
-          for (int n = 0; n < HT; ++n) acc[n] = fmaf(scale[w][gi], __uint_as_float(d[n]), acc[n]);
+      for (int gi = 0; gi < GPB; ++gi) {
+        const float scale = w4::Half<T>::lo(w4::lds32(sa + w * BB + gi * 64));
+        uint32_t d[HT];
+        const uint32_t from = tlane + w * 128 + db8 * 8 + gi * NTOK + half * HT;
+        if constexpr (HT == 32) {
+          tmem_ld32(from, d);
+        } else {
+          tmem_ld16(from, d);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) w4::arrive_at(d_empty0 + w * 16 + db8);
+        tmem_ld_wait();
+#pragma unroll
+        for (int n = 0; n < HT; ++n) acc[n] = fmaf(scale, __uint_as_float(d[n]), acc[n]);
       }
     }
-    if (++st == S) st = 0, ph ^= 1;
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) {
+      w4::arrive_at(d_empty0 + db8);
+      w4::arrive_at(empty0 + st * 8);  // the scales have been read, and x by the products
+    }
+    if (++st == S) st = 0;
   }
   __syncwarp();
   if (lane == 0) mbar_arrive(tmem_done);
