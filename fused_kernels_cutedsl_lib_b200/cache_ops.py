@@ -167,7 +167,7 @@ def cache_attention(q, k_cache, v_cache, cache_seqlens, out=None, lse=None, *, b
     [B, pages] pools [num_pages, page_size, Hkv, D]. ``mass`` fp32
     [B, Hkv, >= L]: for every token j < len,
     ``mass_out[b, h, j] = mass[b, h, j] + sum over h's q heads of the weight of j``;
-    ``mass_out`` defaults to ``mass``, and entries behind the lengths stay as they
+    ``mass_out`` defaults to ``mass`` (else: other memory), and entries behind the lengths stay as they
     are. An empty row gives 0 and lse -inf.
     """
     if isinstance(q, torch.Tensor) and q.dim() == 4 and q.shape[1] == 1:

@@ -700,6 +700,10 @@ extern "C" int fk_cache_attn_fwd(const void* q, long long q_batch_stride, const 
                "caches and workspace must be 16-byte aligned");
   FK_CHECK_ARG((mass_in == nullptr) == (mass_out == nullptr), "give both mass_in and mass_out, or neither");
   FK_CHECK_ARG(!mass_in || mass_capacity >= max_seqlen, "mass_capacity must be >= max_seqlen");
+  FK_CHECK_ARG(!mass_in || mass_in == mass_out ||
+                   !bytes_meet(mass_in, 4LL * batch * num_heads_kv * mass_capacity, mass_out,
+                               4LL * batch * num_heads_kv * mass_capacity),
+               "mass_out must be mass_in or other memory");
   if (block_table) {
     FK_CHECK_ARG(block_size >= 1 && num_blocks >= 1 && max_seqlen % block_size == 0,
                  "paged cache: max_seqlen must be max_blocks_per_seq * block_size, num_blocks >= 1");

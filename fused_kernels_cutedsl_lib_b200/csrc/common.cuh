@@ -84,6 +84,12 @@ __device__ __forceinline__ uint64_t wait_limit_ns(const int* err) {
   return v ? v : kWaitLimitNs;
 }
 
+// Whether the byte ranges [a, a + na) and [b, b + nb) meet.
+inline bool bytes_meet(const void* a, long long na, const void* b, long long nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + (uintptr_t)nb && y < x + (uintptr_t)na;
+}
+
 __device__ __forceinline__ uint64_t global_timer_ns() {
   uint64_t t;
   asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));

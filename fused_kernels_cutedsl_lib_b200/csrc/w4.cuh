@@ -27,13 +27,29 @@ struct Call {
 // The form for more than 16 tokens (w4_tc.cu).
 int linear_tc(const Call& c, cudaStream_t st);
 
+// (a & MASK) | c in one logic instruction. It has room for one immediate only: with both constants known the
+// compiler takes two, so c is kept in a register (`in_register`).
+template <uint32_t MASK>
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t c) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "n"(MASK), "r"(c));
+  return d;
+}
+__device__ __forceinline__ uint32_t in_register(uint32_t v) {
+  uint32_t d;
+  asm volatile("mov.b32 %0, %1;" : "=r"(d) : "r"(v));
+  return d;
+}
 // A word's eight nibbles as fp16 pairs of inputs (0,1) (2,3) (4,5) (6,7), offset by 256, 16, 256, 16.
-__device__ __forceinline__ void expand(uint32_t w, uint32_t (&p)[4]) {
+struct ExpandConsts {
+  uint32_t c256 = in_register(0x5C005C00u), c16 = in_register(0x4C004C00u);
+};
+__device__ __forceinline__ void expand(uint32_t w, uint32_t (&p)[4], const ExpandConsts& k) {
   const uint32_t t = __funnelshift_r(w, w, 8);
-  p[0] = (w & 0x003C003Cu) | 0x5C005C00u;
-  p[1] = (w & 0x03C003C0u) | 0x4C004C00u;
-  p[2] = (t & 0x003C003Cu) | 0x5C005C00u;
-  p[3] = (t & 0x03C003C0u) | 0x4C004C00u;
+  p[0] = and_or<0x003C003Cu>(w, k.c256);
+  p[1] = and_or<0x03C003C0u>(w, k.c16);
+  p[2] = and_or<0x003C003Cu>(t, k.c256);
+  p[3] = and_or<0x03C003C0u>(t, k.c16);
 }
 
 template <typename T>

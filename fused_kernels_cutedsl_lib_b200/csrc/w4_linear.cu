@@ -38,8 +38,8 @@
 // of eight warps take turns at row blocks, each warp one row block or one of KW parts
 // of its slab. A finished row block's partial sums are stored into the shared memory of
 // the CTA of the cluster that owns the rows; when every CTA has told it so (an mbarrier
-// with one arrival per CTA), an owner adds what it got in a fixed order: no workspace, no atomic, and results do not depend on
-// timing. The first weight copies are issued before the wait for the preceding kernel
+// with one arrival per CTA), an owner adds what it got in a fixed order: no workspace, no
+// atomic, and results do not depend on timing. The first weight copies are issued before the wait for the preceding kernel
 // (programmatic dependent launch).
 #include <cuda_fp16.h>
 
@@ -323,6 +323,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, 1) w4_linear_kernel(const Pa
         __syncwarp();
       }
 
+      const ExpandConsts consts;
       for (int rg = 0; rg < nr; rg += NG * rows_stage) {
         const int lr = rg + gid * rows_stage + wrow;                      // this warp's row block of the tile
         const int groups = min(NG, (nr - rg + rows_stage - 1) >> (3 - p.kw_log));  // warp groups with rows in this round
@@ -358,8 +359,8 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, 1) w4_linear_kernel(const Pa
                 for (int jj = 0; jj < WPG; ++jj) {
                   const int j = i * WPG + jj;
                   uint32_t pl[4], ph4[4];
-                  expand(wlo[j], pl);
-                  expand(whi[j], ph4);
+                  expand(wlo[j], pl, consts);
+                  expand(whi[j], ph4, consts);
                   const uint32_t a0[4] = {pl[0], ph4[0], pl[1], ph4[1]};
                   const uint32_t a1[4] = {pl[2], ph4[2], pl[3], ph4[3]};
 #pragma unroll
@@ -570,6 +571,12 @@ extern "C" int fk_w4_linear(const void* x, long long ldx, const void* packed, co
   FK_CHECK_ARG(((uintptr_t)x & 15) == 0 && ((uintptr_t)packed & 15) == 0,
                "x and packed must be 16-byte aligned");
   FK_CHECK_ARG(((uintptr_t)y & 1) == 0 && ((uintptr_t)residual & 1) == 0, "y and residual must be 2-byte aligned");
+  const long long y_bytes = 2LL * M * N, block = 1024 + 128 / group_size * 64;
+  FK_CHECK_ARG(!bytes_meet(y, y_bytes, x, 2 * ((M - 1) * ldx + K)) &&
+                   !bytes_meet(y, y_bytes, packed, (N + 15) / 16 * ((K + 127LL) / 128) * block),
+               "y must not overlap x or the weight");
+  FK_CHECK_ARG(!residual || residual == y || !bytes_meet(y, y_bytes, residual, y_bytes),
+               "residual must be y or other memory");
   int* err = device_error_word();
   if (!err) return fail(kErrCuda, "device error word unavailable");
   cudaStream_t st = static_cast<cudaStream_t>(stream);

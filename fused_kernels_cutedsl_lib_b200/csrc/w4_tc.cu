@@ -2,11 +2,15 @@
 //   y[m, n] = sum_k x[m, k] * (q[n, k] - z[n, k / g]) * s[n, k / g]  (+ residual[m, n])
 // (the layout of the weight and the form for up to 16 tokens are in w4_linear.cu).
 //
-// Bound: up to 64 tokens share one pass over the weight, so a weight is expanded once
-// and the products cost the tensor cores a fraction of the time that the expansion
-// costs the ALU. mma.sync, which the form for few tokens uses, pays 32 products and 16
-// shared-memory reads per KB of weight at 32 tokens: 61 us for 64 tokens on 4096 x 14336
-// against 16 us here.
+// Bound: up to 64 tokens share one pass over the weight. At 6.5 TB/s an SM gets 46 weights
+// a clock, and expanding them to 16 bits (below) keeps its ALU pipe, 64 lanes a clock,
+// busy for about as long; the products themselves are a small load for tcgen05. Measured on
+// 4096 outputs of 14336 inputs: 15.7 us for 32 tokens, 17.9 us for 64 (the form for few
+// tokens: 61 us for 64, since mma.sync pays 32 products and 16 shared-memory reads per KB
+// of weight at 32 tokens); 28672 of 4096: 33.4 and 38.9 us. In the steady state the issue
+// slots are 60 % used, the ALU pipe 40 %, DRAM a quarter. The 16-bit GEMM takes 27 us for up to 128
+// tokens on 4096 x 14336: with more than 64 tokens, two passes, this form has no advantage
+// but the weight's size.
 //
 // One CTA: 128 output rows, a slice of the inputs, N tokens (32 or 64). Per slab of 256
 // inputs
@@ -19,10 +23,13 @@
 //   * warp 17 issues D = A x^T, one accumulator per group of g inputs, and commits;
 //   * warps 8-15 (thread = row and half of the tokens) read D and add s * D to their fp32
 //     sums. Integers and x are exact, so the only roundings are those of fp32 sums and
-//     the output. (The expanding warps adding up themselves: XX us.)
+//     the output.
+// At 64 tokens on 4096 x 14336: 27.5 us with the expanding warps adding up, 20.4 with warps
+// of their own for it, 19.0 with addresses carried along, 17.9 with one logic
+// instruction per pair.
 // The inputs are split over the CS CTAs of a cluster; their sums go to the shared memory
-// of the CTA that owns the rows (mbarrier with one arrival per CTA), which
-// adds them in a fixed order: no workspace, no atomic.
+// of the CTA that owns the rows (mbarrier with one arrival per CTA), which adds them in a
+// fixed order: no workspace, no atomic.
 #include <cuda_fp16.h>
 
 #include <mutex>
@@ -122,19 +129,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// (a & b) | c in one instruction.
-__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t d;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-  return d;
-}
-// A constant that stays in a register: a logic instruction has room for one immediate only, and the
-// compiler would load the other one before every use.
-__device__ __forceinline__ uint32_t in_register(uint32_t v) {
-  uint32_t d;
-  asm volatile("mov.b32 %0, %1;" : "=r"(d) : "r"(v));
-  return d;
-}
 // One row's word as the exact 16-bit integers q - z, four pairs of neighbouring inputs.
 template <typename T>
 struct Expand;
@@ -146,12 +140,12 @@ struct Expand<__nv_bfloat16> {
     c = __float2bfloat162_rn(32.f + z);
   }
   struct Consts {
-    uint32_t mask = in_register(0x003C003Cu), one = in_register(0x42004200u);
+    uint32_t one = w4::in_register(0x42004200u);
   };
   __device__ __forceinline__ void word(uint32_t w, uint32_t* p, const Consts& k) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t v = and_or(__funnelshift_r(w, w, 4 * i), k.mask, k.one);
+      const uint32_t v = w4::and_or<0x003C003Cu>(__funnelshift_r(w, w, 4 * i), k.one);
       const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), c);
       p[i] = *reinterpret_cast<const uint32_t*>(&d);
     }
@@ -165,14 +159,10 @@ struct Expand<__half> {
     c256 = __float2half2_rn(256.f + z);
     c16 = __float2half2_rn(16.f + z);
   }
-  struct Consts {
-    uint32_t mask0 = in_register(0x003C003Cu), one0 = in_register(0x5C005C00u);
-    uint32_t mask1 = in_register(0x03C003C0u), one1 = in_register(0x4C004C00u);
-  };
+  using Consts = w4::ExpandConsts;
   __device__ __forceinline__ void word(uint32_t w, uint32_t* p, const Consts& k) const {
-    const uint32_t t = __funnelshift_r(w, w, 8);
-    const uint32_t v[4] = {and_or(w, k.mask0, k.one0), and_or(w, k.mask1, k.one1), and_or(t, k.mask0, k.one0),
-                           and_or(t, k.mask1, k.one1)};
+    uint32_t v[4];
+    w4::expand(w, v, k);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&v[i]), i & 1 ? c16 : c256);

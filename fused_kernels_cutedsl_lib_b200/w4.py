@@ -1,4 +1,4 @@
-"""Linear layer with 4-bit weights and group scales (host side of ``csrc/w4_linear.cu``).
+"""Linear layer with 4-bit weights and group scales (host side of ``csrc/w4_linear.cu``, ``csrc/w4_tc.cu``).
 
 ``y = x @ W.t() (+ residual)`` for the few tokens of a decode step, with
 ``W[n, k] = (q[n, k] - z[n, k // g]) * s[n, k // g]``, codes ``q`` and zero points
@@ -150,6 +150,7 @@ def w4_linear(x, weight: W4Weight, out=None, *, residual=None, stream=None):
     ``x`` [M, K] in the weight's dtype, any M (made for decode batches: up to 64
     tokens share one pass over the weight), rows may be strided (a multiple of 8
     elements); ``out`` and ``residual`` [M, N] dense, ``residual`` may be ``out``.
+    Otherwise ``out`` shares no memory with ``x``, ``residual`` or the weight.
     """
     if not isinstance(weight, W4Weight):
         raise TypeError(f"weight must be a W4Weight (pack_w4, quantize_w4), got {type(weight).__name__}")

@@ -463,3 +463,51 @@ def test_refusals():
                 dict(kept=torch.zeros(2, 2, 31, dtype=torch.int32, device="cuda"))):
         with pytest.raises(ValueError):
             ev(**bad)
+
+
+# Long rows of few heads: more stretches of a row than a warp has lanes, several times over.
+@pytest.mark.parametrize("B,L,Hkv,G,lens", [(1, 40000, 1, 4, [39999]), (2, 33000, 1, 16, [33000, 1]),
+                                            (1, 70000, 2, 1, [65537])])
+@pytest.mark.parametrize("D,dtype", [(64, FP16), (128, BF16)])
+def test_attention_long_rows(B, L, Hkv, G, lens, D, dtype):
+    q, k, v, lens, mass = make(B, L, Hkv, G, D, dtype, lens, seed=L)
+    got = run(q, k, v, lens, mass)
+    live = torch.arange(L + 3, device="cuda")[None, None] < lens[:, None, None]
+    ref.check_attention(got[0], got[1], torch.where(live, got[2], mass), mass, q, k, v, lens)
+    assert (got[2].masked_select(~live.expand_as(mass)) == -7.0).all()
+
+
+# More masses per lane than the other sizes have, and more than a lane's registers hold.
+@pytest.mark.parametrize("B,L,H,D,lens,budget", [(20, 20000, 8, 8, [20000 - 997 * i for i in range(20)], 3000),
+                                                 (1, 300000, 2, 16, [300000], 5000), (1, 270001, 1, 8, [262145], 262144)])
+def test_evict_long_rows(B, L, H, D, lens, budget):
+    _, k, v, lens, mass = make(B, L, H, 1, D, BF16, lens, seed=L)
+    mass *= torch.rand_like(mass) > 0.3
+    check_evict(k, v, lens, mass, budget, 4, 60)
+
+
+def test_mass_may_not_overlap_itself():
+    q, k, v, lens, _ = make(2, 64, 2, 4, 128, BF16, [64, 10], seed=21)
+    flat = torch.zeros(2 * 2 * 64 + 2 * 64, device="cuda")
+    mass, shifted = flat[:256].view(2, 2, 64), flat[128:384].view(2, 2, 64)
+    with pytest.raises(ValueError):
+        cache_attention(q, k, v, lens, mass=mass, mass_out=shifted)
+    cache_attention(q, k, v, lens, mass=mass, mass_out=flat[:256].view(2, 2, 64))  # the same memory: in place
+    assert (flat[256:] == 0).all()
+
+
+def test_evictions_on_two_streams_at_once():
+    sets = []
+    for seed in (31, 32):
+        _, k, v, lens, mass = make(6, 3000, 2, 1, 64, BF16, [3000, 0, 77, 1500, 513, 2999], seed=seed)
+        want, new = ref.evict(k, v, lens, mass, 512, 4, 32)
+        out = [torch.empty(6, 512, 2, 64, dtype=BF16, device="cuda") for _ in range(2)]
+        sets.append((k, v, lens, mass, out, torch.empty_like(lens), torch.empty(6, 2, 512, device="cuda"), want,
+                     torch.empty_like(want), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for k, v, lens, mass, out, new, m, want, kept, st in sets:
+            cache_evict(k, v, lens, mass, *out, new, m, 512, sinks=4, recent=32, kept=kept, stream=st)
+    torch.cuda.synchronize()
+    for k, v, lens, mass, out, new, m, want, kept, st in sets:
+        assert torch.equal(kept, want)

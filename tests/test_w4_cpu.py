@@ -74,3 +74,17 @@ def test_entry_point_refuses_before_launch():
                 dict(k=0), dict(group=16), dict(k=224)):
         assert call(**bad) == -1, bad
         assert lib.fk_last_error()
+
+
+def test_entry_point_refuses_overlaps():
+    lib = _native.load()
+
+    def call(x=1 << 20, packed=1 << 24, residual=None, y=1 << 28):  # addresses are compared, never read
+        return lib.fk_w4_linear(x, 512, packed, residual, y, 0, 3, 100, 256, 64, None)
+
+    y = 1 << 28
+    x_bytes, w_bytes, y_bytes = 2 * (2 * 512 + 256), 7 * 2 * (1024 + 128), 2 * 3 * 100
+    for bad in (dict(x=y), dict(x=y - x_bytes + 16), dict(x=y + y_bytes - 8), dict(packed=y - w_bytes + 16),
+                dict(packed=y + 592), dict(residual=y + 2), dict(residual=y - 2)):
+        assert call(**bad) == -1, bad
+        assert b"overlap" in lib.fk_last_error() or b"other memory" in lib.fk_last_error()

@@ -170,3 +170,65 @@ def test_refusals():
         w4_linear(x, w, residual=torch.empty(1, 32, dtype=BF16, device="cuda"))
     with pytest.raises(ValueError):  # 2-byte aligned rows
         w4_linear(torch.empty(2 * 256 + 1, dtype=BF16, device="cuda")[1:].view(2, 256), w)
+
+
+# Sizes that take the ways the shapes above do not: output rows in several rounds per cluster (with a
+# last slab of one block), inputs staged in several pieces, one row tile for a whole cluster, many
+# passes of tokens, one block of inputs.
+@pytest.mark.parametrize("m,n,k,group", [(16, 70000, 800, 32), (9, 70000, 896, 128), (16, 40, 20480, 64),
+                                         (10, 700, 20480, 32), (64, 16400, 512, 128), (130, 6200, 640, 64),
+                                         (70, 210, 512, 32), (50, 128, 14336, 128), (1000, 48, 256, 64),
+                                         (17, 1, 32, 32), (64, 20000, 1152, 32)])
+def test_splits_and_rounds(m, n, k, group):
+    q, s, z = weight(n, k, group, BF16, seed=n)
+    x = activations(m, k, BF16)
+    y = torch.full((m, n), float("nan"), dtype=BF16, device="cuda")
+    w4_linear(x, pack_w4(q, s, z), y)
+    check(y, x, q, s, z)
+    assert _native.device_error() == 0
+
+
+@pytest.mark.parametrize("m", [4, 40])
+def test_two_streams_at_once_and_strided_rows(m):
+    q, s, z = weight(1000, 2048, 64, BF16, seed=m)
+    w = pack_w4(q, s, z)
+    xs = [activations(m, 2048 + 1024, BF16, seed=i)[:, 512:2560] for i in range(2)]
+    want = [w4_linear(x, w) for x in xs]
+    for x, y in zip(xs, want):
+        check(y, x, q, s, z)
+    streams = [torch.cuda.Stream() for _ in xs]
+    outs = [torch.zeros(20, m, 1000, dtype=BF16, device="cuda") for _ in xs]
+    torch.cuda.synchronize()
+    for i in range(20):
+        for x, o, st in zip(xs, outs, streams):
+            w4_linear(x, w, o[i], stream=st)
+    torch.cuda.synchronize()
+    for o, y in zip(outs, want):
+        assert all(torch.equal(o[i], y) for i in range(20))
+
+
+def test_infinite_and_nan_activations_stay_in_their_rows():
+    for m in (3, 33):
+        q, s, z = weight(130, 512, 64, BF16)
+        w = pack_w4(q, s, z)
+        x = activations(m, 512, BF16)
+        clean = w4_linear(x, w)
+        x[1, 100], x[2, 7] = float("nan"), float("inf")
+        y = w4_linear(x, w)
+        rest = [i for i in range(m) if i not in (1, 2)]
+        assert torch.equal(y[rest], clean[rest])
+        assert y[1].isnan().all() and not y[2].isfinite().any()
+
+
+def test_overlaps_are_refused():
+    q, s, z = weight(256, 256, 64, BF16)
+    w = pack_w4(q, s, z)
+    for m in (2, 20):
+        buf = torch.zeros(4 * m, 256, dtype=BF16, device="cuda")
+        x = buf[:m]
+        for out in (x, buf[m - 1:2 * m - 1]):
+            with pytest.raises(ValueError):
+                w4_linear(x, w, out)
+        with pytest.raises(ValueError):
+            w4_linear(x, w, buf[m:2 * m], residual=buf[m + 1:2 * m + 1])
+        w4_linear(x, w, buf[m:2 * m], residual=buf[2 * m:3 * m])
