@@ -24,7 +24,7 @@ struct Call {
   bool bf16;
   int M, N, K, group;
 };
-// The form for more than 16 tokens (w4_tc.cu).
+// The form of w4_tc.cu.
 int linear_tc(const Call& c, cudaStream_t st);
 
 // (a & MASK) | c in one logic instruction. It has room for one immediate only: with both constants known the

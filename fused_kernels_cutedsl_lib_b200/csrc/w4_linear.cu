@@ -1,4 +1,5 @@
-// Linear layer with 4-bit weights and group scales for up to 16 tokens (more: w4_tc.cu):
+// Linear layer with 4-bit weights and group scales for up to 16 tokens (more, and some sizes
+// from 9 on: w4_tc.cu):
 //   y[m, n] = sum_k x[m, k] * (q[n, k] - z[n, k / g]) * s[n, k / g]  (+ residual[m, n])
 // with q, z in [0, 15], g in {32, 64, 128} and x, s, y bf16 or fp16.
 //
@@ -580,7 +581,12 @@ extern "C" int fk_w4_linear(const void* x, long long ldx, const void* packed, co
   int* err = device_error_word();
   if (!err) return fail(kErrCuda, "device error word unavailable");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (M > 16) {
+  // The form of w4_tc.cu for more than 16 tokens, and for more than 8 where four of its CTAs per 128 rows fit
+  // the SMs at once. At 9 and 16 tokens it took, against the form of this file: 4.4 / 4.9 us on 1024 x
+  // 2048, 7.3 / 8.3 on 4096 x 4096, 15.6 / 22.1 on 4096 x 14336; but 9.9 / 9.5 on 6144 x 4096, where two CTAs
+  // per 128 rows leave a third of the SMs idle, and 32.5 / 25.4 on 28672 x 4096, a wave and a half. At 8
+  // tokens: 15.5 / 14.2 on 4096 x 14336.
+  if (M > 16 || (M > 8 && 4 * ((N + 127) / 128) <= num_sms())) {
     const w4::Call c{x, ldx, static_cast<const uint8_t*>(packed), residual, y, err, dtype == FK_BF16, M, N, K, group_size};
     return w4::linear_tc(c, st);
   }

@@ -1,6 +1,6 @@
-// Linear layer with 4-bit weights and group scales for more than 16 tokens, on tcgen05:
+// Linear layer with 4-bit weights and group scales for more than 8 or 16 tokens, on tcgen05:
 //   y[m, n] = sum_k x[m, k] * (q[n, k] - z[n, k / g]) * s[n, k / g]  (+ residual[m, n])
-// (the layout of the weight and the form for up to 16 tokens are in w4_linear.cu).
+// (the layout of the weight, the form for fewer tokens and the choice are in w4_linear.cu).
 //
 // Bound: up to 64 tokens share one pass over the weight. At 6.5 TB/s an SM gets 46 weights
 // a clock, and expanding them to 16 bits (below) keeps its ALU pipe, 64 lanes a clock,
@@ -8,9 +8,9 @@
 // 4096 outputs of 14336 inputs: 15.7 us for 32 tokens, 17.9 us for 64 (the form for few
 // tokens: 61 us for 64, since mma.sync pays 32 products and 16 shared-memory reads per KB
 // of weight at 32 tokens); 28672 of 4096: 33.4 and 38.9 us. In the steady state the issue
-// slots are 60 % used, the ALU pipe 40 %, DRAM a quarter. The 16-bit GEMM takes 27 us for up to 128
-// tokens on 4096 x 14336: with more than 64 tokens, two passes, this form has no advantage
-// but the weight's size.
+// slots are 60 % used, the ALU pipe 40 %, DRAM a quarter. This package's 16-bit
+// linear (skinny_gemm) takes 24.8 and 26.9 us for 64 and 128 tokens on 4096 x 14336, where
+// this form takes 18.0 and, in two passes, 29.0: from 65 tokens on it saves memory, not time.
 //
 // One CTA: 128 output rows, a slice of the inputs, N tokens (32 or 64). Per slab of 256
 // inputs
