@@ -47,8 +47,8 @@ using w4::kSlab;
 
 constexpr int kRows = 128;     // output rows per CTA (UMMA M, TMEM lanes)
 constexpr int kRowBlocks = 8;  // of 16 rows
-constexpr int kThreads = 576;
-constexpr int kLoadWarp = 16, kMmaWarp = 17;  // 0-7 expand, 8-15 add up
+// Warps: 0-15 expand, 16-23 add up, 24 loads, 25 issues the products.
+constexpr int kAddWarp = 16, kLoadWarp = 24, kMmaWarp = 25, kThreads = 26 * 32;
 constexpr int kSmem = 227 * 1024;
 constexpr uint32_t kACol = 256;  // TMEM: D of warp group w at 128 w, its A buffers at 256 + 128 w + 64 buf
 
@@ -108,16 +108,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
       "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]),
       "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
       : "memory");
-}
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
 }
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
   asm volatile(
@@ -323,16 +313,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t smem0 = smem_u32(smem), full0 = smem_u32(full), empty0 = smem_u32(empty);
   const bool short_tail = nsl > 0 && slab_blocks(rank + (nsl - 1) * cs) < kSlab;  // the last slab has one block
   uint32_t st = 0;  // stage
-  if (warp < 8) {
+  if (warp < kAddWarp) {
     // ------------------------------ expand ------------------------------
-    const int w = warp >> 2;  // of the slab's two blocks
+    const int w = (warp >> 2) & 1;    // block of the slab
+    const int parity = warp >> 3;     // of this warp's slabs, and A's buffer
     const uint32_t a_full0 = smem_u32(a_full), d_full0 = smem_u32(d_full);
     const uint32_t a0 = tlane + kACol + w * 128;
-    uint32_t ph = 0;  // parity of the stage
+    const uint32_t b8 = parity * 8;
+    uint32_t ph = 0;  // parity of the stage's phase
+    st = parity % S;
     const typename Expand<T>::Consts consts;
-    for (int i = 0; i < nsl; ++i) {
+    for (int i = parity; i < nsl; i += 2) {
       const bool tail = short_tail && i == nsl - 1;
-      const uint32_t b8 = (i & 1) * 8;
       // The buffer's last products: their phase over, this warp's next arrival counts for slab i.
       auto buffer_free = [&] {
         return i < 2 || __all_sync(~0u, w4::wait_at(d_full0 + b8, ((i >> 1) & 1) ^ 1, p.err, kDevErrMmaWait));
@@ -371,7 +363,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         w4::arrive_at(a_full0 + b8);
         w4::arrive_at(empty0 + st * 8);
       }
-      if (++st == S) st = 0, ph ^= 1;
+      st += 2;
+      if (st >= S) st -= S, ph ^= 1;
     }
     __syncwarp();
     w4::cluster_wait();
@@ -379,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 
   // ------------------------------ add up ------------------------------
-  constexpr int HT = NTOK / 2;  // tokens of this warp: warps 8-11 the first half
+  constexpr int HT = NTOK / 2;  // tokens of this warp: the first four warps take the first half
   const int half = (warp >> 2) & 1;
   const uint32_t d_full0 = smem_u32(d_full), d_empty0 = smem_u32(d_empty);
   float acc[HT];
@@ -399,16 +392,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int gi = 0; gi < GPB; ++gi) {
         const float scale = w4::Half<T>::lo(w4::lds32(sa + w * BB + gi * 64));
-        uint32_t d[HT];
-        const uint32_t from = tlane + w * 128 + db8 * 8 + gi * NTOK + half * HT;
-        if constexpr (HT == 32) {
-          tmem_ld32(from, d);
-        } else {
-          tmem_ld16(from, d);
-        }
-        tmem_ld_wait();
 #pragma unroll
-        for (int n = 0; n < HT; ++n) acc[n] = fmaf(scale, __uint_as_float(d[n]), acc[n]);
+        for (int c = 0; c < HT; c += 16) {
+          uint32_t d[16];
+          tmem_ld16(tlane + w * 128 + db8 * 8 + gi * NTOK + half * HT + c, d);
+          tmem_ld_wait();
+#pragma unroll
+          for (int n = 0; n < 16; ++n) acc[c + n] = fmaf(scale, __uint_as_float(d[n]), acc[c + n]);
+        }
       }
     }
     tc_fence_before();
@@ -426,14 +417,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   w4::cluster_wait();
   asm volatile("griddepcontrol.wait;" ::: "memory");
   {
-    const int tid = threadIdx.x - 256;
+    const int tid = threadIdx.x - kAddWarp * 32;
     const int rows_log = 7 - p.cs_log, owner = r >> rows_log, slot = r & ((1 << rows_log) - 1);
     const uint32_t to =
         w4::map_to(smem_u32(part_buf + ((size_t)(rank << rows_log) + slot) * PR + half * HT), owner);
 #pragma unroll
     for (int n = 0; n < HT; n += 4) w4::st_cluster4(to + n * 4, acc[n], acc[n + 1], acc[n + 2], acc[n + 3]);
     named_bar_sync(1, 256);
-    if (warp == 8 && lane < cs) w4::arrive_cluster(w4::map_to(smem_u32(done), lane));
+    if (warp == kAddWarp && lane < cs) w4::arrive_cluster(w4::map_to(smem_u32(done), lane));
     if (!w4::wait_cluster(done, 0, p.err)) return;
     const int rows = 1 << rows_log, plane = rows * PR;
     // Lanes along the rows: a token's outputs are contiguous.
