@@ -162,38 +162,47 @@ struct Expand<__half> {
 };
 
 template <int GROUP>
-__host__ __device__ constexpr int weight_bytes() { return (kRowBlocks * kSlab * w4::block_bytes<GROUP>() + 1023) / 1024 * 1024; }
-template <int NTOK, int GROUP>
-__host__ __device__ constexpr int stage_bytes() { return weight_bytes<GROUP>() + kSlab * 2 * NTOK * 128; }
+__host__ __device__ constexpr int weight_bytes() { return kRowBlocks * kSlab * w4::block_bytes<GROUP>(); }
+template <int NTOK>
+__host__ __device__ constexpr int x_bytes() { return kSlab * 2 * NTOK * 128; }
 // Partial sums of the rows a CTA owns, from every CTA of the cluster; 4 floats of padding per row keep a warp's
 // 16-byte stores on distinct banks.
 template <int NTOK>
 __host__ __device__ constexpr int part_bytes() { return kRows * (NTOK + 4) * 4; }
+// Slabs of x (from L2) and of the weight (from memory, released later) in shared memory.
+template <int NTOK>
+__host__ __device__ constexpr int x_stages() { return NTOK > 32 ? 3 : 4; }
 template <int NTOK, int GROUP>
-__host__ __device__ constexpr int stages() {
-  constexpr int s = (kSmem - 2048 - part_bytes<NTOK>()) / stage_bytes<NTOK, GROUP>();
-  return s > 6 ? 6 : s;
+__host__ __device__ constexpr int w_stages() {
+  constexpr int s = (kSmem - 2048 - part_bytes<NTOK>() - x_stages<NTOK>() * x_bytes<NTOK>()) / weight_bytes<GROUP>();
+  return s > 8 ? 8 : s;
+}
+template <int NTOK, int GROUP>
+__host__ __device__ constexpr int ring_bytes() {
+  return x_stages<NTOK>() * x_bytes<NTOK>() + w_stages<NTOK, GROUP>() * weight_bytes<GROUP>();
 }
 
 template <typename T, int NTOK, int GROUP>
 __global__ void __launch_bounds__(kThreads, 1)
     w4_tc_kernel(const __grid_constant__ CUtensorMap tmX, const Params p) {
-  constexpr int S = stages<NTOK, GROUP>();
-  static_assert(S >= 2, "");
+  constexpr int S = w_stages<NTOK, GROUP>(), SX = x_stages<NTOK>();
+  static_assert(S >= 3, "a slab each for the two halves of the expanding warps, and one on its way");
   constexpr int GPB = kBlockK / GROUP;
   static_assert(GPB * NTOK <= 128, "the accumulators of a slab's first and second blocks have 128 columns each");
   constexpr int DB = GPB * NTOK <= 64 ? 2 : 1;  // accumulator buffers
   constexpr int BB = w4::block_bytes<GROUP>();
-  constexpr int STAGE = stage_bytes<NTOK, GROUP>();
-  constexpr int XOFF = weight_bytes<GROUP>();
+  constexpr int STAGE = weight_bytes<GROUP>(), XSTAGE = x_bytes<NTOK>();
   constexpr int PR = NTOK + 4;  // floats per row of partial sums
   extern __shared__ uint8_t smem_raw[];
   // Aligned by the shared-window address: the same in every CTA of the cluster.
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  float* part_buf = reinterpret_cast<float*>(smem + S * STAGE);  // [cs][128 / cs][PR]
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S * STAGE + part_bytes<NTOK>());
-  uint64_t* empty = full + S;    // 8 warps have read codes, 8 have scales and know that x has been read
-  uint64_t* a_full = empty + S;  // [slab & 1]
+  uint8_t* wring = smem + SX * XSTAGE;
+  float* part_buf = reinterpret_cast<float*>(smem + ring_bytes<NTOK, GROUP>());  // [cs][128 / cs][PR]
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + ring_bytes<NTOK, GROUP>() + part_bytes<NTOK>());  // of the weight
+  uint64_t* empty = full + S;      // 8 warps have read its codes, 8 its scales
+  uint64_t* x_full = empty + S;
+  uint64_t* x_empty = x_full + SX;
+  uint64_t* a_full = x_empty + SX;  // [slab & 1]
   uint64_t* d_full = a_full + 2; // the products are done, A's buffer is free
   uint64_t* d_empty = d_full + 2;
   uint64_t* done = d_empty + 2;  // one arrival per CTA: its partial sums are stored
@@ -210,6 +219,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < S; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 16);
+    }
+    for (int i = 0; i < SX; ++i) {
+      mbar_init(&x_full[i], 1);
+      mbar_init(&x_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&a_full[i], 8);
@@ -242,25 +255,29 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto load_w = [&](int i) {
         const int st = i % S, s = rank + i * cs, nb = slab_blocks(s);
         const uint32_t bytes = (uint32_t)(rows * nb) * BB;
-        mbar_arrive_expect_tx(&full[st], bytes + nb * 2 * NTOK * 128);
-        w4::bulk_load(smem_u32(smem + st * STAGE),
+        mbar_arrive_expect_tx(&full[st], bytes);
+        w4::bulk_load(smem_u32(wring + st * STAGE),
                       p.packed + ((size_t)s * kSlab * p.nrb + (size_t)tile * kRowBlocks * nb) * BB, bytes, &full[st], pol_w);
       };
       auto load_x = [&](int i) {
-        const int st = i % S, s = rank + i * cs, nb = slab_blocks(s);
+        const int st = i % SX, s = rank + i * cs, nb = slab_blocks(s);
+        mbar_arrive_expect_tx(&x_full[st], nb * 2 * NTOK * 128);
         for (int q = 0; q < nb * 2; ++q)
-          tma_load_2d(smem + st * STAGE + XOFF + q * (NTOK * 128), &tmX, &full[st], s * kSlab * kBlockK + q * 64, tok0,
-                      pol_x);
+          tma_load_2d(smem + st * XSTAGE + q * (NTOK * 128), &tmX, &x_full[st], s * kSlab * kBlockK + q * 64, tok0, pol_x);
       };
       // The weights' first copies do not wait for the preceding kernel, x does.
-      const int ahead = min(S, nsl);
-      for (int i = 0; i < ahead; ++i) load_w(i);
+      for (int i = 0; i < min(S, nsl); ++i) load_w(i);
       asm volatile("griddepcontrol.wait;" ::: "memory");
-      for (int i = 0; i < ahead; ++i) load_x(i);
-      for (int i = ahead; i < nsl; ++i) {
-        if (!w4::wait(&empty[i % S], ((i / S) & 1) ^ 1, p.err, kDevErrEmptyWait)) break;
-        load_w(i);
-        load_x(i);
+      for (int i = 0; i < min(SX, nsl); ++i) load_x(i);
+      for (int i = 0; i + min(S, SX) < nsl; ++i) {
+        if (i + SX < nsl) {
+          if (!w4::wait(&x_empty[i % SX], (i / SX) & 1, p.err, kDevErrEmptyWait)) break;
+          load_x(i + SX);
+        }
+        if (i + S < nsl) {
+          if (!w4::wait(&empty[i % S], (i / S) & 1, p.err, kDevErrEmptyWait)) break;
+          load_w(i + S);
+        }
       }
     }
     __syncwarp();
@@ -272,17 +289,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------ products ------------------------------
     constexpr uint32_t ID = idesc<T>(NTOK);
     const bool leader = elect_one();
-    const uint64_t x0 = desc_k_sw128(smem_u32(smem) + XOFF);
-    const uint32_t full0 = smem_u32(full), a_full0 = smem_u32(a_full), d_empty0 = smem_u32(d_empty);
+    const uint64_t x0 = desc_k_sw128(smem_u32(smem));
+    const uint32_t x_full0 = smem_u32(x_full), a_full0 = smem_u32(a_full), d_empty0 = smem_u32(d_empty);
     uint32_t st = 0, ph = 0;
     for (int i = 0; i < nsl; ++i) {
       const int b = i & 1, nb = slab_blocks(rank + i * cs);
-      if (!__all_sync(~0u, w4::wait_at(full0 + st * 8, ph, p.err, kDevErrFullWait) &&
+      if (!__all_sync(~0u, w4::wait_at(x_full0 + st * 8, ph, p.err, kDevErrFullWait) &&
                                (i < DB || w4::wait_at(d_empty0 + i % DB * 8, (i / DB - 1) & 1, p.err, kDevErrMmaWait)) &&
                                w4::wait_at(a_full0 + b * 8, (i >> 1) & 1, p.err, kDevErrMmaWait)))
         break;
       tc_fence_after();
-      const uint64_t xd = x0 + (st * STAGE >> 4);
+      const uint64_t xd = x0 + (st * XSTAGE >> 4);
       const uint32_t a = tmem + kACol + b * 64, d = tmem + i % DB * 64;
       if (leader) {
 #pragma unroll
@@ -294,9 +311,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     xd + (((w * 2 + (kk >> 2)) * (NTOK * 128) + (kk & 3) * 32) >> 4), ID, kk * 16 % GROUP ? 1u : 0u);
         }
         umma_commit(&d_full[b]);
+        umma_commit(&x_empty[st]);
       }
       __syncwarp();
-      if (++st == S) st = 0, ph ^= 1;
+      if (++st == SX) st = 0, ph ^= 1;
     }
     __syncwarp();
     w4::wait(tmem_done, 0, p.err, kDevErrMmaWait);  // D has been read
@@ -310,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // addresses are carried along, not derived from the slab's index.
   const int quarter = warp & 3, r = 32 * quarter + lane;  // this thread's row of the tile, its TMEM lane
   const uint32_t tlane = tmem + ((uint32_t)(32 * quarter) << 16);
-  const uint32_t smem0 = smem_u32(smem), full0 = smem_u32(full), empty0 = smem_u32(empty);
+  const uint32_t smem0 = smem_u32(wring), full0 = smem_u32(full), empty0 = smem_u32(empty);
   const bool short_tail = nsl > 0 && slab_blocks(rank + (nsl - 1) * cs) < kSlab;  // the last slab has one block
   uint32_t st = 0;  // stage
   if (warp < kAddWarp) {
@@ -406,7 +424,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
     if (lane == 0) {
       w4::arrive_at(d_empty0 + db8);
-      w4::arrive_at(empty0 + st * 8);  // the scales have been read, and x by the products
+      w4::arrive_at(empty0 + st * 8);  // the scales have been read
     }
     if (++st == S) st = 0;
   }
@@ -488,7 +506,7 @@ static int resident_clusters(int smem, int (&out)[4]) {
 
 template <typename T, int NTOK, int GROUP>
 static int launch(const w4::Call& c, cudaStream_t st) {
-  constexpr int smem = 1024 + stages<NTOK, GROUP>() * stage_bytes<NTOK, GROUP>() + part_bytes<NTOK>() + 512;
+  constexpr int smem = 1024 + ring_bytes<NTOK, GROUP>() + part_bytes<NTOK>() + 512;
   static_assert(smem <= kSmem, "shared memory budget");
   int resident[4];
   int rc = resident_clusters<T, NTOK, GROUP>(smem, resident);
