@@ -201,10 +201,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + ring_bytes<NTOK, GROUP>() + part_bytes<NTOK>());  // of the weight
   uint64_t* empty = full + S;      // 8 warps have read its codes, 8 its scales
   uint64_t* x_full = empty + S;
-  uint64_t* x_empty = x_full + SX;
+  uint64_t* x_empty = x_full + SX;  // the slab's products are done: x and A's buffer are free
   uint64_t* a_full = x_empty + SX;  // [slab & 1]
-  uint64_t* d_full = a_full + 2; // the products are done, A's buffer is free
-  uint64_t* d_empty = d_full + 2;
+  uint64_t* d_full = a_full + 2;    // [slab & 1], with one accumulator buffer: [block of the slab]
+  uint64_t* d_empty = d_full + 2;   // same
   uint64_t* done = d_empty + 2;  // one arrival per CTA: its partial sums are stored
   uint64_t* tmem_done = done + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_done + 1);
@@ -292,28 +292,34 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t x0 = desc_k_sw128(smem_u32(smem));
     const uint32_t x_full0 = smem_u32(x_full), a_full0 = smem_u32(a_full), d_empty0 = smem_u32(d_empty);
     uint32_t st = 0, ph = 0;
-    for (int i = 0; i < nsl; ++i) {
+    bool ok = true;
+    for (int i = 0; i < nsl && ok; ++i) {
       const int b = i & 1, nb = slab_blocks(rank + i * cs);
-      if (!__all_sync(~0u, w4::wait_at(x_full0 + st * 8, ph, p.err, kDevErrFullWait) &&
-                               (i < DB || w4::wait_at(d_empty0 + i % DB * 8, (i / DB - 1) & 1, p.err, kDevErrMmaWait)) &&
-                               w4::wait_at(a_full0 + b * 8, (i >> 1) & 1, p.err, kDevErrMmaWait)))
-        break;
-      tc_fence_after();
+      ok = w4::wait_at(x_full0 + st * 8, ph, p.err, kDevErrFullWait) &&
+           (DB == 1 || i < 2 || w4::wait_at(d_empty0 + b * 8, ((i >> 1) & 1) ^ 1, p.err, kDevErrMmaWait)) &&
+           w4::wait_at(a_full0 + b * 8, (i >> 1) & 1, p.err, kDevErrMmaWait);
       const uint64_t xd = x0 + (st * XSTAGE >> 4);
-      const uint32_t a = tmem + kACol + b * 64, d = tmem + i % DB * 64;
-      if (leader) {
+      const uint32_t a = tmem + kACol + b * 64, d = tmem + (DB == 2 ? b * 64 : 0);
 #pragma unroll
-        for (int w = 0; w < kSlab; ++w) {
-          if (w >= nb) break;
+      for (int w = 0; w < kSlab; ++w) {
+        if (w >= nb) break;
+        if (DB == 1 && i > 0) ok = ok && w4::wait_at(d_empty0 + w * 8, (i - 1) & 1, p.err, kDevErrMmaWait);
+        ok = __all_sync(~0u, ok);
+        if (!ok) break;
+        tc_fence_after();
+        if (leader) {
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)
             umma_ts(d + w * 128 + kk * 16 / GROUP * NTOK, a + w * 128 + kk * 8,
                     xd + (((w * 2 + (kk >> 2)) * (NTOK * 128) + (kk & 3) * 32) >> 4), ID, kk * 16 % GROUP ? 1u : 0u);
+          if (DB == 1) umma_commit(&d_full[w]);
+          if (w == nb - 1) {
+            if (DB == 2) umma_commit(&d_full[b]);
+            umma_commit(&x_empty[st]);
+          }
         }
-        umma_commit(&d_full[b]);
-        umma_commit(&x_empty[st]);
+        __syncwarp();
       }
-      __syncwarp();
       if (++st == SX) st = 0, ph ^= 1;
     }
     __syncwarp();
@@ -335,17 +341,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------ expand ------------------------------
     const int w = (warp >> 2) & 1;    // block of the slab
     const int parity = warp >> 3;     // of this warp's slabs, and A's buffer
-    const uint32_t a_full0 = smem_u32(a_full), d_full0 = smem_u32(d_full);
+    const uint32_t a_full0 = smem_u32(a_full), x_empty0 = smem_u32(x_empty);
     const uint32_t a0 = tlane + kACol + w * 128;
     const uint32_t b8 = parity * 8;
     uint32_t ph = 0;  // parity of the stage's phase
-    st = parity % S;
+    st = parity;
+    uint32_t xst = parity, xph = 0;  // x's stage of the slab two before, its phase
     const typename Expand<T>::Consts consts;
     for (int i = parity; i < nsl; i += 2) {
       const bool tail = short_tail && i == nsl - 1;
-      // The buffer's last products: their phase over, this warp's next arrival counts for slab i.
+      // The products of the buffer's last slab are done, and with them the phase of a_full that this warp's
+      // next arrival must not count for.
       auto buffer_free = [&] {
-        return i < 2 || __all_sync(~0u, w4::wait_at(d_full0 + b8, ((i >> 1) & 1) ^ 1, p.err, kDevErrMmaWait));
+        if (i < 2) return true;
+        const bool done = __all_sync(~0u, w4::wait_at(x_empty0 + xst * 8, xph, p.err, kDevErrMmaWait));
+        xst += 2;
+        if (xst >= SX) xst -= SX, xph ^= 1;
+        return done;
       };
       if (w == 1 && tail) {
         if (buffer_free() && lane == 0) w4::arrive_at(a_full0 + b8);
@@ -400,13 +412,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   for (int i = 0; i < nsl && ok; ++i) {
     const bool tail = short_tail && i == nsl - 1;
     const uint32_t b8 = (i & 1) * 8, db8 = DB == 2 ? b8 : 0;
-    ok = __all_sync(~0u, w4::wait_at(d_full0 + b8, (i >> 1) & 1, p.err, kDevErrMmaWait));
-    if (!ok) break;
-    tc_fence_after();
+    if (DB == 2) {
+      ok = __all_sync(~0u, w4::wait_at(d_full0 + b8, (i >> 1) & 1, p.err, kDevErrMmaWait));
+      if (!ok) break;
+      tc_fence_after();
+    }
     const uint32_t sa = smem0 + st * STAGE + (r >> 4) * (tail ? BB : kSlab * BB) + (r & 15) * 4 + 1024;
 #pragma unroll
     for (int w = 0; w < kSlab; ++w) {
       if (w == 1 && tail) break;
+      if (DB == 1) {
+        ok = __all_sync(~0u, w4::wait_at(d_full0 + w * 8, i & 1, p.err, kDevErrMmaWait));
+        if (!ok) break;
+        tc_fence_after();
+      }
 #pragma unroll
       for (int gi = 0; gi < GPB; ++gi) {
         const float scale = w4::Half<T>::lo(w4::lds32(sa + w * BB + gi * 64));
@@ -419,11 +438,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int n = 0; n < 16; ++n) acc[c + n] = fmaf(scale, __uint_as_float(d[n]), acc[c + n]);
         }
       }
+      if (DB == 1) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) w4::arrive_at(d_empty0 + w * 8);
+      }
     }
     tc_fence_before();
     __syncwarp();
     if (lane == 0) {
-      w4::arrive_at(d_empty0 + db8);
+      if (DB == 2) w4::arrive_at(d_empty0 + db8);
       w4::arrive_at(empty0 + st * 8);  // the scales have been read
     }
     if (++st == S) st = 0;
