@@ -581,12 +581,14 @@ extern "C" int fk_w4_linear(const void* x, long long ldx, const void* packed, co
   int* err = device_error_word();
   if (!err) return fail(kErrCuda, "device error word unavailable");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // The form of w4_tc.cu for more than 16 tokens, and for more than 8 where four of its CTAs per 128 rows fit
-  // the SMs at once. At 9 and 16 tokens it took, against the form of this file: 4.4 / 4.9 us on 1024 x
-  // 2048, 7.3 / 8.3 on 4096 x 4096, 15.6 / 22.1 on 4096 x 14336; but 9.9 / 9.5 on 6144 x 4096, where two CTAs
-  // per 128 rows leave a third of the SMs idle, and 32.5 / 25.4 on 28672 x 4096, a wave and a half. At 8
-  // tokens: 15.5 / 14.2 on 4096 x 14336.
-  if (M > 16 || (M > 8 && 4 * ((N + 127) / 128) <= num_sms())) {
+  // The form of w4_tc.cu for more than 16 tokens, and from 9 on unless its tiles of 128 rows are one to 1.6 to an
+  // SM: the second wave then leaves most SMs idle. For 16 tokens it took, against the form of this file (groups of
+  // 128): 4.1 / 5.1 us on 1024 x 2048, 7.0 / 8.3 on 4096 x 4096, 13.2 / 21.9 on 4096 x 14336, 14.6 / 19.4 on
+  // 18944 x 4096, 27.2 / 25.4 on 28672 x 4096 (1.5 tiles per SM), 29.1 / 31.6 on 37888 x 4096, 53.4 / 59.4 on 57344
+  // x 4096. For 8 tokens, where this form does half the products: 7.0 / 6.1 on 4096 x 4096, 13.2 / 14.1 on 4096 x
+  // 14336, 27.1 / 19.0 on 28672 x 4096.
+  const int tiles = (N + 127) / 128, sms = num_sms();
+  if (M > 16 || (M > 8 && (tiles <= sms || 5 * tiles > 8 * sms))) {
     const w4::Call c{x, ldx, static_cast<const uint8_t*>(packed), residual, y, err, dtype == FK_BF16, M, N, K, group_size};
     return w4::linear_tc(c, st);
   }

@@ -5,28 +5,31 @@
 // Bound: up to 64 tokens share one pass over the weight. At 6.5 TB/s an SM gets 46 weights
 // a clock, and expanding them to 16 bits (below) keeps its ALU pipe, 64 lanes a clock,
 // busy for about as long; the products themselves are a small load for tcgen05. Measured on
-// 4096 outputs of 14336 inputs: 15.7 us for 32 tokens, 17.9 us for 64 (the form for few
-// tokens: 61 us for 64, since mma.sync pays 32 products and 16 shared-memory reads per KB
-// of weight at 32 tokens); 28672 of 4096: 33.4 and 38.9 us. In the steady state the issue
-// slots are 60 % used, the ALU pipe 40 %, DRAM a quarter. This package's 16-bit
-// linear (skinny_gemm) takes 24.8 and 26.9 us for 64 and 128 tokens on 4096 x 14336, where
-// this form takes 18.0 and, in two passes, 29.0: from 65 tokens on it saves memory, not time.
+// 4096 outputs of 14336 inputs, groups of 128: 13.2 us for 16 or 32 tokens, 16.3 us for 64
+// (mma.sync, with 32 products and 16 shared-memory reads per KB of weight at 32 tokens:
+// 61 us for 64); 28672 of 4096: 28.1 and 34.9 us. This package's 16-bit linear
+// (skinny_gemm) takes 23.7, 24.8 and 26.9 us for 32, 64 and 128 tokens on 4096 x 14336: from
+// 65 tokens on, two passes, this form saves memory, not time.
 //
 // One CTA: 128 output rows, a slice of the inputs, N tokens (32 or 64). Per slab of 256
 // inputs
-//   * warp 16 copies the rows' packed blocks (one bulk copy, contiguous) and x (TMA,
-//     128B-swizzled boxes of 64 inputs x N tokens) into a ring of stages;
-//   * warps 0-3 take the slab's first 128 inputs, warps 4-7 the others. Thread = row =
+//   * warp 24 copies the rows' packed blocks (one bulk copy, contiguous) and x (TMA,
+//     128B-swizzled boxes of 64 inputs x N tokens) into two rings: x comes from L2 and is
+//     released by the products, the weight comes from memory and is held longer (one ring
+//     of three stages for both: 18.5 us at 64 tokens);
+//   * of warps 0-15, four take each block of 128 inputs of every second slab. Thread = row =
 //     TMEM lane: it expands its row's 16 words to the exact integers q - z (bf16: 32 + q
 //     from a rotation and a logic instruction per pair, minus 32 + z; fp16: 256 + q and
-//     16 + q) and stores them to TMEM as the A operand (two buffers);
-//   * warp 17 issues D = A x^T, one accumulator per group of g inputs, and commits;
-//   * warps 8-15 (thread = row and half of the tokens) read D and add s * D to their fp32
+//     16 + q) and stores them to TMEM as the A operand (two buffers). With eight warps, one
+//     slab at a time: 15.7 instead of 13.6 us at 32 tokens;
+//   * warp 25 issues D = A x^T, one accumulator per group of g inputs, and commits;
+//   * warps 16-23 (thread = row and half of the tokens) read D and add s * D to their fp32
 //     sums. Integers and x are exact, so the only roundings are those of fp32 sums and
 //     the output.
-// At 64 tokens on 4096 x 14336: 27.5 us with the expanding warps adding up, 20.4 with warps
-// of their own for it, 19.0 with addresses carried along, 17.9 with one logic
-// instruction per pair.
+// Earlier steps, 64 tokens on 4096 x 14336: 27.5 us with the expanding warps adding up too,
+// 20.4 with warps of their own for it, 19.0 with addresses carried along, 17.9 with one
+// logic instruction per pair. CTAs that go on to the next tile of rows instead of leaving:
+// 15.6 for 32 tokens instead of 13.3, no gain elsewhere.
 // The inputs are split over the CS CTAs of a cluster; their sums go to the shared memory
 // of the CTA that owns the rows (mbarrier with one arrival per CTA), which adds them in a
 // fixed order: no workspace, no atomic.

@@ -178,7 +178,8 @@ def test_refusals():
 @pytest.mark.parametrize("m,n,k,group", [(16, 70000, 800, 32), (9, 70000, 896, 128), (16, 40, 20480, 64),
                                          (10, 700, 20480, 32), (64, 16400, 512, 128), (130, 6200, 640, 64),
                                          (70, 210, 512, 32), (50, 128, 14336, 128), (1000, 48, 256, 64),
-                                         (17, 1, 32, 32), (64, 20000, 1152, 32)])
+                                         (17, 1, 32, 32), (64, 20000, 1152, 32), (40, 70000, 896, 32),
+                                         (200, 30000, 128, 128), (33, 25000, 640, 64)])
 def test_splits_and_rounds(m, n, k, group):
     q, s, z = weight(n, k, group, BF16, seed=n)
     x = activations(m, k, BF16)
