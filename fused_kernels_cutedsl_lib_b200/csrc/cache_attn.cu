@@ -193,8 +193,9 @@ __global__ void __launch_bounds__(kThreads, kCtas) attend_kernel(const Params p)
   const int G = p.G;
   const uint32_t ring = smem_u32(smem) + warp * S * stage_bytes<D>();
 
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  // After the wait: the second kernel reads lengths and masses, which kernels before this one wrote, before its own.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   TileIter ld, it;
   ld.init(p);
@@ -441,8 +442,9 @@ __device__ __forceinline__ float merge_lse(const float* src, size_t plane, int n
 template <typename E, int D>
 __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const Params p, int merge_blocks, int wpr_log,
                                                                 FastDiv stretches, FastDiv heads_q, FastDiv heads_kv) {
+  // What the first kernel wrote (partial results, scores) is read behind this wait only.
+  auto wait_first = [] { asm volatile("griddepcontrol.wait;" ::: "memory"); };
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   constexpr int kWarps = kFinishThreads / 32;
   __shared__ float s_acc[kWarps][D];
   __shared__ float s_lse[16];
@@ -459,6 +461,7 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const Params p, 
     for (int i = 0; i < PER; ++i) acc[i] = 0.f;
     if (in_range) {
       const int n = num_splits(p, seq_len(p, heads_q.div(row)));
+      wait_first();
       float ls[CH], v[CH][PER];
       // Splits part, part + wpr, ..: each warp's in order, then the warps' in order.
       auto load = [&](int s0) {
@@ -528,6 +531,7 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const Params p, 
     mass[u] = t < t1 ? p.mass_in[mrow + t] : 0.f;
     w[u] = 0.f;
   }
+  wait_first();
   float4 first[kMassUnroll];  // scores of the first four heads, or of the only one or two
 #pragma unroll
   for (int u = 0; u < kMassUnroll; ++u) {

@@ -68,7 +68,8 @@ def pack_w4(q: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = 
 
     ``q`` uint8 [N, K] holds one code (0..15) per element, ``scales`` [N, K // g]
     bf16 or fp16 with g in {32, 64, 128}, ``zeros`` uint8 of the same shape (0..15;
-    None: 8 everywhere). Works on any device; synchronises once to check the codes.
+    None: 8 everywhere). Works on any device, and waits for it: the result may be
+    used on any stream.
     """
     if not isinstance(q, torch.Tensor) or q.dtype != torch.uint8:
         raise TypeError("q must be a uint8 tensor")
@@ -111,6 +112,8 @@ def pack_w4(q: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = 
     full = kb // _SLAB
     packed = torch.cat([packed[:, :full * _SLAB].view(nb, full, _SLAB, words).transpose(0, 1).reshape(-1),
                         packed[:, full * _SLAB:].reshape(-1)])
+    if packed.is_cuda:  # the linear's first copies of a weight do not wait for the kernel before it on the stream
+        torch.cuda.current_stream(dev).synchronize()
     return W4Weight(packed, n, k, group, scales.dtype)
 
 
