@@ -28,6 +28,10 @@
 //
 // `gather_kernel` (a programmatic dependent): copies the kept rows, 16 bytes per
 // thread and cache, neighbouring threads along the heads of one output token.
+//
+// Measured, 8 kv heads of 128 dims: 32 ragged rows of up to 32768 tokens to 4096 213 us, 47 the
+// selection and 166 the copy, at a plain copy's rate (the copy in the selection's
+// kernel was slower: its CTAs are few). One row of 32768 to 2048 19.6 us: the passes' barriers.
 #include <cooperative_groups.h>
 
 #include "common.cuh"

@@ -5,7 +5,9 @@
 //
 // Bound: the 4-bit weights are read once (N*K/2 bytes). What it takes to keep up with
 // them is instructions: at 6.5 TB/s an SM gets 46 weights a clock, and its ALU pipe
-// issues 64 lanes a clock.
+// issues 64 lanes a clock. Measured with groups of 128, bf16: 4096 x 4096 5.8 us for one
+// token, of which some 4 are launch, cluster start and join; 28672 x 4096 18.6 us for one
+// token (3.4 TB/s) and 25.4 for 16.
 //
 // Arithmetic. The weights never become rounded 16-bit products q*s. Nibbles are or-ed
 // into the mantissa of fp16 256.0 (bit 2) or 16.0 (bit 6), which gives the exact numbers

@@ -233,3 +233,35 @@ def test_overlaps_are_refused():
         with pytest.raises(ValueError):
             w4_linear(x, w, buf[m:2 * m], residual=buf[m + 1:2 * m + 1])
         w4_linear(x, w, buf[m:2 * m], residual=buf[2 * m:3 * m])
+
+
+def test_captured_chain_of_layers():
+    """Two layers, the second on the first one's output, and a residual onto it, replayed on new inputs."""
+    for m in (12, 40, 100):
+        q1, s1, z1 = weight(512, 384, 64, BF16, seed=1)
+        q2, s2, z2 = weight(384, 512, 128, BF16, seed=2)
+        w1, w2 = pack_w4(q1, s1, z1), pack_w4(q2, s2, z2)
+        x = activations(m, 384, BF16)
+        h = torch.empty(m, 512, dtype=BF16, device="cuda")
+        y = torch.empty(m, 384, dtype=BF16, device="cuda")
+
+        def step():
+            w4_linear(x, w1, h)
+            w4_linear(h, w2, y, residual=x)
+            w4_linear(y, w1, h, residual=h)
+
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for _ in range(3):
+                step()
+        for seed in (7, 8):
+            x.copy_(activations(m, 384, BF16, seed=seed))
+            graph.replay()
+            first = w4_linear(x, w1)
+            check(first, x, q1, s1, z1)
+            mid = w4_linear(first, w2, residual=x)
+            check(mid, first, q2, s2, z2, x)
+            assert torch.equal(y, mid)
+            assert torch.equal(h, w4_linear(mid, w1, residual=first))
