@@ -168,13 +168,14 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, 1) w4_linear_kernel(const Pa
     const uint64_t pol = l2_policy_evict_first();
     int stage = 0, filled = 0;
     uint32_t phase = 0;
+    bool live = true;  // until a wait runs out: nothing more is loaded then
     for (int r0 = rb0; r0 < rb1; r0 += p.tile) {
       const int nr = min(p.tile, rb1 - r0);
       if (lane == 0) {
-        for (int c0 = 0; c0 < max_sl; c0 += p.chunk) {
+        for (int c0 = 0; c0 < max_sl && live; c0 += p.chunk) {
           const int c1 = min(c0 + p.chunk, nsl);
-          for (int rg = 0; rg < nr; rg += NG * rows_stage) {
-            for (int sl = c0; sl < c1; ++sl) {
+          for (int rg = 0; rg < nr && live; rg += NG * rows_stage) {
+            for (int sl = c0; sl < c1 && live; ++sl) {
               const int s = rank + sl * cs, nb = slab_blocks(s);
               const uint8_t* src = p.packed + ((size_t)s * kSlab * p.nrb + (size_t)(r0 + rg) * nb) * BB;
 #pragma unroll
@@ -182,7 +183,8 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, 1) w4_linear_kernel(const Pa
                 const int n = min(rows_stage, nr - rg - q * rows_stage);
                 if (n <= 0) break;
                 const uint32_t bytes = (uint32_t)(n * nb) * BB;
-                if (filled >= kStages) w4::wait(&empty[stage], phase ^ 1, p.err, kDevErrEmptyWait);
+                if (filled >= kStages) live = w4::wait(&empty[stage], phase ^ 1, p.err, kDevErrEmptyWait);
+                if (!live) break;
                 mbar_arrive_expect_tx(&full[stage], bytes);
                 bulk_load(smem_u32(smem + stage * stage_bytes<GROUP>()), src + (size_t)(q * rows_stage * nb) * BB, bytes,
                           &full[stage], pol);

@@ -372,9 +372,10 @@ FK_API int fk_skinny_gemm_noalloc(const void* x, const void* w, void* y, int M, 
  * W[n, k] = (q[n, k] - z[n, k / group]) * s[n, k / group], q and z in [0, 15],
  * group_size 32, 64 or 128 dividing K. x, s, residual and y are bf16 or fp16
  * (dtype); x rows are ldx elements apart (ldx >= K, a multiple of 8), y and
- * residual dense; residual may be null and may alias y. fp32 accumulation, one
- * rounding. Weights never become 16-bit products: integers are multiplied and the
- * scale is applied in fp32, so a non-finite x gives non-finite y.
+ * residual dense; residual may be null or y itself, otherwise y shares no memory
+ * with the inputs. fp32 accumulation, one rounding. Weights never become 16-bit
+ * products: integers are multiplied and the scale is applied in fp32, so a non-finite
+ * x gives non-finite y.
  *   packed  blocks of 16 rows x 128 inputs, 1024 + 8192 / group_size bytes each,
  *           16-byte aligned, ceil(N/16) x ceil(K/128) of them, ordered by slab of 2
  *           input blocks (the last may have one), row block, input block. As uint32 a
