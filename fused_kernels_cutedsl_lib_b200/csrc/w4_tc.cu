@@ -212,6 +212,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* tmem_done = done + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_done + 1);
 
+  using Half = w4::Half<T>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cs = 1 << p.cs_log, rank = blockIdx.x & (cs - 1), tile = blockIdx.x >> p.cs_log;
   const int tok0 = blockIdx.y * NTOK;
@@ -468,30 +469,48 @@ __global__ void __launch_bounds__(kThreads, 1)
         w4::map_to(smem_u32(part_buf + ((size_t)(rank << rows_log) + slot) * PR + half * HT), owner);
 #pragma unroll
     for (int n = 0; n < HT; n += 4) w4::st_cluster4(to + n * 4, acc[n], acc[n + 1], acc[n + 2], acc[n + 3]);
+    // Element e of this CTA's part of the output: four tokens of a row, lanes along the rows, so that a
+    // token's outputs are contiguous.
+    const int rows = 1 << rows_log, plane = rows * PR, elems = rows * (NTOK / 4);
+    auto locate = [&](int e, int& row, int& n) {
+      row = tile * kRows + rank * rows + (e & (rows - 1));
+      n = (e >> rows_log) * 4;
+      return e < elems && row < p.N && tok0 + n < p.M;
+    };
+    auto load_residual = [&](int e, T (&res)[4]) {
+      int row, n;
+      const bool in = locate(e, row, n) && p.residual;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (in && tok0 + n + i < p.M) res[i] = static_cast<const T*>(p.residual)[(size_t)(tok0 + n + i) * p.N + row];
+    };
+    // The first two elements' residuals arrive during the exchange.
+    T res[2][4] = {};
+    load_residual(tid, res[0]);
+    load_residual(tid + 256, res[1]);
     named_bar_sync(1, 256);
     if (warp == kAddWarp && lane < cs) w4::arrive_cluster(w4::map_to(smem_u32(done), lane));
     if (!w4::wait_cluster(done, 0, p.err)) return;
-    const int rows = 1 << rows_log, plane = rows * PR;
-    // Lanes along the rows: a token's outputs are contiguous.
-    for (int e = tid; e < rows * (NTOK / 4); e += 256) {
-      const int row_in = e & (rows - 1), n = (e >> rows_log) * 4;
-      const int row = tile * kRows + rank * rows + row_in;
-      if (row >= p.N || tok0 + n >= p.M) continue;
-      const float* from = part_buf + row_in * PR + n;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int q = 0; q < cs; ++q) {
-        const float4 f = *reinterpret_cast<const float4*>(from + q * plane);
-        v.x += f.x, v.y += f.y, v.z += f.z, v.w += f.w;
-      }
-      const float out[4] = {v.x, v.y, v.z, v.w};
+    for (int e0 = tid; e0 < elems; e0 += 512) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (tok0 + n + i >= p.M) break;
-        const size_t off = (size_t)(tok0 + n + i) * p.N + row;
-        float o = out[i];
-        if (p.residual) o += w4::Half<T>::to_float(static_cast<const T*>(p.residual)[off]);
-        static_cast<T*>(p.y)[off] = w4::Half<T>::round(o);
+      for (int u = 0; u < 2; ++u) {
+        int row, n;
+        if (!locate(e0 + u * 256, row, n)) continue;
+        const float* from = part_buf + (row & (rows - 1)) * PR + n;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int q = 0; q < cs; ++q) {
+          const float4 f = *reinterpret_cast<const float4*>(from + q * plane);
+          v.x += f.x, v.y += f.y, v.z += f.z, v.w += f.w;
+        }
+        const float out[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (tok0 + n + i < p.M)
+            static_cast<T*>(p.y)[(size_t)(tok0 + n + i) * p.N + row] =
+                Half::round(p.residual ? out[i] + Half::to_float(res[u][i]) : out[i]);
       }
+      load_residual(e0 + 512, res[0]);
+      load_residual(e0 + 768, res[1]);
     }
   }
 }
