@@ -5,9 +5,9 @@
 //
 // Bound: the 4-bit weights are read once (N*K/2 bytes). What it takes to keep up with
 // them is instructions: at 6.5 TB/s an SM gets 46 weights a clock, and its ALU pipe
-// issues 64 lanes a clock. Measured with groups of 128, bf16: 4096 x 4096 5.8 us for one
+// issues 64 lanes a clock. Measured with groups of 128, bf16: 4096 x 4096 5.7 us for one
 // token, of which some 4 are launch, cluster start and join; 28672 x 4096 18.6 us for one
-// token (3.4 TB/s) and 25.4 for 16.
+// token (3.4 TB/s) and 26.0 for 16.
 //
 // Arithmetic. The weights never become rounded 16-bit products q*s. Nibbles are or-ed
 // into the mantissa of fp16 256.0 (bit 2) or 16.0 (bit 6), which gives the exact numbers
@@ -429,23 +429,36 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, 1) w4_linear_kernel(const Pa
 
     // ---- every owner adds up its rows' partial sums, in order ----
     tell(done);
-    if (ok) ok = wait_cluster(done, tile_phase, p.err);
     {
       // Row block lr of the tile belongs to CTA lr mod cs; 16 lanes take its rows, for four tokens.
       const int n_own = (nr - rank + cs - 1) >> p.cs_log, parts = cs << p.kw_log;
       const int plane = own_max * 16 * TOK;
       const int r = lane & 15;
-      for (int i = warp * 2 + (lane >> 4); i < n_own * (TOK / 4); i += W * 2) {
-        const int slot = i / (TOK / 4), n = (i % (TOK / 4)) * 4;  // TOK is a power of two
+      auto locate = [&](int i, int& slot, int& n, size_t& off) {
+        slot = i / (TOK / 4), n = (i % (TOK / 4)) * 4;  // TOK is a power of two
         const int row = (r0 + (slot << p.cs_log) + rank) * 16 + r;
-        if (n >= ntok || row >= p.N) continue;
-        const size_t off = (size_t)n * p.N + row;
-        float res[4] = {0.f, 0.f, 0.f, 0.f};
-        if (p.residual) {
+        off = (size_t)n * p.N + row;
+        return i < n_own * (TOK / 4) && n < ntok && row < p.N;
+      };
+      auto load_residual = [&](int i, T (&res)[4]) {
+        int slot, n;
+        size_t off;
+        const bool in = locate(i, slot, n, off) && p.residual;
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (n + e < ntok) res[e] = H::to_float(static_cast<const T*>(p.residual)[off + (size_t)e * p.N]);
-        }
+        for (int e = 0; e < 4; ++e)
+          if (in && n + e < ntok) res[e] = static_cast<const T*>(p.residual)[off + (size_t)e * p.N];
+      };
+      const int i0 = warp * 2 + (lane >> 4);
+      T res[4] = {};
+      // Arrives during the wait. (Two tiles of tokens have no registers to spare for it: 26.3 instead of 26.0 us
+      // for 16 tokens on 28672 x 4096. One: 5.65 instead of 5.8 for one token on 4096 x 4096.)
+      if (NT == 1) load_residual(i0, res);
+      if (ok) ok = wait_cluster(done, tile_phase, p.err);
+      for (int i = i0; i < n_own * (TOK / 4); i += W * 2) {
+        int slot, n;
+        size_t off;
+        if (NT > 1 || i > i0) load_residual(i, res);
+        if (!locate(i, slot, n, off)) continue;
         const float* from = part_buf + (slot * 16 + r) * TOK + n;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
@@ -453,10 +466,12 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, 1) w4_linear_kernel(const Pa
           const float4 f = *reinterpret_cast<const float4*>(from + q * plane);
           v.x += f.x, v.y += f.y, v.z += f.z, v.w += f.w;
         }
-        const float out[4] = {v.x + res[0], v.y + res[1], v.z + res[2], v.w + res[3]};
+        const float out[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (n + e < ntok) static_cast<T*>(p.y)[off + (size_t)e * p.N] = H::round(out[e]);
+          if (n + e < ntok)
+            static_cast<T*>(p.y)[off + (size_t)e * p.N] =
+                H::round(p.residual ? out[e] + H::to_float(res[e]) : out[e]);
       }
     }
     if (r0 + p.tile < rb1) tell(taken);  // the next tile's partial sums overwrite these
@@ -588,7 +603,7 @@ extern "C" int fk_w4_linear(const void* x, long long ldx, const void* packed, co
   // The form of w4_tc.cu for more than 16 tokens, and from 9 on unless its tiles of 128 rows are one to 1.6 to an
   // SM: the second wave then leaves most SMs idle. For 16 tokens it took, against the form of this file (groups of
   // 128): 4.1 / 5.1 us on 1024 x 2048, 7.0 / 8.3 on 4096 x 4096, 13.2 / 21.9 on 4096 x 14336, 14.6 / 19.4 on
-  // 18944 x 4096, 27.2 / 25.4 on 28672 x 4096 (1.5 tiles per SM), 29.1 / 31.6 on 37888 x 4096, 53.4 / 59.4 on 57344
+  // 18944 x 4096, 27.2 / 26.0 on 28672 x 4096 (1.5 tiles per SM), 29.1 / 31.6 on 37888 x 4096, 53.4 / 59.4 on 57344
   // x 4096. For 8 tokens, where this form does half the products: 7.0 / 6.1 on 4096 x 4096, 13.2 / 14.1 on 4096 x
   // 14336, 27.1 / 19.0 on 28672 x 4096.
   const int tiles = (N + 127) / 128, sms = num_sms();
