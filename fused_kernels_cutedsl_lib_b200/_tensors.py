@@ -109,7 +109,8 @@ def one_device(*ts) -> int:
     return idx
 
 
-current_device = torch.cuda.current_device
+# Without torch's test for initialisation: the callers hold a CUDA tensor.
+current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 class on_device:
