@@ -1,0 +1,44 @@
+"""Corners of cache attention: non-finite keys and values, weights far apart (GPU)."""
+import pytest
+import torch
+
+import cache_reference as ref
+from fused_kernels_cutedsl_lib_b200 import cache_attention
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP16 = torch.bfloat16, torch.float16
+NAN, INF = float("nan"), float("inf")
+
+
+def make(B, L, Hkv, G, D, dtype, lens, seed=0):
+    """q, caches with NaN behind every length, lengths and masses."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    q = (1.5 * torch.randn(B, Hkv * G, D, generator=g, device="cuda")).to(dtype)
+    k = torch.randn(B, L, Hkv, D, generator=g, device="cuda").to(dtype)
+    v = torch.randn(B, L, Hkv, D, generator=g, device="cuda").to(dtype)
+    lens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    dead = torch.arange(L, device="cuda")[None, :] >= lens[:, None]
+    k[dead] = NAN
+    v[dead] = NAN
+    return q, k, v, lens, torch.rand(B, Hkv, L, generator=g, device="cuda")
+
+
+@pytest.mark.parametrize("G", [1, 2, 3, 5, 7, 8, 9, 13, 15, 16])
+@pytest.mark.parametrize("D,dtype", [(64, FP16), (128, BF16)])
+def test_keys_of_minus_infinity_leave_their_masses(G, D, dtype):
+    """A key of -inf has weight exactly 0 for every number of heads per kv head, odd ones among them."""
+    B, L, Hkv = 2, 300, 2
+    q, k, v, lens, mass = make(B, L, Hkv, G, D, dtype, [300, 140], seed=G)
+    q = q.abs() + 0.1
+    gone = torch.zeros(L, dtype=torch.bool, device="cuda")
+    gone[50:60] = True
+    gone[129] = True
+    k[:, gone] = -INF
+    before = mass.clone()
+    out, lse = cache_attention(q, k, v, lens, mass=mass)
+    assert torch.isfinite(out).all() and torch.isfinite(lse).all() and torch.isfinite(mass).all()
+    assert torch.equal(mass[:, :, gone], before[:, :, gone])
+    keep = (~gone).nonzero().flatten()
+    fewer = torch.tensor([289, 129], dtype=torch.int32, device="cuda")
+    ref.check_attention(out, lse, mass[..., keep], before[..., keep], q, k[:, keep], v[:, keep], fewer)
