@@ -305,10 +305,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) attend_kernel(const Params p)
           float* dst = p.scores + (((size_t)b * p.Hkv + h) * p.Lmax + (t + g)) * p.gs + h0;
           if (p.gs > 1) {  // gs is even: a pair of heads per store
             if (h0 < p.gs) {
-              // An odd group's last pair has a head of padding. Its q is 0, but 0 times an infinite key is NaN.
-              const bool both = h0 + 1 < G;
-              if (g < nv) *reinterpret_cast<float2*>(dst) = make_float2(x0, both ? x1 : 0.f);
-              if (g + 8 < nv) *reinterpret_cast<float2*>(dst + 8 * (size_t)p.gs) = make_float2(x2, both ? x3 : 0.f);
+              if (g < nv) *reinterpret_cast<float2*>(dst) = make_float2(x0, x1);
+              if (g + 8 < nv) *reinterpret_cast<float2*>(dst + 8 * (size_t)p.gs) = make_float2(x2, x3);
             }
           } else if (h0 == 0) {
             if (g < nv) dst[0] = x0;
@@ -558,9 +556,12 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const Params p, 
 #pragma unroll
     for (int u = 0; u < kMassUnroll; ++u) {
       const int t = t0 + u * kFinishThreads + (int)threadIdx.x;
-      const float4 x = h0 == 0 ? first[u]
-                       : t < t1 ? load_scores(sc + (size_t)t * p.gs, h0, p.gs) : make_float4(0.f, 0.f, 0.f, 0.f);
-      // Heads past the group hold 0, and z = +inf there.
+      float4 x = h0 == 0 ? first[u]
+                 : t < t1 ? load_scores(sc + (size_t)t * p.gs, h0, p.gs) : make_float4(0.f, 0.f, 0.f, 0.f);
+      // Heads past the group: 0, and z = +inf. An odd group's scores have one head of padding, at an odd place.
+      // Its q is 0, but 0 times an infinite key is NaN.
+      if (h0 + 1 >= p.G) x.y = 0.f;
+      if (h0 + 3 >= p.G) x.w = 0.f;
       w[u] += (exp2f(x.x - z[0]) + exp2f(x.y - z[1])) + (exp2f(x.z - z[2]) + exp2f(x.w - z[3]));
     }
   }
