@@ -440,12 +440,50 @@ __device__ __forceinline__ float merge_lse(const float* src, size_t plane, int n
   return W == 0.f ? -INFINITY : top + log2f(W);
 }
 
+// One (row, q head)'s output once more, with each weight as one fp32 number. Two 16-bit parts of a weight
+// (`attend_kernel`) are right for every finite v, but not for an infinite one: a second part of 0 or below
+// makes NaN of it. Only an output that is NaN although its lse is not comes here; one token at a time.
+// A warp, D / 32 dims per lane; lse in the log2 domain.
+template <typename E, int D>
+__device__ __noinline__ float4 attend_again(const Params& p, int row, int b, int len, float lse) {
+  constexpr int PER = D / 32;
+  const int lane = threadIdx.x & 31, head = row - b * p.Hq, h = head / p.G;
+  const float z = lse == -INFINITY ? 0.f : lse;
+  auto load = [](const void* base, size_t off, float (&f)[PER]) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(static_cast<const E*>(base) + off);
+#pragma unroll
+    for (int i = 0; i < PER / 2; ++i) f[2 * i] = Elem<E>::lo(w[i]), f[2 * i + 1] = Elem<E>::hi(w[i]);
+  };
+  float qv[PER], acc[4] = {};
+  load(p.q, (size_t)b * p.q_stride + (size_t)head * D + PER * lane, qv);
+  for (int t = 0; t < len; ++t) {
+    long long at = (long long)b * p.Lmax + t;
+    if (p.block_table) {
+      const int pg = p.page.div(t), page = p.block_table[(size_t)b * p.max_blocks + pg];
+      if (page < 0 || page >= p.num_blocks) continue;  // zero rows
+      at = (long long)page * p.block_size + (t - pg * p.block_size);
+    }
+    const size_t off = ((size_t)at * p.Hkv + h) * D + PER * lane;
+    float kv[PER], vv[PER], s = 0.f;
+    load(p.k, off, kv);
+    load(p.v, off, vv);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) s += qv[i] * kv[i];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    const float w = exp2f(s * p.scale_log2 - z);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) acc[i] += w * vv[i];
+  }
+  return make_float4(acc[0], acc[1], acc[2], acc[3]);
+}
+
 // Blocks [0, merge_blocks) merge splits: 8 >> wpr_log (row, q head) pairs each, with
 // 1 << wpr_log warps per pair. The others: one stretch of kMassTokens tokens of one (row,
 // kv head). Both read what pass 1 left, mostly in L2, and are short: what matters is that
 // a thread's loads are issued before the first is used.
 template <typename E, int D>
-__global__ void __launch_bounds__(kFinishThreads) finish_kernel(const Params p, int merge_blocks, int wpr_log,
+__global__ void __launch_bounds__(kFinishThreads) finish_kernel(const __grid_constant__ Params p, int merge_blocks, int wpr_log,
                                                                 FastDiv stretches, FastDiv heads_q, FastDiv heads_kv) {
   // What the first kernel wrote (partial results, scores) is read behind this wait only.
   auto wait_first = [] { asm volatile("griddepcontrol.wait;" ::: "memory"); };
@@ -462,10 +500,12 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const Params p, 
     constexpr int PER = D / 32;  // dims per lane
     constexpr int CH = 8;        // splits whose loads are in flight together
     float acc[PER], lse = -INFINITY;
+    int len = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) acc[i] = 0.f;
     if (in_range) {
-      const int n = num_splits(p, seq_len(p, heads_q.div(row)));
+      len = seq_len(p, heads_q.div(row));
+      const int n = num_splits(p, len);
       wait_first();
       float ls[CH], v[CH][PER];
       // Splits part, part + wpr, ..: each warp's in order, then the warps' in order.
@@ -512,6 +552,14 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const Params p, 
       }
     }
     if (!in_range) return;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) sum += acc[i];
+    if (__any_sync(0xffffffffu, sum != sum) && lse == lse) {
+      const float4 f = attend_again<E, D>(p, row, heads_q.div(row), len, lse);
+      acc[0] = f.x, acc[1] = f.y;
+      if constexpr (PER == 4) acc[2] = f.z, acc[3] = f.w;
+    }
     uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<E*>(p.out) + (size_t)row * D + PER * lane);
 #pragma unroll
     for (int i = 0; i < PER / 2; ++i) dst[i] = Elem<E>::pack(acc[2 * i], acc[2 * i + 1]);

@@ -401,6 +401,8 @@ FK_API int fk_w4_linear(const void* x, long long ldx, const void* packed, const 
  * head. mass_in / mass_out [batch, num_heads_kv, mass_capacity] fp32, may be the
  * same, null for no mass. Lengths are clamped to [0, max_seqlen]; a row of length 0
  * gives out = 0, lse = -inf. A page id outside [0, num_blocks) reads as zero rows.
+ * Infinities and NaN of live tokens follow the formulas: a score of -inf has weight 0,
+ * an infinite v makes its dimension infinite (NaN where its weight is 0).
  * workspace: fk_cache_attn_workspace_bytes bytes, 16-byte aligned, any contents;
  * calls that may overlap on the GPU need their own. */
 FK_API int fk_cache_attn_workspace_bytes(int batch, int max_seqlen, int num_heads_q, int num_heads_kv,

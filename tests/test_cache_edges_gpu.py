@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import cache_reference as ref
-from fused_kernels_cutedsl_lib_b200 import cache_attention
+from fused_kernels_cutedsl_lib_b200 import _native, cache_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -42,3 +42,30 @@ def test_keys_of_minus_infinity_leave_their_masses(G, D, dtype):
     keep = (~gone).nonzero().flatten()
     fewer = torch.tensor([289, 129], dtype=torch.int32, device="cuda")
     ref.check_attention(out, lse, mass[..., keep], before[..., keep], q, k[:, keep], v[:, keep], fewer)
+
+
+@pytest.mark.parametrize("D,dtype", [(64, FP16), (64, BF16), (128, FP16), (128, BF16)])
+@pytest.mark.parametrize("G", [1, 4, 9])
+def test_infinite_and_nan_values(G, D, dtype):
+    """An infinite element of v makes its dimension infinite, with its sign, and no other; opposite
+    infinities and NaN make it NaN: the products' own rules. The masses do not see v."""
+    lens = [1, 40, 700, 333]
+    q, k, v, lens, mass = make(4, 700, 2, G, D, dtype, lens, seed=D + G)
+    _, clean_lse = cache_attention(q, k, v, lens, mass=(clean_mass := mass.clone()))
+    v[0, 0, 0, 3] = INF
+    v[1, 7, 1, 0], v[1, 39, 1, 0] = INF, INF
+    v[1, 9, 0, D - 1] = -INF
+    v[2, 650, 0, 5], v[2, 3, 0, 6], v[2, 699, 0, 6] = -INF, INF, -INF
+    v[2, 333, 1, 17] = NAN
+    out, lse = cache_attention(q, k, v, lens, mass=mass)
+    assert torch.equal(lse, clean_lse) and torch.equal(mass, clean_mass)
+    want = ref.attention(q, k, v, lens)[0].float()
+    assert torch.equal(out.isnan(), want.isnan()), "NaN"
+    assert torch.equal(out.isposinf(), want.isposinf()) and torch.equal(out.isneginf(), want.isneginf())
+    finite = torch.where(v.isfinite(), v, 0.0)
+    expect, _ = cache_attention(q, k, finite, lens)
+    # Elsewhere the dimension does not know of it: fp32 sums in another order at most.
+    ok = want.isfinite()
+    err = (out.float() - expect.float()).abs()[ok]
+    assert (err <= torch.finfo(dtype).eps * expect.float().abs()[ok] + 2.0 ** -15).all()
+    assert _native.device_error() == 0
