@@ -20,7 +20,9 @@
 // share it. Running maximum and sum are fp32, in the log2 domain. P is multiplied as
 // a sum of two 16-bit numbers (its rounding and the rounding of the rest): the products
 // cost nothing next to the loads, and the output's error is then that of its own
-// rounding instead of sqrt(2) times it. With a mass, the raw log2-domain scores go
+// rounding instead of sqrt(2) times it. For fp16, whose least number is 2^-24, P is scaled by
+// 2^15: weights are held to 2^-40 of the greatest of their unit, not to 2^-25 (behind a
+// token that takes nearly all the weight, the others would vanish). With a mass, the raw log2-domain scores go
 // to scratch as fp32 (4 bytes per token and q head), because a token's weight is
 // known only with the lse of the whole row.
 //
@@ -79,6 +81,7 @@ template <typename E>
 struct Elem;
 template <>
 struct Elem<__nv_bfloat16> {
+  static constexpr float kShift = 0.f;  // P is 2^kShift times exp2(score - maximum)
   static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
   static __device__ __forceinline__ float lo(uint32_t v) { return __uint_as_float(v << 16); }
   static __device__ __forceinline__ float hi(uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); }
@@ -88,6 +91,7 @@ struct Elem<__nv_bfloat16> {
 };
 template <>
 struct Elem<__half> {
+  static constexpr float kShift = 15.f;
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<uint32_t*>(&h);
@@ -325,8 +329,9 @@ __global__ void __launch_bounds__(kThreads, kCtas) attend_kernel(const Params p)
         const float sf0 = mn0 == NEG_INF ? 0.f : mn0;  // nothing but -inf so far
         const float sf1 = mn1 == NEG_INF ? 0.f : mn1;
         const float al0 = exp2f(m[nt][0] - sf0), al1 = exp2f(m[nt][1] - sf1);
-        const float p0 = exp2f(y0 - sf0), p1 = exp2f(y1 - sf1);
-        const float p2 = exp2f(y2 - sf0), p3 = exp2f(y3 - sf1);
+        const float pf0 = sf0 - El::kShift, pf1 = sf1 - El::kShift;
+        const float p0 = exp2f(y0 - pf0), p1 = exp2f(y1 - pf1);
+        const float p2 = exp2f(y2 - pf0), p3 = exp2f(y3 - pf1);
         l[nt][0] = l[nt][0] * al0 + (p0 + p2);
         l[nt][1] = l[nt][1] * al1 + (p1 + p3);
         m[nt][0] = mn0;
@@ -386,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) attend_kernel(const Params p)
           dst[16 * i] = o[nt][i][e] * inv;
           dst[16 * i + 8] = o[nt][i][e + 2] * inv;
         }
-        if (g == 0) p.lse_part[row0 + hh] = L == 0.f ? NEG_INF : m[nt][e] + log2f(L);
+        if (g == 0) p.lse_part[row0 + hh] = L == 0.f ? NEG_INF : m[nt][e] + (log2f(L) - El::kShift);
       }
     }
   }

@@ -1,4 +1,6 @@
 """Corners of cache attention: non-finite keys and values, weights far apart (GPU)."""
+import math
+
 import pytest
 import torch
 
@@ -69,3 +71,30 @@ def test_infinite_and_nan_values(G, D, dtype):
     err = (out.float() - expect.float()).abs()[ok]
     assert (err <= torch.finfo(dtype).eps * expect.float().abs()[ok] + 2.0 ** -15).all()
     assert _native.device_error() == 0
+
+
+@pytest.mark.parametrize("D,dtype", [(64, FP16), (64, BF16), (128, FP16), (128, BF16)])
+@pytest.mark.parametrize("G", [1, 3, 12])
+@pytest.mark.parametrize("bits", [20, 26, 30])
+def test_small_weights_beside_a_dominant_one(bits, G, D, dtype):
+    """A first token that takes nearly all the weight and has values of 0, as attention sinks do: the
+    output is the sum over the others, whose weights lie 2^-bits below."""
+    L = 250
+    g = torch.Generator(device="cuda").manual_seed(bits)
+    q = torch.ones(1, G, D, device="cuda", dtype=dtype)
+    k = (0.01 * torch.randn(1, L, 1, D, generator=g, device="cuda")).to(dtype)
+    k[0, 0] = bits * math.log(2.0) / D ** 0.5
+    v = (2000.0 * (1.0 + torch.rand(1, L, 1, D, generator=g, device="cuda"))).to(dtype)
+    v[0, 0] = 0
+    lens = torch.tensor([L], dtype=torch.int32, device="cuda")
+    out, lse = cache_attention(q, k, v, lens)
+    want, rlse, _, absv, mag = ref.attention(q, k, v, lens)
+    # Half a step of the output (fp16: or of its subnormals), and the weights' relative errors as in
+    # cache_reference.check_attention. In fp16 the second part of a weight, 2^15 at most for the greatest, is a
+    # multiple of 2^-24: the two parts are off by half of that, 2^-25 / 2^15 = 2^-40 of the greatest weight per
+    # token, which is at most 1.
+    half = torch.finfo(dtype).eps / 2
+    tol = half * want.abs() + (2 * (D / 8 + 4) * 2.0 ** -24 * mag + 2.0 ** -19 + 2.0 ** -15)[..., None] * absv
+    tol += 2.0 ** -25 + 2.0 ** -40 * v.double().abs().sum(1) if dtype == FP16 else torch.finfo(dtype).tiny
+    err = (out.double() - want).abs()
+    assert (err <= tol).all(), f"worst {(err / tol).max().item():.3g} of the tolerance"
