@@ -136,12 +136,12 @@ def launch_stream(idx: int, stream=None) -> int:
     return stream.cuda_stream if isinstance(stream, torch.cuda.Stream) else int(stream)
 
 
-def scratch(nbytes: int, idx: int, stream_handle: int) -> torch.Tensor:
-    """Uninitialised bytes for one call on the given stream. Taken from torch's allocator on that
-    stream, so a block is reused only by work behind the call (and, in a captured graph, only by
-    that graph)."""
+def empty_on(shape, dtype: torch.dtype, idx: int, stream_handle: int) -> torch.Tensor:
+    """Uninitialised memory for a call on the given stream: scratch, or an output that the caller left to the
+    call. Taken from torch's allocator on that stream, so a block is reused only by work behind the call (and, in
+    a captured graph, only by that graph), and pending work of another stream never still needs it."""
     dev = torch.device("cuda", idx)
     if stream_handle == raw_current_stream(idx):
-        return torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        return torch.empty(shape, dtype=dtype, device=dev)
     with torch.cuda.stream(torch.cuda.ExternalStream(stream_handle, device=dev)):
-        return torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        return torch.empty(shape, dtype=dtype, device=dev)

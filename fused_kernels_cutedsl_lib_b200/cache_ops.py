@@ -24,8 +24,8 @@ import math
 import torch
 
 from . import _native
-from ._tensors import (current_device, dtype_code, launch_stream, on_device, one_device, require_dense, require_half,
-                       require_tensor, scratch)
+from ._tensors import (current_device, dtype_code, empty_on, launch_stream, on_device, one_device, require_dense,
+                       require_half, require_tensor)
 
 HEAD_DIMS = (64, 128)
 MAX_GROUP = 16
@@ -106,7 +106,7 @@ def _quick_attention(q, k, v, lens, out, lse, table, mass, mass_out, softmax_sca
 
 def _check_attention(q, k_cache, v_cache, cache_seqlens, out, lse, block_table, mass, mass_out, softmax_scale,
                      workspace):
-    """Raises what is wrong with the arguments of :func:`cache_attention`; (out, lse, scale), allocated if None."""
+    """Raises what is wrong with the arguments of :func:`cache_attention`; the scale."""
     require_half("q", q, strided_rows=True)
     dt = q.dtype
     if q.dim() != 3:
@@ -142,20 +142,16 @@ def _check_attention(q, k_cache, v_cache, cache_seqlens, out, lse, block_table, 
     scale = D ** -0.5 if softmax_scale is None else float(softmax_scale)
     if not math.isfinite(scale):
         raise ValueError(f"softmax_scale must be finite, got {softmax_scale}")
-    if out is None:
-        out = torch.empty((B, Hq, D), dtype=dt, device=q.device)
-    else:
+    if out is not None:
         require_half("out", out, dtype=dt)
         if out.numel() != B * Hq * D:
             raise ValueError(f"out must hold {B}x{Hq}x{D} elements, got shape {tuple(out.shape)}")
-    if lse is None:
-        lse = torch.empty((B, Hq), dtype=torch.float32, device=q.device)
-    else:
+    if lse is not None:
         require_dense("lse", lse, torch.float32, (B, Hq))
     if workspace is not None:
         require_tensor("workspace", workspace, torch.uint8, 1)
     one_device(q, k_cache, v_cache, cache_seqlens, block_table, mass, mass_out, out, lse, workspace)
-    return out, lse, scale
+    return scale
 
 
 def cache_attention(q, k_cache, v_cache, cache_seqlens, out=None, lse=None, *, block_table=None, mass=None,
@@ -168,7 +164,8 @@ def cache_attention(q, k_cache, v_cache, cache_seqlens, out=None, lse=None, *, b
     [B, Hkv, >= L]: for every token j < len,
     ``mass_out[b, h, j] = mass[b, h, j] + sum over h's q heads of the weight of j``;
     ``mass_out`` defaults to ``mass`` (else: other memory), and entries behind the lengths stay as they
-    are. An empty row gives 0 and lse -inf.
+    are. An empty row gives 0 and lse -inf. An ``out``, ``lse`` or ``workspace`` left to the call is memory of the
+    stream it runs on (``stream``, or torch's current one).
     """
     if isinstance(q, torch.Tensor) and q.dim() == 4 and q.shape[1] == 1:
         q = q.squeeze(1)
@@ -179,8 +176,8 @@ def cache_attention(q, k_cache, v_cache, cache_seqlens, out=None, lse=None, *, b
         scale = _quick_attention(q, k_cache, v_cache, cache_seqlens, out, lse, block_table, mass, mass_out,
                                  softmax_scale, workspace)
     if scale is None:
-        out, lse, scale = _check_attention(q, k_cache, v_cache, cache_seqlens, out, lse, block_table, mass, mass_out,
-                                           softmax_scale, workspace)
+        scale = _check_attention(q, k_cache, v_cache, cache_seqlens, out, lse, block_table, mass, mass_out, softmax_scale,
+                                 workspace)
     B, Hq, D = q.shape
     rows, L, Hkv = k_cache.shape[:3]
     idx = q.get_device()
@@ -188,15 +185,19 @@ def cache_attention(q, k_cache, v_cache, cache_seqlens, out=None, lse=None, *, b
     if block_table is not None:
         page, pages = L, rows
         L = block_table.shape[1] * page
-    if B == 0:
-        return out, lse
     if idx != current_device():
         with on_device(idx):
             return cache_attention(q, k_cache, v_cache, cache_seqlens, out, lse, block_table=block_table, mass=mass,
                                    mass_out=mass_out, softmax_scale=softmax_scale, workspace=workspace, stream=stream)
     st = launch_stream(idx, stream)
+    if out is None:
+        out = empty_on((B, Hq, D), q.dtype, idx, st)
+    if lse is None:
+        lse = empty_on((B, Hq), torch.float32, idx, st)
+    if B == 0:
+        return out, lse
     if workspace is None:
-        workspace = scratch(cache_attention_workspace_bytes(B, L, Hq, Hkv, D, mass is not None), idx, st)
+        workspace = empty_on(cache_attention_workspace_bytes(B, L, Hq, Hkv, D, mass is not None), torch.uint8, idx, st)
     _native.check(_native.load().fk_cache_attn_fwd(
         q.data_ptr(), q.stride(0) if B > 1 else Hq * D, k_cache.data_ptr(), v_cache.data_ptr(),
         block_table.data_ptr() if block_table is not None else None, cache_seqlens.data_ptr(),
@@ -270,7 +271,7 @@ def _quick_evict(k, v, lens, mass, k_out, v_out, lens_out, mass_out, budget, sin
 
 def _check_evict(k_cache, v_cache, cache_seqlens, mass, k_out, v_out, seqlens_out, mass_out, budget, sinks, recent,
                  block_table, out_block_table, kept):
-    """Raises what is wrong with the arguments of :func:`cache_evict`; kept, allocated if None."""
+    """Raises what is wrong with the arguments of :func:`cache_evict`."""
     require_half("k_cache", k_cache, 4)
     dt = k_cache.dtype
     rows, L, Hkv, D = k_cache.shape
@@ -311,9 +312,7 @@ def _check_evict(k_cache, v_cache, cache_seqlens, mass, k_out, v_out, seqlens_ou
         raise ValueError(f"mass must be [{B}, {Hkv}, >= {L}], got {tuple(mass.shape)}")
     if mass_out.shape[0] != B or mass_out.shape[1] != Hkv or cap_out < need:
         raise ValueError(f"mass_out must be [{B}, {Hkv}, >= {need}], got {tuple(mass_out.shape)}")
-    if kept is None:
-        kept = torch.empty((B, Hkv, budget), dtype=torch.int32, device=k_cache.device)
-    else:
+    if kept is not None:
         require_dense("kept", kept, torch.int32, (B, Hkv, budget))
     one_device(k_cache, v_cache, cache_seqlens, mass, k_out, v_out, seqlens_out, mass_out, block_table,
                out_block_table, kept)
@@ -321,7 +320,6 @@ def _check_evict(k_cache, v_cache, cache_seqlens, mass, k_out, v_out, seqlens_ou
                       out_block_table)
     if wrong is not None:
         raise ValueError(wrong)
-    return kept
 
 
 def cache_evict(k_cache, v_cache, cache_seqlens, mass, k_out, v_out, seqlens_out, mass_out, budget: int, *,
@@ -336,7 +334,7 @@ def cache_evict(k_cache, v_cache, cache_seqlens, mass, k_out, v_out, seqlens_out
     to ``mass_out`` [B, Hkv, >= min(budget, L)], which is zeroed behind them, the
     lengths to ``seqlens_out`` [B], and the old positions to ``kept`` int32
     [B, Hkv, budget] (-1 behind). Slots of ``k_out`` / ``v_out`` behind the lengths
-    stay as they are.
+    stay as they are. A ``kept`` left to the call is memory of the stream it runs on.
 
     The output cache is other memory than the input cache, or other pages of the
     same pools: ``out_block_table`` must name no page twice, and none that
@@ -345,8 +343,8 @@ def cache_evict(k_cache, v_cache, cache_seqlens, mass, k_out, v_out, seqlens_out
     budget, sinks, recent = int(budget), int(sinks), int(recent)
     if kept is None or not _quick_evict(k_cache, v_cache, cache_seqlens, mass, k_out, v_out, seqlens_out, mass_out, budget,
                                         sinks, recent, block_table, out_block_table, kept):
-        kept = _check_evict(k_cache, v_cache, cache_seqlens, mass, k_out, v_out, seqlens_out, mass_out, budget, sinks,
-                            recent, block_table, out_block_table, kept)
+        _check_evict(k_cache, v_cache, cache_seqlens, mass, k_out, v_out, seqlens_out, mass_out, budget, sinks, recent,
+                     block_table, out_block_table, kept)
     rows, L, Hkv, D = k_cache.shape
     rows_out, L_out = k_out.shape[:2]
     B, idx = cache_seqlens.shape[0], k_cache.get_device()
@@ -357,17 +355,20 @@ def cache_evict(k_cache, v_cache, cache_seqlens, mass, k_out, v_out, seqlens_out
     if out_block_table is not None:
         page_out, pages_out = L_out, rows_out
         L_out = out_block_table.shape[1] * page_out
-    if B == 0:
-        return kept
     if idx != current_device():
         with on_device(idx):
             return cache_evict(k_cache, v_cache, cache_seqlens, mass, k_out, v_out, seqlens_out, mass_out, budget,
                                sinks=sinks, recent=recent, block_table=block_table, out_block_table=out_block_table,
                                kept=kept, stream=stream)
+    st = launch_stream(idx, stream)
+    if kept is None:
+        kept = empty_on((B, Hkv, budget), torch.int32, idx, st)
+    if B == 0:
+        return kept
     _native.check(_native.load().fk_cache_evict(
         k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr() if block_table is not None else None,
         cache_seqlens.data_ptr(), mass.data_ptr(), mass.shape[2], k_out.data_ptr(), v_out.data_ptr(),
         out_block_table.data_ptr() if out_block_table is not None else None, seqlens_out.data_ptr(),
         mass_out.data_ptr(), mass_out.shape[2], kept.data_ptr(), B, L,
-        page, pages, L_out, page_out, pages_out, Hkv, D * 2, budget, sinks, recent, launch_stream(idx, stream)))
+        page, pages, L_out, page_out, pages_out, Hkv, D * 2, budget, sinks, recent, st))
     return kept

@@ -17,8 +17,8 @@ from dataclasses import dataclass
 import torch
 
 from . import _native
-from ._tensors import (current_device, dtype_code, launch_stream, on_device, one_device, require_dense, require_half,
-                       same_device)
+from ._tensors import (current_device, dtype_code, empty_on, launch_stream, on_device, one_device, require_dense,
+                       require_half, same_device)
 
 GROUP_SIZES = (32, 64, 128)
 _BLOCK_K = 128  # inputs per block
@@ -153,7 +153,8 @@ def w4_linear(x, weight: W4Weight, out=None, *, residual=None, stream=None):
     ``x`` [M, K] in the weight's dtype, any M (made for decode batches: up to 64
     tokens share one pass over the weight), rows may be strided (a multiple of 8
     elements); ``out`` and ``residual`` [M, N] dense, ``residual`` may be ``out``.
-    Otherwise ``out`` shares no memory with ``x``, ``residual`` or the weight.
+    Otherwise ``out`` shares no memory with ``x``, ``residual`` or the weight. An ``out`` left to the call
+    is memory of the stream it runs on (``stream``, or torch's current one).
     """
     if not isinstance(weight, W4Weight):
         raise TypeError(f"weight must be a W4Weight (pack_w4, quantize_w4), got {type(weight).__name__}")
@@ -173,22 +174,23 @@ def w4_linear(x, weight: W4Weight, out=None, *, residual=None, stream=None):
             raise ValueError(f"x is [M, K={xk}] but the weight is [N={n}, K={k}]")
         if m > 1 and (x.stride(0) < k or x.stride(0) % 8):
             raise ValueError(f"x row stride must be >= K and a multiple of 8 elements, got {x.stride(0)}")
-        if out is None:
-            out = torch.empty((m, n), dtype=dt, device=x.device)
-        else:
+        if out is not None:
             require_dense("out", out, dt, (m, n))
         if residual is not None:
             require_dense("residual", residual, dt, (m, n))
         idx = one_device(x, packed, out, residual)
     m = x.shape[0]
     ldx = x.stride(0) if m > 1 else k
-    if m == 0:
-        return out
     if idx != current_device():
         with on_device(idx):
             return w4_linear(x, weight, out, residual=residual, stream=stream)
+    st = launch_stream(idx, stream)
+    if out is None:
+        out = empty_on((m, n), dt, idx, st)
+    if m == 0:
+        return out
     _native.check(_native.load().fk_w4_linear(
         x.data_ptr(), ldx, packed.data_ptr(),
         residual.data_ptr() if residual is not None else None, out.data_ptr(), dtype_code(dt), m, n, k,
-        weight.group_size, launch_stream(idx, stream)))
+        weight.group_size, st))
     return out
