@@ -29,6 +29,7 @@ from ._tensors import (current_device, dtype_code, empty_on, launch_stream, on_d
 
 HEAD_DIMS = (64, 128)
 MAX_GROUP = 16
+MAX_TOKENS = 1 << 30  # of a row, in a cache or to be kept
 
 _HALF = (torch.bfloat16, torch.float16)
 _I32, _F32, _U8 = torch.int32, torch.float32, torch.uint8
@@ -39,6 +40,8 @@ def cache_attention_workspace_bytes(batch: int, max_seqlen: int, num_heads_q: in
     """Bytes of scratch a :func:`cache_attention` call of these sizes needs on the current device
     (``max_seqlen``: tokens a row of the cache can hold)."""
     n = ctypes.c_size_t(0)
+    if max_seqlen > MAX_TOKENS:
+        raise ValueError(f"max_seqlen must be <= {MAX_TOKENS}, got {max_seqlen}")
     _native.check(_native.load().fk_cache_attn_workspace_bytes(
         int(batch), int(max_seqlen), int(num_heads_q), int(num_heads_kv), int(head_dim), int(bool(mass)),
         ctypes.byref(n)))
@@ -87,6 +90,8 @@ def _quick_attention(q, k, v, lens, out, lse, table, mass, mass_out, softmax_sca
             if tb != B or tp < 1:
                 return None
             L *= tp
+        if L > MAX_TOKENS:
+            return None
         if mass is not None:
             if not (mass.dtype == _F32 and mass.is_contiguous() and mass.get_device() == idx and mass.dim() == 3
                     and mass.shape[0] == B and mass.shape[1] == Hkv and mass.shape[2] >= L):
@@ -129,6 +134,8 @@ def _check_attention(q, k_cache, v_cache, cache_seqlens, out, lse, block_table, 
         raise ValueError(f"the caches hold {rows} rows but q has {B}")
     if L < 1 or (block_table is not None and pages < 1):
         raise ValueError("the cache holds no tokens")
+    if L > MAX_TOKENS:
+        raise ValueError(f"a row of the cache holds {L} tokens, at most {MAX_TOKENS} are supported")
     cap = 0
     if mass is not None:
         require_tensor("mass", mass, torch.float32, 3)
@@ -236,7 +243,7 @@ def _quick_evict(k, v, lens, mass, k_out, v_out, lens_out, mass_out, budget, sin
         dt, idx = k.dtype, k.get_device()
         (B,) = lens.shape
         if not (dt in _HALF and idx >= 0 and h_out == H and d_out == D and H and D and D % 8 == 0 and L
-                and budget >= 1 and sinks >= 0 and recent >= 0 and sinks + recent <= budget and k.is_contiguous()
+                and 1 <= budget <= MAX_TOKENS and sinks >= 0 and recent >= 0 and sinks + recent <= budget and k.is_contiguous()
                 and v.dtype == dt and v.is_contiguous() and v.get_device() == idx and v.shape == k.shape
                 and k_out.dtype == dt and k_out.is_contiguous() and k_out.get_device() == idx
                 and v_out.dtype == dt and v_out.is_contiguous() and v_out.get_device() == idx
@@ -263,7 +270,7 @@ def _quick_evict(k, v, lens, mass, k_out, v_out, lens_out, mass_out, budget, sin
         need = min(budget, L)
         mb, mh, cap = mass.shape
         ob, oh, out_cap = mass_out.shape
-        return (L_out >= need and mb == B and mh == H and cap >= L and ob == B and oh == H and out_cap >= need
+        return (L <= MAX_TOKENS and L_out <= MAX_TOKENS and L_out >= need and mb == B and mh == H and cap >= L and ob == B and oh == H and out_cap >= need
                 and _overlaps(k, v, lens, mass, k_out, v_out, lens_out, mass_out, table, out_table) is None)
     except (AttributeError, TypeError, ValueError):
         return False  # something is no tensor, or has other dimensions: the checks say what
@@ -286,8 +293,8 @@ def _check_evict(k_cache, v_cache, cache_seqlens, mass, k_out, v_out, seqlens_ou
     require_tensor("cache_seqlens", cache_seqlens, torch.int32, 1)
     B = cache_seqlens.shape[0]
     require_dense("seqlens_out", seqlens_out, torch.int32, (B,))
-    if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
-        raise ValueError(f"budget ({budget}) must be >= 1 and sinks ({sinks}) + recent ({recent}) must lie in "
+    if budget < 1 or budget > MAX_TOKENS or sinks < 0 or recent < 0 or sinks + recent > budget:
+        raise ValueError(f"budget ({budget}) must lie in [1, {MAX_TOKENS}] and sinks ({sinks}) + recent ({recent}) must lie in "
                          f"[0, budget]")
     page = pages = page_out = pages_out = 0
     if block_table is not None:
@@ -303,6 +310,8 @@ def _check_evict(k_cache, v_cache, cache_seqlens, mass, k_out, v_out, seqlens_ou
     elif rows_out != B:
         raise ValueError(f"the output caches hold {rows_out} rows but there are {B} lengths")
     need = min(budget, L)
+    if max(L, L_out) > MAX_TOKENS:
+        raise ValueError(f"rows of the caches hold {L} and {L_out} tokens, at most {MAX_TOKENS} are supported")
     if L < 1 or L_out < need:
         raise ValueError(f"the output cache holds {L_out} tokens per row, needs {need} (and the input at least 1)")
     require_tensor("mass", mass, torch.float32, 3)

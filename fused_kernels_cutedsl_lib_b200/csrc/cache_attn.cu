@@ -724,6 +724,7 @@ static int by_group(const Params& p, cudaStream_t st) {
 
 static int check_sizes(int B, int Lmax, int Hq, int Hkv, int D) {
   FK_CHECK_ARG(B >= 1 && Lmax >= 1, "batch and max_seqlen must be >= 1");
+  FK_CHECK_ARG(Lmax <= (1 << 30), "max_seqlen must be <= 2^30");
   FK_CHECK_ARG(D == 64 || D == 128, "head_dim must be 64 or 128");
   FK_CHECK_ARG(Hkv >= 1 && Hq >= Hkv && Hq % Hkv == 0, "num_heads_q must be a positive multiple of num_heads_kv");
   FK_CHECK_ARG(Hq / Hkv <= 16, "GQA group size (num_heads_q / num_heads_kv) must be <= 16");

@@ -413,6 +413,8 @@ extern "C" int fk_cache_evict(const void* k_cache, const void* v_cache, const in
   FK_CHECK_ARG(k_cache && v_cache && cache_seqlens && mass && k_out && v_out && seqlens_out && mass_out && kept,
                "null tensor pointer");
   FK_CHECK_ARG(batch >= 1 && max_seqlen >= 1 && num_heads_kv >= 1, "sizes must be positive");
+  FK_CHECK_ARG(max_seqlen <= (1 << 30) && out_max_seqlen <= (1 << 30) && budget <= (1 << 30),
+               "max_seqlen, out_max_seqlen and budget must be <= 2^30");
   FK_CHECK_ARG(row_bytes >= 16 && row_bytes % 16 == 0, "row_bytes must be a positive multiple of 16");
   FK_CHECK_ARG(budget >= 1 && sinks >= 0 && recent >= 0 && (long long)sinks + recent <= budget,
                "budget must be >= 1 and sinks + recent must lie in [0, budget]");

@@ -399,8 +399,9 @@ FK_API int fk_w4_linear(const void* x, long long ldx, const void* packed, const 
  * head_dim] with pages of any size; all bf16 or fp16 (dtype). lse [batch,
  * num_heads_q] fp32, natural log. head_dim 64 or 128, at most 16 q heads per kv
  * head. mass_in / mass_out [batch, num_heads_kv, mass_capacity] fp32, may be the
- * same, null for no mass. Lengths are clamped to [0, max_seqlen]; a row of length 0
- * gives out = 0, lse = -inf. A page id outside [0, num_blocks) reads as zero rows.
+ * same, null for no mass. max_seqlen is at most 2^30. Lengths are clamped to
+ * [0, max_seqlen]; a row of length 0 gives out = 0, lse = -inf. A page id outside
+ * [0, num_blocks) reads as zero rows.
  * Infinities and NaN of live tokens follow the formulas: a score of -inf has weight 0,
  * an infinite v makes its dimension infinite (NaN where its weight is 0).
  * workspace: fk_cache_attn_workspace_bytes bytes, 16-byte aligned, any contents;
@@ -424,8 +425,9 @@ FK_API int fk_cache_attn_fwd(const void* q, long long q_batch_stride, const void
  * layouts as fk_cache_attn_fwd; the output cache (contiguous [batch,
  * out_max_seqlen, ...] or paged) is other memory than the input cache, or other
  * pages of the same pools: no page that the input table names for a live token.
- * No output page may serve two places. Input page ids outside the pool read as
- * zero rows, output ones are not written. */
+ * max_seqlen, out_max_seqlen and budget are at most 2^30. No output page may serve two
+ * places. Input page ids outside the pool read as zero rows, output ones are not
+ * written. */
 FK_API int fk_cache_evict(const void* k_cache, const void* v_cache, const int32_t* block_table,
                           const int32_t* cache_seqlens, const float* mass, long long mass_capacity, void* k_out,
                           void* v_out, const int32_t* out_block_table, int32_t* seqlens_out, float* mass_out,

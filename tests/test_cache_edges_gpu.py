@@ -1,11 +1,11 @@
-"""Corners of cache attention: non-finite keys and values, weights far apart (GPU)."""
+"""Corners of the cache operators: non-finite keys and values, weights far apart, sizes past an int (GPU)."""
 import math
 
 import pytest
 import torch
 
 import cache_reference as ref
-from fused_kernels_cutedsl_lib_b200 import _native, cache_attention
+from fused_kernels_cutedsl_lib_b200 import _native, cache_attention, cache_evict
 
 pytestmark = pytest.mark.gpu
 
@@ -98,3 +98,17 @@ def test_small_weights_beside_a_dominant_one(bits, G, D, dtype):
     tol += 2.0 ** -25 + 2.0 ** -40 * v.double().abs().sum(1) if dtype == FP16 else torch.finfo(dtype).tiny
     err = (out.double() - want).abs()
     assert (err <= tol).all(), f"worst {(err / tol).max().item():.3g} of the tolerance"
+
+
+def test_sizes_past_a_c_int_are_refused():
+    """2^32 + 4 tokens to keep are not 4, and a table of 2^32 + 1024 tokens is not one of 1024."""
+    _, k, v, lens, mass = make(1, 64, 1, 1, 64, BF16, [64])
+    outs = (torch.zeros_like(k), torch.zeros_like(v), torch.zeros_like(lens), torch.zeros_like(mass))
+    for budget in (2 ** 32 + 4, 2 ** 31 + 4, 2 ** 30 + 1):
+        with pytest.raises(ValueError):
+            cache_evict(k, v, lens, mass, *outs, budget)
+    q, pool = torch.zeros(1, 1, 64, device="cuda").to(BF16), torch.zeros(2, 1024, 1, 64, device="cuda").to(BF16)
+    table = torch.zeros(1, 2 ** 22 + 1, dtype=torch.int32, device="cuda")
+    for out, lse in ((None, None), (torch.empty_like(q), torch.empty(1, 1, device="cuda"))):
+        with pytest.raises(ValueError):
+            cache_attention(q, pool, pool, lens, out, lse, block_table=table)
