@@ -183,6 +183,8 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, 1) w4_linear_kernel(const Pa
                 const int n = min(rows_stage, nr - rg - q * rows_stage);
                 if (n <= 0) break;
                 const uint32_t bytes = (uint32_t)(n * nb) * BB;
+                // Stages are emptied by warps that wait for the preceding kernel, however long it takes.
+                if (filled == kStages) asm volatile("griddepcontrol.wait;" ::: "memory");
                 if (filled >= kStages) live = w4::wait(&empty[stage], phase ^ 1, p.err, kDevErrEmptyWait);
                 if (!live) break;
                 mbar_arrive_expect_tx(&full[stage], bytes);

@@ -33,6 +33,10 @@
 // The inputs are split over the CS CTAs of a cluster; their sums go to the shared memory
 // of the CTA that owns the rows (mbarrier with one arrival per CTA), which adds them in a
 // fixed order: no workspace, no atomic.
+//
+// Every wait here is bounded, except that for the preceding kernel of the stream (programmatic
+// dependent launch): each warp waits for that before its first bounded wait for anything that
+// follows from x, so that a long predecessor is not taken for a fault.
 #include <cuda_fp16.h>
 
 #include <mutex>
@@ -297,6 +301,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t x_full0 = smem_u32(x_full), a_full0 = smem_u32(a_full), d_empty0 = smem_u32(d_empty);
     uint32_t st = 0, ph = 0;
     bool ok = true;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     for (int i = 0; i < nsl && ok; ++i) {
       const int b = i & 1, nb = slab_blocks(rank + i * cs);
       ok = w4::wait_at(x_full0 + st * 8, ph, p.err, kDevErrFullWait) &&
@@ -358,6 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // next arrival must not count for.
       auto buffer_free = [&] {
         if (i < 2) return true;
+        if (i < 4) asm volatile("griddepcontrol.wait;" ::: "memory");  // this warp's first wait for products
         const bool done = __all_sync(~0u, w4::wait_at(x_empty0 + xst * 8, xph, p.err, kDevErrMmaWait));
         xst += 2;
         if (xst >= SX) xst -= SX, xph ^= 1;
@@ -413,6 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
   for (int n = 0; n < HT; ++n) acc[n] = 0.f;
   bool ok = true;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   for (int i = 0; i < nsl && ok; ++i) {
     const bool tail = short_tail && i == nsl - 1;
     const uint32_t b8 = (i & 1) * 8, db8 = DB == 2 ? b8 : 0;
@@ -461,7 +468,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // ---- the sums go to the CTAs that own the rows, 128 / cs each ----
   w4::cluster_wait();
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   {
     const int tid = threadIdx.x - kAddWarp * 32;
     const int rows_log = 7 - p.cs_log, owner = r >> rows_log, slot = r & ((1 << rows_log) - 1);
