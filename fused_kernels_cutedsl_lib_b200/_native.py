@@ -129,6 +129,7 @@ SIGNATURES: dict[str, tuple] = {
         _c_int,
         [_p, ctypes.c_longlong, _p, _p, _p, _c_int, _c_int, _c_int, _c_int, _c_int, _p],
     ),
+    "fk_debug_w4_withhold_slab": (_c_int, [_c_int]),
     "fk_cache_attn_workspace_bytes": (
         _c_int,
         [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, ctypes.POINTER(ctypes.c_size_t)],

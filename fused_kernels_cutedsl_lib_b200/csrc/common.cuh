@@ -278,6 +278,10 @@ struct FastDiv {
   __device__ __forceinline__ int div(int n) const { return shift < 0 ? n : (int)(__umulhi((uint32_t)n, m) >> shift); }
 };
 
+// Arrival at a named barrier without waiting for it.
+__device__ __forceinline__ void named_bar_arrive(int id, int nthreads) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
+}
 // Named barrier among `nthreads` threads (id 0 is __syncthreads).
 __device__ __forceinline__ void named_bar_sync(int id, int nthreads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");

@@ -23,6 +23,7 @@ struct Call {
   int* err;
   bool bf16;
   int M, N, K, group;
+  int withhold;  // test hook: the slab whose copy the first CTA leaves out (-1: none)
 };
 // The form of w4_tc.cu.
 int linear_tc(const Call& c, cudaStream_t st);
@@ -152,6 +153,14 @@ __device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, int
   }
   record_device_error(err, kDevErrFlagWait);
   return false;
+}
+// A thread whose wait for the cluster ran out keeps its CTA in place for another four bounds before it leaves:
+// others of the cluster may still store into the CTA's shared memory. They stop at the latest when a wait
+// of their own for this CTA has run out. (A second phase of the cluster's barrier would not do: it has
+// no bound, and a CTA that has ended without arriving is waited for.)
+__device__ __forceinline__ void linger(const int* err) {
+  const uint64_t t0 = global_timer_ns(), lim = 4 * wait_limit_ns(err);
+  while (global_timer_ns() - t0 < lim) __nanosleep(1000);
 }
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   uint4 v;

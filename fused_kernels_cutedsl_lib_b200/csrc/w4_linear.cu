@@ -75,6 +75,7 @@ struct Params {
   int kw_log;                // log2 of the warps that share a row block
   int chunk;                 // slabs of a CTA whose x is staged at a time
   int tile;                  // row blocks per cluster whose partial sums are held at a time
+  int withhold;              // test hook: the fill that the first CTA's producer leaves out (-1: none)
 };
 
 // D = A * B: the first step of a group starts from nothing.
@@ -140,6 +141,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, 1) w4_linear_kernel(const Pa
   uint64_t* empty = full + kStages;
   uint64_t* done = empty + kStages;  // one arrival per CTA: its partial sums of the tile are stored
   uint64_t* taken = done + 1;        // one arrival per CTA: it has added up the tile's
+  volatile int* gave_up = reinterpret_cast<volatile int*>(taken + 1);  // a wait of this CTA has run out
   uint8_t* xmem = smem + ring_bytes<GROUP>();
   uint4* xs = reinterpret_cast<uint4*>(xmem);                                           // [chunk][blocks][4 words j][NT][32 lanes]
   float4* xsum = reinterpret_cast<float4*>(xmem + (size_t)p.chunk * xop_bytes<NT>());   // [chunk][blocks][GPB][TOK / 2]: sums of two tokens, then their offset sums
@@ -154,6 +156,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, 1) w4_linear_kernel(const Pa
     }
     mbar_init(done, cs);
     mbar_init(taken, cs);
+    *gave_up = 0;
     fence_barrier_init();
   }
   __syncthreads();
@@ -187,9 +190,11 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, 1) w4_linear_kernel(const Pa
                 if (filled == kStages) asm volatile("griddepcontrol.wait;" ::: "memory");
                 if (filled >= kStages) live = w4::wait(&empty[stage], phase ^ 1, p.err, kDevErrEmptyWait);
                 if (!live) break;
-                mbar_arrive_expect_tx(&full[stage], bytes);
-                bulk_load(smem_u32(smem + stage * stage_bytes<GROUP>()), src + (size_t)(q * rows_stage * nb) * BB, bytes,
-                          &full[stage], pol);
+                if (filled != p.withhold || blockIdx.x != 0) {
+                  mbar_arrive_expect_tx(&full[stage], bytes);
+                  bulk_load(smem_u32(smem + stage * stage_bytes<GROUP>()), src + (size_t)(q * rows_stage * nb) * BB,
+                            bytes, &full[stage], pol);
+                }
                 ++filled;
                 if (++stage == kStages) {
                   stage = 0;
@@ -231,13 +236,16 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, 1) w4_linear_kernel(const Pa
       ph ^= 1;
     }
   };
-  bool ok = true;
+  bool ok = true;  // the same in all lanes wherever products depend on it
 
   uint32_t tile_phase = 0;
-  // All of this CTA's multiplying warps have come here, and one of them tells the cluster.
+  // All of this CTA's multiplying warps have come here, and one of them tells the cluster; no more of that once a
+  // wait of any of them has run out. The CTA then goes through the rest without waiting; the cluster's other
+  // CTAs, which now wait in vain, do the same.
   auto tell = [&](uint64_t* bar) {
+    if (!ok) *gave_up = 1;
     named_bar_sync(1, W * 32);
-    if (warp == 0 && lane < cs) arrive_cluster(map_to(smem_u32(bar), lane));
+    if (warp == 0 && lane < cs && *gave_up == 0) arrive_cluster(map_to(smem_u32(bar), lane));
   };
   for (int r0 = rb0; r0 < rb1; r0 += p.tile, tile_phase ^= 1) {
     const int nr = min(p.tile, rb1 - r0);
@@ -327,14 +335,15 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, 1) w4_linear_kernel(const Pa
           cluster_wait();
         else if (ok)  // the owners are done with the tile before
           ok = wait_cluster(taken, tile_phase ^ 1, p.err);
-        __syncwarp();
+        if (__any_sync(0xffffffffu, !ok)) ok = false;
       }
 
       const ExpandConsts consts;
       for (int rg = 0; rg < nr; rg += NG * rows_stage) {
         const int lr = rg + gid * rows_stage + wrow;                      // this warp's row block of the tile
         const int groups = min(NG, (nr - rg + rows_stage - 1) >> (3 - p.kw_log));  // warp groups with rows in this round
-        const bool mine = gid < groups, live = lr < nr;
+        bool mine = gid < groups && ok;
+        const bool live = lr < nr;
         float acc[NT][4];
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
@@ -344,7 +353,10 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, 1) w4_linear_kernel(const Pa
         for (int sl = c0; sl < c1; ++sl) {
           advance(stage, phase, groups);
           if (!mine) continue;
-          if (ok && !w4::wait(&full[st], ph, p.err, kDevErrFullWait)) ok = false;
+          if (!__all_sync(0xffffffffu, w4::wait(&full[st], ph, p.err, kDevErrFullWait))) {
+            ok = mine = false;  // nor are its stages given back
+            continue;
+          }
           if (live) {
             const int nb = slab_blocks(rank + sl * cs);
             const int b0 = wk * (kSlab >> p.kw_log), b1 = min(nb, b0 + (kSlab >> p.kw_log));
@@ -478,7 +490,10 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, 1) w4_linear_kernel(const Pa
     }
     if (r0 + p.tile < rb1) tell(taken);  // the next tile's partial sums overwrite these
   }
+  if (__any_sync(0xffffffffu, !ok)) linger(p.err);
 }
+
+static int g_withhold = -1;  // fk_debug_w4_withhold_slab
 
 // Clusters of 1, 2, 4 and 8 CTAs that can be resident at once, one CTA per SM; asked once per
 // kernel and device (asking takes longer than a launch).
@@ -610,7 +625,8 @@ extern "C" int fk_w4_linear(const void* x, long long ldx, const void* packed, co
   // 14336, 27.1 / 19.0 on 28672 x 4096.
   const int tiles = (N + 127) / 128, sms = num_sms();
   if (M > 16 || (M > 8 && (tiles <= sms || 5 * tiles > 8 * sms))) {
-    const w4::Call c{x, ldx, static_cast<const uint8_t*>(packed), residual, y, err, dtype == FK_BF16, M, N, K, group_size};
+    const w4::Call c{x, ldx, static_cast<const uint8_t*>(packed), residual, y, err, dtype == FK_BF16, M, N, K, group_size,
+                    w4::g_withhold};
     return w4::linear_tc(c, st);
   }
   w4::Params p = {};
@@ -626,6 +642,12 @@ extern "C" int fk_w4_linear(const void* x, long long ldx, const void* packed, co
   p.nrb = (N + 15) / 16;
   p.nkb = (K + w4::kBlockK - 1) / w4::kBlockK;
   p.nslab = (p.nkb + w4::kSlab - 1) / w4::kSlab;
+  p.withhold = w4::g_withhold;
   if (dtype == FK_BF16) return w4::by_tokens<__nv_bfloat16>(p, group_size, st);
   return w4::by_tokens<__half>(p, group_size, st);
+}
+
+extern "C" int fk_debug_w4_withhold_slab(int slab) {
+  w4::g_withhold = slab < 0 ? -1 : slab;
+  return kOk;
 }

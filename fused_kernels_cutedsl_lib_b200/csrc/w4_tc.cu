@@ -34,9 +34,9 @@
 // of the CTA that owns the rows (mbarrier with one arrival per CTA), which adds them in a
 // fixed order: no workspace, no atomic.
 //
-// Every wait here is bounded, except that for the preceding kernel of the stream (programmatic
-// dependent launch): each warp waits for that before its first bounded wait for anything that
-// follows from x, so that a long predecessor is not taken for a fault.
+// Waits for copies, products and other CTAs are bounded, that for the preceding kernel of the stream
+// (programmatic dependent launch) is not: each warp waits for it before its first bounded wait for
+// anything that follows from x, so that a long predecessor is not taken for a fault.
 #include <cuda_fp16.h>
 
 #include <mutex>
@@ -57,6 +57,7 @@ constexpr int kRowBlocks = 8;  // of 16 rows
 // Warps: 0-15 expand, 16-23 add up, 24 loads, 25 issues the products.
 constexpr int kAddWarp = 16, kLoadWarp = 24, kMmaWarp = 25, kThreads = 26 * 32;
 constexpr int kSmem = 227 * 1024;
+constexpr int kTmemBar = 2, kTmemThreads = 25 * 32;  // named barrier: all but the loading warp are done with TMEM
 constexpr uint32_t kACol = 256;  // TMEM: D of warp group w at 128 w, its A buffers at 256 + 128 w + 64 buf
 
 struct Params {
@@ -67,6 +68,7 @@ struct Params {
   int M, N;
   int nrb, nkb, nslab;
   int cs_log;
+  int withhold;  // test hook: the slab of x that the first CTA does not load (-1: none)
 };
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -213,8 +215,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* d_full = a_full + 2;    // [slab & 1], with one accumulator buffer: [block of the slab]
   uint64_t* d_empty = d_full + 2;   // same
   uint64_t* done = d_empty + 2;  // one arrival per CTA: its partial sums are stored
-  uint64_t* tmem_done = done + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_done + 1);
+  uint64_t* idle = done + 1;     // every product that was issued is done
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(idle + 1);
 
   using Half = w4::Half<T>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -238,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&d_empty[i], 8);
     }
     mbar_init(done, cs);
-    mbar_init(tmem_done, 8);
+    mbar_init(idle, 1);
     fence_barrier_init();
   }
   if (warp == kMmaWarp) {
@@ -256,24 +258,28 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == kLoadWarp) {
     // ------------------------------ loads ------------------------------
+    const uint64_t pol_w = l2_policy_evict_first(), pol_x = l2_policy_evict_last();
+    const int rows = min(kRowBlocks, p.nrb - tile * kRowBlocks);
+    int nw = 0, nx = 0;  // slabs of the weight and of x whose copies have been issued
+    auto load_w = [&](int i) {
+      const int st = i % S, s = rank + i * cs, nb = slab_blocks(s);
+      nw = i + 1;
+      const uint32_t bytes = (uint32_t)(rows * nb) * BB;
+      mbar_arrive_expect_tx(&full[st], bytes);
+      w4::bulk_load(smem_u32(wring + st * STAGE),
+                    p.packed + ((size_t)s * kSlab * p.nrb + (size_t)tile * kRowBlocks * nb) * BB, bytes, &full[st], pol_w);
+    };
+    auto load_x = [&](int i) {
+      const int st = i % SX, s = rank + i * cs, nb = slab_blocks(s);
+      nx = i + 1;
+      if (i == p.withhold && blockIdx.x == 0 && blockIdx.y == 0) return;
+      mbar_arrive_expect_tx(&x_full[st], nb * 2 * NTOK * 128);
+      for (int q = 0; q < nb * 2; ++q)
+        tma_load_2d(smem + st * XSTAGE + q * (NTOK * 128), &tmX, &x_full[st], s * kSlab * kBlockK + q * 64, tok0, pol_x);
+    };
+    // The weights' first copies do not wait for the preceding kernel, x does.
     if (lane == 0) {
       tma_prefetch_desc(&tmX);
-      const uint64_t pol_w = l2_policy_evict_first(), pol_x = l2_policy_evict_last();
-      const int rows = min(kRowBlocks, p.nrb - tile * kRowBlocks);
-      auto load_w = [&](int i) {
-        const int st = i % S, s = rank + i * cs, nb = slab_blocks(s);
-        const uint32_t bytes = (uint32_t)(rows * nb) * BB;
-        mbar_arrive_expect_tx(&full[st], bytes);
-        w4::bulk_load(smem_u32(wring + st * STAGE),
-                      p.packed + ((size_t)s * kSlab * p.nrb + (size_t)tile * kRowBlocks * nb) * BB, bytes, &full[st], pol_w);
-      };
-      auto load_x = [&](int i) {
-        const int st = i % SX, s = rank + i * cs, nb = slab_blocks(s);
-        mbar_arrive_expect_tx(&x_full[st], nb * 2 * NTOK * 128);
-        for (int q = 0; q < nb * 2; ++q)
-          tma_load_2d(smem + st * XSTAGE + q * (NTOK * 128), &tmX, &x_full[st], s * kSlab * kBlockK + q * 64, tok0, pol_x);
-      };
-      // The weights' first copies do not wait for the preceding kernel, x does.
       for (int i = 0; i < min(S, nsl); ++i) load_w(i);
       asm volatile("griddepcontrol.wait;" ::: "memory");
       for (int i = 0; i < min(SX, nsl); ++i) load_x(i);
@@ -287,11 +293,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           load_w(i + S);
         }
       }
+      // No copy may be in flight when the CTA ends, also when the warps that wait for them gave up.
+      for (int i = max(0, nw - S); i < nw; ++i) w4::wait(&full[i % S], (i / S) & 1, p.err, kDevErrFullWait);
+      for (int i = max(0, nx - SX); i < nx; ++i) w4::wait(&x_full[i % SX], (i / SX) & 1, p.err, kDevErrFullWait);
     }
     __syncwarp();
     w4::cluster_wait();
     return;
   }
+  w4::cluster_wait();  // the other warps have something to wait for in any case
 
   if (warp == kMmaWarp) {
     // ------------------------------ products ------------------------------
@@ -332,10 +342,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (++st == SX) st = 0, ph ^= 1;
     }
     __syncwarp();
-    w4::wait(tmem_done, 0, p.err, kDevErrMmaWait);  // D has been read
+    // TMEM is given back when all products are done and all warps are through with it, those that gave up
+    // among them: their waits are bounded, so the barrier fills.
+    if (leader) umma_commit(idle);
+    __syncwarp();
+    w4::wait(idle, 0, p.err, kDevErrMmaWait);
+    named_bar_sync(kTmemBar, kTmemThreads);
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
-    w4::cluster_wait();
     return;
   }
 
@@ -406,8 +420,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       st += 2;
       if (st >= S) st -= S, ph ^= 1;
     }
+    tc_fence_before();
     __syncwarp();
-    w4::cluster_wait();
+    named_bar_arrive(kTmemBar, kTmemThreads);
     return;
   }
 
@@ -463,11 +478,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (++st == S) st = 0;
   }
+  tc_fence_before();
   __syncwarp();
-  if (lane == 0) mbar_arrive(tmem_done);
+  named_bar_arrive(kTmemBar, kTmemThreads);
 
   // ---- the sums go to the CTAs that own the rows, 128 / cs each ----
-  w4::cluster_wait();
   {
     const int tid = threadIdx.x - kAddWarp * 32;
     const int rows_log = 7 - p.cs_log, owner = r >> rows_log, slot = r & ((1 << rows_log) - 1);
@@ -496,7 +511,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     load_residual(tid + 256, res[1]);
     named_bar_sync(1, 256);
     if (warp == kAddWarp && lane < cs) w4::arrive_cluster(w4::map_to(smem_u32(done), lane));
-    if (!w4::wait_cluster(done, 0, p.err)) return;
+    if (!__all_sync(~0u, w4::wait_cluster(done, 0, p.err))) {
+      w4::linger(p.err);
+      return;
+    }
     for (int e0 = tid; e0 < elems; e0 += 512) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -570,6 +588,7 @@ static int launch(const w4::Call& c, cudaStream_t st) {
   p.err = c.err;
   p.M = c.M;
   p.N = c.N;
+  p.withhold = c.withhold;
   p.nrb = (c.N + 15) / 16;
   p.nkb = (c.K + kBlockK - 1) / kBlockK;
   p.nslab = (p.nkb + kSlab - 1) / kSlab;

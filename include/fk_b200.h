@@ -388,6 +388,9 @@ FK_API int fk_skinny_gemm_noalloc(const void* x, const void* w, void* y, int M, 
  * kernel of this library that precedes the call on its stream. */
 FK_API int fk_w4_linear(const void* x, long long ldx, const void* packed, const void* residual, void* y, int dtype,
                         int M, int N, int K, int group_size, void* stream);
+/* Test hook: the first CTA of the following fk_w4_linear calls leaves out the copy of one
+ * slab, so that waits run out (-1: none). Their results are undefined. */
+FK_API int fk_debug_w4_withhold_slab(int slab);
 
 /* Attention of one new token per row over a KV cache, with the attention mass:
  *   out = softmax(scale q K^T) V over the first cache_seqlens[b] tokens,
