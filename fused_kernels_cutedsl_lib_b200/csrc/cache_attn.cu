@@ -107,8 +107,11 @@ struct Elem<__half> {
   }
 };
 
+// Both kernels are resident while kernels before them still write what they read: lengths, q, tables and caches, and
+// in pass 2 the partial results and scores. So nothing is read through the read-only path (__ldg): such
+// loads may be moved ahead of the wait.
 __device__ __forceinline__ int seq_len(const Params& p, int b) {
-  const int L = __ldg(p.seqlens + b);
+  const int L = p.seqlens[b];
   return min(max(L, 0), p.Lmax);
 }
 
@@ -218,7 +221,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) attend_kernel(const Params p)
     if (t >= ld.t1) return -1;
     if (p.block_table == nullptr) return ld.b * p.Lmax + t;
     const int pg = p.page.div(t);
-    const int page = __ldg(p.block_table + (size_t)ld.b * p.max_blocks + pg);
+    const int page = p.block_table[(size_t)ld.b * p.max_blocks + pg];
     if (page < 0 || page >= p.num_blocks) return -1;
     return page * p.block_size + (t - pg * p.block_size);
   };
@@ -260,8 +263,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) attend_kernel(const Params p)
       const E* qrow = static_cast<const E*>(p.q) + (size_t)b * p.q_stride + ((size_t)h * G + hh) * D;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        qf[nt][ks][0] = hh < G ? __ldg(reinterpret_cast<const uint32_t*>(qrow + 16 * ks + 2 * c)) : 0u;
-        qf[nt][ks][1] = hh < G ? __ldg(reinterpret_cast<const uint32_t*>(qrow + 16 * ks + 8 + 2 * c)) : 0u;
+        qf[nt][ks][0] = hh < G ? *reinterpret_cast<const uint32_t*>(qrow + 16 * ks + 2 * c) : 0u;
+        qf[nt][ks][1] = hh < G ? *reinterpret_cast<const uint32_t*>(qrow + 16 * ks + 8 + 2 * c) : 0u;
       }
     }
     float o[NT][KS][4];
@@ -427,7 +430,7 @@ __device__ __forceinline__ float merge_lse(const float* src, size_t plane, int n
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int s = s0 + u * 32 + lane;
-      x[u] = s < n ? __ldg(src + s * plane) : -INFINITY;
+      x[u] = s < n ? src[s * plane] : -INFINITY;
     }
     // fmaxf passes over NaN, the sum does not.
     const float top = fmaxf(fmaxf(M, fmaxf(x[0], x[1])), fmaxf(x[2], x[3]));
@@ -519,13 +522,13 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const __grid_con
         for (int u = 0; u < CH; ++u) {
           const int s = s0 + u * wpr;
           const bool in = s < n;
-          ls[u] = in ? __ldg(p.lse_part + s * plane + row) : -INFINITY;
+          ls[u] = in ? p.lse_part[s * plane + row] : -INFINITY;
           const float* src = p.o_part + (s * plane + row) * D + PER * lane;
           if constexpr (PER == 4) {
-            const float4 f = in ? __ldg(reinterpret_cast<const float4*>(src)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            const float4 f = in ? *reinterpret_cast<const float4*>(src) : make_float4(0.f, 0.f, 0.f, 0.f);
             v[u][0] = f.x, v[u][1] = f.y, v[u][2] = f.z, v[u][3] = f.w;
           } else {
-            const float2 f = in ? __ldg(reinterpret_cast<const float2*>(src)) : make_float2(0.f, 0.f);
+            const float2 f = in ? *reinterpret_cast<const float2*>(src) : make_float2(0.f, 0.f);
             v[u][0] = f.x, v[u][1] = f.y;
           }
         }
