@@ -35,6 +35,7 @@
 #include <cooperative_groups.h>
 
 #include "common.cuh"
+#include "evict_key.cuh"
 #include "fk_b200.h"
 
 namespace fk {
@@ -89,19 +90,14 @@ __device__ __forceinline__ int seq_len(const Params& p, int b) {
   return min(max(L, 0), p.Lmax);
 }
 
-// Order-preserving key: -inf < ... < -0 = +0 < ... < +inf < NaN.
-__device__ __forceinline__ uint32_t mass_key(float f) {
-  if (f != f) return 0xFFFFFFFFu;
-  const uint32_t u = __float_as_uint(f + 0.f);  // -0 + 0 = +0
-  return (u & 0x80000000u) ? ~u : u | 0x80000000u;
-}
+__device__ __forceinline__ uint32_t mass_key(float f) { return key_of_bits(__float_as_uint(f + 0.f)); }  // -0 + 0 = +0
 
 // KEYS: keys per lane kept in registers; 0: any number, read again from memory in every pass.
 template <int KEYS>
 __global__ void __launch_bounds__(kThreads, 1) select_kernel(const Params p) {
   __shared__ int s_hist[2][kBins];  // this CTA's counts, double-buffered over the passes
-  __shared__ uint32_t s_min[kWarps], s_max[kWarps];
-  __shared__ uint32_t s_range[2];   // this CTA's least and greatest key
+  __shared__ uint32_t s_below[kWarps], s_greatest[kWarps];
+  __shared__ uint32_t s_range[2];   // this CTA's KeyRange
   __shared__ int s_warp[kWarps];    // sums of the scan
   __shared__ int s_bin, s_above, s_count;
   __shared__ int s_gt[kWarps], s_tie[kWarps];
@@ -148,14 +144,13 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const Params p) {
   const int seg = ((((m + 31) >> 5) + cl * kWarps - 1) >> (p.cl_log + 5)) << 5;
   const int w0 = min(gw * seg, m), w1 = min(w0 + seg, m);
   mass += first;
-  // Keys of places past the stretch are 0, below every mass (the key of -inf is 0x007FFFFF).
   uint32_t reg[KEYS > 0 ? KEYS : 1];
   if constexpr (KEYS > 0) {
     float f[KEYS];
 #pragma unroll
     for (int u = 0; u < KEYS; ++u) f[u] = w0 + u * 32 + lane < w1 ? load_now(mass + w0 + u * 32 + lane) : 0.f;
 #pragma unroll
-    for (int u = 0; u < KEYS; ++u) reg[u] = w0 + u * 32 + lane < w1 ? mass_key(f[u]) : 0u;
+    for (int u = 0; u < KEYS; ++u) reg[u] = w0 + u * 32 + lane < w1 ? mass_key(f[u]) : kNoKey;
   }
   // Calls f(key, index) for this lane's candidates, in order, whole warps at a time.
   auto each = [&](auto f) {
@@ -165,7 +160,7 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const Params p) {
     } else {
       for (int i0 = w0; i0 < w1; i0 += 32) {
         const int i = i0 + lane;
-        f(i < w1 ? mass_key(load_now(mass + i)) : 0u, i);
+        f(i < w1 ? mass_key(load_now(mass + i)) : kNoKey, i);
       }
     }
   };
@@ -174,36 +169,37 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const Params p) {
   };
 
   // ---- the keys' range ----
-  uint32_t lo = 0xFFFFFFFFu, hi = 0u;
-  each([&](uint32_t key, int) {
-    lo = min(lo, key - 1);  // 0 wraps to the greatest
-    hi = max(hi, key);
-  });
-  lo += 1;
-  lo = __reduce_min_sync(0xffffffffu, lo);
-  hi = __reduce_max_sync(0xffffffffu, hi);
+  KeyRange range;
+  each([&](uint32_t key, int) { range.add(key); });
+  auto over_warp = [](KeyRange r) {
+    r.below = __reduce_min_sync(0xffffffffu, r.below);
+    r.greatest = __reduce_max_sync(0xffffffffu, r.greatest);
+    return r;
+  };
+  range = over_warp(range);
   if (lane == 0) {
-    s_min[warp] = lo;
-    s_max[warp] = hi;
+    s_below[warp] = range.below;
+    s_greatest[warp] = range.greatest;
   }
   s_hist[0][threadIdx.x] = 0;
   __syncthreads();
   if (warp == 0) {
-    lo = __reduce_min_sync(0xffffffffu, s_min[lane]);
-    hi = __reduce_max_sync(0xffffffffu, s_max[lane]);
+    range.below = s_below[lane];
+    range.greatest = s_greatest[lane];
+    range = over_warp(range);
     if (lane == 0) {
-      s_range[0] = lo;
-      s_range[1] = hi;
+      s_range[0] = range.below;
+      s_range[1] = range.greatest;
     }
   }
   sync_all();
-  lo = s_range[0];
-  hi = s_range[1];
+  range.below = s_range[0];
+  range.greatest = s_range[1];
   for (int q = 0; q < cl && cl > 1; ++q) {
     const uint32_t* r = cluster.map_shared_rank(s_range, q);
-    lo = min(lo, r[0]);
-    hi = max(hi, r[1]);
+    range.join(r[0], r[1]);
   }
+  uint32_t lo = range.least(), hi = range.greatest;
 
   // ---- narrow [lo, lo + 2^width) to the want-th greatest key ----
   int width = 32 - __clz(hi - lo);  // bits of the interval
@@ -213,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, 1) select_kernel(const Params p) {
     const int shift = max(0, width - kBinBits);
     int* hist = s_hist[pass & 1];
     each([&](uint32_t key, int) {
-      const uint32_t d = key - lo;  // wraps to a great number below the interval
+      const uint32_t d = key - lo;  // wraps to a great number below the interval, kNoKey's place
       if (d <= hi - lo) atomicAdd(&hist[d >> shift], 1);
     });
     sync_all();
