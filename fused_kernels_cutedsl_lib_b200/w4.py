@@ -123,10 +123,11 @@ def quantize_w4(w: torch.Tensor, group_size: int = 128, symmetric: bool = False,
     Asymmetric: the codes span the group's [min(w, 0), max(w, 0)], with a zero point.
     ``symmetric``: scale ``max |w| / 7``, zero point 8. ``dtype`` (default: the
     weight's, bf16 for fp32 weights) is the type of the scales and of the activations.
+    Weights that are not finite, or whose scales are not in that type, are refused.
     """
     if not isinstance(w, torch.Tensor) or w.dtype not in (torch.bfloat16, torch.float16, torch.float32):
         raise TypeError("w must be a bfloat16, float16 or float32 tensor")
-    if w.dim() != 2:
+    if w.dim() != 2 or w.shape[0] < 1 or w.shape[1] < 1:
         raise ValueError(f"w must be [N, K], got {tuple(w.shape)}")
     if group_size not in GROUP_SIZES or w.shape[1] % group_size:
         raise ValueError(f"group_size must be one of {GROUP_SIZES} and divide K={w.shape[1]}, got {group_size}")
@@ -142,6 +143,8 @@ def quantize_w4(w: torch.Tensor, group_size: int = 128, symmetric: bool = False,
         sf = scales.float()
         zeros = torch.where(sf > 0, (-lo / sf.clamp_min(1e-30)).round().clamp_(0, 15), 0.0).to(torch.uint8)
         z = zeros.float()[..., None]
+    if not bool(torch.isfinite(scales).all()):  # of a NaN or infinite weight as well
+        raise ValueError(f"w has an element that is not finite, or whose scale is not finite in {dt}")
     sf = scales.float()[..., None]
     q = torch.where(sf > 0, (v / sf.clamp_min(1e-30) + z).round().clamp_(0, 15), z if zeros is not None else 8.0)
     return pack_w4(q.to(torch.uint8).view(w.shape), scales, zeros)
