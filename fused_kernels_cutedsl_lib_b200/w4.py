@@ -141,12 +141,12 @@ def quantize_w4(w: torch.Tensor, group_size: int = 128, symmetric: bool = False,
         lo, hi = v.amin(-1).clamp_max(0.0), v.amax(-1).clamp_min(0.0)
         scales = ((hi - lo) / 15.0).to(dt)
         sf = scales.float()
-        zeros = torch.where(sf > 0, (-lo / sf.clamp_min(1e-30)).round().clamp_(0, 15), 0.0).to(torch.uint8)
+        zeros = torch.where(sf > 0, (-lo / torch.where(sf > 0, sf, 1.0)).round().clamp_(0, 15), 0.0).to(torch.uint8)
         z = zeros.float()[..., None]
     if not bool(torch.isfinite(scales).all()):  # of a NaN or infinite weight as well
         raise ValueError(f"w has an element that is not finite, or whose scale is not finite in {dt}")
     sf = scales.float()[..., None]
-    q = torch.where(sf > 0, (v / sf.clamp_min(1e-30) + z).round().clamp_(0, 15), z if zeros is not None else 8.0)
+    q = torch.where(sf > 0, (v / torch.where(sf > 0, sf, 1.0) + z).round().clamp_(0, 15), z if zeros is not None else 8.0)
     return pack_w4(q.to(torch.uint8).view(w.shape), scales, zeros)
 
 
