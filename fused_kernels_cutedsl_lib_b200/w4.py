@@ -35,6 +35,20 @@ class W4Weight:
     group_size: int
     dtype: torch.dtype    # of the scales, the activations and the output
 
+    def __post_init__(self):
+        # The kernels take the sizes on trust: a buffer that is shorter would be read past its end.
+        if not isinstance(self.packed, torch.Tensor) or self.packed.dtype != torch.int32:
+            raise TypeError("packed must be an int32 tensor")
+        if self.dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError(f"dtype must be bfloat16 or float16, got {self.dtype}")
+        if self.group_size not in GROUP_SIZES or self.n < 1 or self.k < 1 or self.k % self.group_size:
+            raise ValueError(f"group size must be one of {GROUP_SIZES} and divide K, got {self.group_size} for "
+                             f"[{self.n}, {self.k}]")
+        words = -(-self.n // 16) * -(-self.k // _BLOCK_K) * (256 + 2048 // self.group_size)
+        if not self.packed.is_contiguous() or self.packed.numel() != words:
+            raise ValueError(f"packed must hold {words} contiguous words for [{self.n}, {self.k}] and groups of "
+                             f"{self.group_size}, got shape {tuple(self.packed.shape)}")
+
     def nbytes(self) -> int:
         return self.packed.numel() * 4
 
