@@ -617,14 +617,22 @@ extern "C" int fk_w4_linear(const void* x, long long ldx, const void* packed, co
   int* err = device_error_word();
   if (!err) return fail(kErrCuda, "device error word unavailable");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // The form of w4_tc.cu for more than 16 tokens, and from 9 on unless its tiles of 128 rows are one to 1.6 to an
-  // SM: the second wave then leaves most SMs idle. For 16 tokens it took, against the form of this file (groups of
-  // 128): 4.1 / 5.1 us on 1024 x 2048, 7.0 / 8.3 on 4096 x 4096, 13.2 / 21.9 on 4096 x 14336, 14.6 / 19.4 on
-  // 18944 x 4096, 27.2 / 26.0 on 28672 x 4096 (1.5 tiles per SM), 29.1 / 31.6 on 37888 x 4096, 53.4 / 59.4 on 57344
-  // x 4096. For 8 tokens, where this form does half the products: 7.0 / 6.1 on 4096 x 4096, 13.2 / 14.1 on 4096 x
-  // 14336, 27.1 / 19.0 on 28672 x 4096.
+  // The form of w4_tc.cu for more than 16 tokens; for 9 to 16 where its tiles of 128 rows are one wave on the SMs, or
+  // so many that this form, which goes through its rows in rounds, is slower than its part-filled last wave.
+  // For 16 tokens of 4096 inputs it took, against the form of this file, in us with groups of 128 / 64 / 32 and
+  // weights that do not lie in L2:
+  //   16384 rows (0.9 tiles per SM)  15.4 : 17.1   16.9 : 18.5   18.0 : 21.6
+  //   33024 (1.7)                    30.6 : 28.8   33.4 : 31.4   35.6 : 37.9
+  //   37888 (2.0)                    31.4 : 32.6   34.1 : 35.5   36.5 : 47.1
+  //   40960 (2.2)                    43.9 : 34.4   48.0 : 37.8   51.3 : 49.6
+  //   49152 (2.6)                    45.2 : 44.3   49.5 : 48.2   52.9 : 66.9
+  //   53248 (2.8)                    45.9 : 47.9   50.0 : 62.4   53.5 : 85.1
+  //   57344 (3.0)                    58.0 : 60.7   63.6 : 75.5   68.2 : 87.3
+  // (fp16, groups of 128: 31.9 : 30.0 at 2.0, 45.8 : 41.3 at 2.6, 46.7 : 44.6 at 2.8, 59.9 : 69.6 at 3.2.) For 8 tokens,
+  // where this form does half the products: 7.0 : 6.1 on 4096 x 4096, 13.2 : 14.1 on 4096 x 14336, 27.1 : 19.0 on
+  // 28672 x 4096.
   const int tiles = (N + 127) / 128, sms = num_sms();
-  if (M > 16 || (M > 8 && (tiles <= sms || 5 * tiles > 8 * sms))) {
+  if (M > 16 || (M > 8 && (tiles <= sms || 5 * tiles > (group_size == 32 ? 8 : 13) * sms))) {
     const w4::Call c{x, ldx, static_cast<const uint8_t*>(packed), residual, y, err, dtype == FK_BF16, M, N, K, group_size,
                     w4::g_withhold};
     return w4::linear_tc(c, st);
