@@ -30,10 +30,10 @@
 // splits of each (row, q head) into out and lse, and blocks that turn a stretch
 // of scores into weights and add them to the mass.
 //
-// Measured, 8 kv heads of 128 dims, 4 q heads each: 64 ragged rows of up to 32768 tokens (4.5 GB)
-// 683 us without masses, 0.99 of a plain copy's rate, and 758 to 772 with them, 59 of them
-// in pass 2. Small calls are two launches and a join: 6.5 us for one row of 1000 tokens,
-// 18 for four of 4096 (pass 1 12, pass 2 5).
+// Measured, 8 kv heads of 128 dims, 4 q heads each, caches from memory: 64 ragged rows of up to 32768 tokens
+// (4.5 GB) 683 to 690 us without masses, a plain copy's rate, and 767 to 777 with them, 84 of them in pass 2.
+// Small calls are two launches and a join: 7.5 us for one row of 1000 tokens, 18 for four of 4096 (pass
+// 1 12, pass 2 5).
 //
 // A row of length 0 gives out = 0, lse = -inf and leaves its mass. A page id
 // outside the pool reads as zero rows, as a TMA load outside its tensor does.

@@ -31,7 +31,8 @@
 //
 // Measured, 8 kv heads of 128 dims: 32 ragged rows of up to 32768 tokens to 4096 213 us, 47 the
 // selection and 166 the copy, at a plain copy's rate (the copy in the selection's
-// kernel was slower: its CTAs are few). One row of 32768 to 2048 19.6 us: the passes' barriers.
+// kernel was slower: its CTAs are few). One row of 32768 to 2048 19.2 us, 18.7 without masses of 0 (one value
+// for a tenth of the tokens): the passes' barriers.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -362,10 +363,10 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const Params p, 
 }
 
 static int launch(Params p, cudaStream_t st) {
-  // CTAs per (row, head): enough that the pairs fill the SMs, as long as each warp
-  // still has 32 candidates of the longest row; and enough that a lane's keys fit 32 registers (at
-  // 32 rows of up to 32768 tokens one CTA with 32 keys per lane measured 47 us, two with 16 each 55:
-  // a pass is latency, and a cluster's barrier costs more than a CTA's).
+  // CTAs per (row, head): doubled while the pairs do not fill the SMs and the CTAs so far have fewer lanes than the
+  // longest row has tokens, so that each warp has at least 16 candidates of it; and until a lane's keys
+  // fit 32 registers (at 32 rows of up to 32768 tokens one CTA with 32 keys per lane measured 47 us, two with 16
+  // each 55: a pass is latency, and a cluster's barrier costs more than a CTA's).
   p.cl_log = 0;
   while ((1 << p.cl_log) < kMaxCluster && p.Lmax > (kThreads << p.cl_log) &&
          (((long long)p.B * p.Hkv << p.cl_log) < num_sms() || p.Lmax > (32 * kThreads << p.cl_log)))

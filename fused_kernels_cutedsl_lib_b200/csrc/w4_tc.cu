@@ -2,14 +2,14 @@
 //   y[m, n] = sum_k x[m, k] * (q[n, k] - z[n, k / g]) * s[n, k / g]  (+ residual[m, n])
 // (the layout of the weight, the form for fewer tokens and the choice are in w4_linear.cu).
 //
-// Bound: up to 64 tokens share one pass over the weight. At 6.5 TB/s an SM gets 46 weights
-// a clock, and expanding them to 16 bits (below) keeps its ALU pipe, 64 lanes a clock,
-// busy for about as long; the products themselves are a small load for tcgen05. Measured on
-// 4096 outputs of 14336 inputs, groups of 128: 13.2 us for 16 or 32 tokens, 16.3 us for 64
-// (mma.sync, with 32 products and 16 shared-memory reads per KB of weight at 32 tokens:
-// 61 us for 64); 28672 of 4096: 28.1 and 34.9 us. This package's 16-bit linear
-// (skinny_gemm) takes 23.7, 24.8 and 26.9 us for 32, 64 and 128 tokens on 4096 x 14336: from
-// 65 tokens on, two passes, this form saves memory, not time.
+// Up to 64 tokens share one pass over the weight, 32 with groups of 32 (the accumulators of a block's four
+// groups fill the columns). What bounds it is the latency of its stages: 0.45 instructions per cycle and
+// scheduler, tcgen05 16 % busy, DRAM 16 % (64 tokens, groups of 64, 4096 x 14336); past one wave of tiles also
+// the part-filled last one. Measured on weights that do not lie in L2, groups of 128: 4096 outputs of 14336
+// inputs 14.1 us for 16 tokens, 14.4 for 32, 17.5 for 64 (mma.sync, with 32 products and 16 shared-memory reads
+// per KB of weight at 32 tokens: 61 us for 64); 28672 of 4096: 30.6 and 38.4 us for 32 and 64. This
+// package's 16-bit linear (skinny_gemm) takes 24.0, 25.2 and 26.8 us for 32, 64 and 128 tokens on 4096 x 14336:
+// from 65 tokens on, two passes, this form saves memory, not time.
 //
 // One CTA: 128 output rows, a slice of the inputs, N tokens (32 or 64). Per slab of 256
 // inputs
@@ -26,7 +26,7 @@
 //   * warps 16-23 (thread = row and half of the tokens) read D and add s * D to their fp32
 //     sums. Integers and x are exact, so the only roundings are those of fp32 sums and
 //     the output.
-// Earlier steps, 64 tokens on 4096 x 14336: 27.5 us with the expanding warps adding up too,
+// Earlier steps, 64 tokens on 4096 x 14336, part of the weight from L2: 27.5 us with the expanding warps adding up too,
 // 20.4 with warps of their own for it, 19.0 with addresses carried along, 17.9 with one
 // logic instruction per pair. CTAs that go on to the next tile of rows instead of leaving:
 // 15.6 for 32 tokens instead of 13.3, no gain elsewhere.

@@ -168,7 +168,7 @@ def w4_linear(x, weight: W4Weight, out=None, *, residual=None, stream=None):
     """``out = x @ W.t() (+ residual)`` for a 4-bit weight; returns ``out``.
 
     ``x`` [M, K] in the weight's dtype, any M (made for decode batches: up to 64
-    tokens share one pass over the weight), rows may be strided (a multiple of 8
+    tokens share one pass over the weight, 32 with groups of 32), rows may be strided (a multiple of 8
     elements); ``out`` and ``residual`` [M, N] dense, ``residual`` may be ``out``.
     Otherwise ``out`` shares no memory with ``x``, ``residual`` or the weight. An ``out`` left to the call
     is memory of the stream it runs on (``stream``, or torch's current one).
