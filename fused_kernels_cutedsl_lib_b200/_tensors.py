@@ -145,3 +145,13 @@ def empty_on(shape, dtype: torch.dtype, idx: int, stream_handle: int) -> torch.T
         return torch.empty(shape, dtype=dtype, device=dev)
     with torch.cuda.stream(torch.cuda.ExternalStream(stream_handle, device=dev)):
         return torch.empty(shape, dtype=dtype, device=dev)
+
+
+def result_on(shape, dtype: torch.dtype, dev: torch.device, stream=None) -> torch.Tensor:
+    """:func:`empty_on` for a call on ``dev`` with the given ``stream`` argument (None: torch's current one)."""
+    idx = dev.index if dev.index is not None else torch.cuda.current_device()
+    if stream is None:
+        handle = raw_current_stream(idx)
+    else:
+        handle = stream.cuda_stream if isinstance(stream, torch.cuda.Stream) else int(stream)
+    return empty_on(shape, dtype, idx, handle)

@@ -31,7 +31,7 @@ import threading
 import torch
 
 from . import _native
-from ._tensors import ptr, require_tensor, same_device, stream_for
+from ._tensors import ptr, require_tensor, result_on, same_device, stream_for
 
 FLAG_SWIGLU = 1
 _ws_lock = threading.Lock()
@@ -96,7 +96,7 @@ def linear(x, w, out=None, *, gamma=None, eps: float = 1e-6, w_up=None, up_row_o
         raise ValueError(f"w must have N={N} rows, got {w.shape[0]}")
     dev = x.device
     if out is None:
-        out = torch.empty((M, N), dtype=torch.bfloat16, device=dev)
+        out = result_on((M, N), torch.bfloat16, dev, stream)
     _check_out(out, M, N)
     if gamma is not None:
         require_tensor("gamma", gamma, torch.bfloat16, 1)
@@ -135,8 +135,6 @@ def swiglu_gemm(x, w_gate_up, out=None, *, gamma=None, eps: float = 1e-6, worksp
     if w_gate_up.shape[0] % 2:
         raise ValueError("w_gate_up must have an even number of rows [2N, K]")
     n = w_gate_up.shape[0] // 2
-    if out is None:
-        out = torch.empty((x.shape[0], n), dtype=torch.bfloat16, device=x.device)
     return linear(x, w_gate_up, out, gamma=gamma, eps=eps, w_up=w_gate_up, up_row_offset=n,
                   workspace=workspace, stream=stream)
 
@@ -180,7 +178,7 @@ def lora_linear(x, w, lora_b, out=None, *, lora_a=None, lora_xa=None, residual=N
         raise ValueError(f"lora_xa must be [{M}, {r}], got {tuple(lora_xa.shape)}")
     dev = x.device
     if out is None:
-        out = torch.empty((M, N), dtype=torch.bfloat16, device=dev)
+        out = result_on((M, N), torch.bfloat16, dev, stream)
     _check_out(out, M, N)
     if residual is not None:
         _check_out(residual, M, N, "residual")

@@ -20,7 +20,7 @@ import math
 import torch
 
 from . import _native
-from ._tensors import ptr, require_tensor, same_device, stream_for
+from ._tensors import ptr, require_tensor, result_on, same_device, stream_for
 
 
 def flash_attention(q, k, v, out=None, *, softmax_scale=None, lse=None, return_lse=False, stream=None):
@@ -44,12 +44,12 @@ def flash_attention(q, k, v, out=None, *, softmax_scale=None, lse=None, return_l
     if D not in (64, 128):
         raise ValueError(f"head_dim must be 64 or 128, got {D}")
     if out is None:
-        out = torch.empty_like(q)
+        out = result_on(q.shape, q.dtype, q.device, stream)
     require_tensor("out", out, torch.bfloat16, 4)
     if tuple(out.shape) != tuple(q.shape):
         raise ValueError(f"out must have shape {tuple(q.shape)}, got {tuple(out.shape)}")
     if lse is None and return_lse:
-        lse = torch.empty(B, Hq, Lq, dtype=torch.float32, device=q.device)
+        lse = result_on((B, Hq, Lq), torch.float32, q.device, stream)
     if lse is not None:
         require_tensor("lse", lse, torch.float32, 3)
         if tuple(lse.shape) != (B, Hq, Lq):

@@ -2,7 +2,16 @@
 import pytest
 import torch
 
-from fused_kernels_cutedsl_lib_b200 import cache_attention, cache_evict, pack_w4, w4_linear
+from fused_kernels_cutedsl_lib_b200 import (
+    cache_attention,
+    cache_evict,
+    flash_attention,
+    linear,
+    lora_linear,
+    pack_w4,
+    swiglu_gemm,
+    w4_linear,
+)
 
 pytestmark = pytest.mark.gpu
 
@@ -83,3 +92,22 @@ def test_no_rows():
     lens, mass = torch.empty(0, dtype=torch.int32, device="cuda"), torch.empty(0, 2, 8, device="cuda")
     out, lse = cache_attention(q, k, k, lens, mass=mass)
     assert out.shape == (0, 4, 64) and lse.shape == (0, 4)
+
+
+def test_linear_family_and_prefill_attention():
+    x = torch.randn(64, 256, device="cuda").to(BF16)
+    w = (0.05 * torch.randn(20000, 256, device="cuda")).to(BF16)
+    a, b = torch.randn(16, 256, device="cuda").to(BF16), torch.randn(20000, 16, device="cuda").to(BF16)
+    q = torch.randn(2, 8, 1024, 128, device="cuda").to(BF16)
+    k = torch.randn(2, 2, 1024, 128, device="cuda").to(BF16)
+    for shape, call in (((64, 20000), lambda s: linear(x, w, stream=s)),
+                        ((64, 10000), lambda s: swiglu_gemm(x, w, stream=s)),
+                        ((64, 20000), lambda s: lora_linear(x, w, b, lora_a=a, stream=s)),
+                        (tuple(q.shape), lambda s: flash_attention(q, k, k, stream=s))):
+        want = call(None)
+        assert torch.equal(check_pending_copy(shape, BF16, call), want)
+    lse_shape = (2, 8, 1024)
+    out = torch.empty_like(q)
+    want = flash_attention(q, k, k, out, return_lse=True)[1]
+    got = check_pending_copy(lse_shape, torch.float32, lambda s: flash_attention(q, k, k, out, return_lse=True, stream=s))
+    assert torch.equal(got[1], want)
